@@ -544,6 +544,61 @@ int mc_rank_runs_debug_groups(const void *workspace, uint64_t n, uint64_t *out, 
 int mc_rank_query(const double *keys_sorted, const double *positions, uint64_t n, const double *x, uint64_t t,
                   double *out_pos, uint64_t *out_cnt, void *stream);
 
+/* ---- a language model's logits --------------------------------------------------------------------------------
+ * The same path for a model that answers with logits instead of tables (a neural character or sub-word model run by the
+ * caller): what calc_ml2p, sample1 / pick_expand and the sum over a password (lib4mc/MonteCarloParent.py:17-31,
+ * lib4mc/ProbLib.py:31-43, nwords_simulator.py:92-116) are on a row of logits x over V tokens, p = softmax(x / T).  No
+ * counterpart in the reference, whose models are tables; units and conventions are those of the calls above (bits,
+ * draws by inversion, 1022.0 for what is impossible).
+ *
+ * Rows: logits[o][i][0..vocab) of MC_LOGITS_F32 / _F16 / _BF16, row o * inner + i at o * outer_stride + i * inner_stride
+ * ELEMENTS, consecutive tokens adjacent; any strides (a slice of a longer sequence, rows that overlap or repeat), any
+ * alignment of the element's own.  Tokens and weights come with strides of their own for the same (outer, inner); outputs
+ * are contiguous [outer * inner].  Sums are held in 32 bits (the draw decides in 64).  All calls are asynchronous on
+ * `stream`, allocate nothing and may be captured into a graph.  Temperatures 1e-30 .. 1e30.
+ *   token ids   0 .. vocab - 1; MC_TOKEN_SKIP: the row is not read (padding), its outputs are 0; anything else is a token
+ *               outside the model, as MC_TOKEN_OUTSIDE: impossible (+inf)
+ *   -inf        a token switched off: probability 0.  A row with nothing left: ml2p +inf, entropy 0, no alternatives, no
+ *               draw, gradient 0.  Finite logits of any size are numbers (a row of the type's lowest value is uniform)
+ *   NaN, +inf   a row that holds one answers NaN (alternatives and draws: MC_TOKEN_OUTSIDE) */
+enum { MC_LOGITS_F32 = 0, MC_LOGITS_F16 = 1, MC_LOGITS_BF16 = 2 };
+#define MC_TOKEN_OUTSIDE (-1)
+#define MC_TOKEN_SKIP (-2)
+#define MC_LOGITS_MAX_TOP 64
+/* out_ml2p = -log2 p of the given token, out_entropy (may be NULL) = the row's entropy in bits, and with top > 0 the
+ * `top` most probable tokens (<= MC_LOGITS_MAX_TOP and <= vocab) in descending order, equal logits by the lower id:
+ * out_top[rows][top] and their -log2 p out_top_ml2p[rows][top]; where fewer have any probability the rest is
+ * MC_TOKEN_OUTSIDE / +inf, in a skipped row MC_TOKEN_SKIP / 0. */
+int mc_logits_score(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
+                    int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
+                    int64_t token_outer_stride, int64_t token_inner_stride, double temperature, float *out_ml2p,
+                    float *out_entropy, uint32_t top, int32_t *out_top, float *out_top_ml2p, void *stream);
+/* out_grad[rows][vocab] (contiguous, the logits' type, one rounding) = the gradient of
+ *     sum over rows of weights[r] * ml2p[r] + entropy_weights[r] * entropy[r]
+ * (entropy_weights may be NULL) for the logits, with ml2p and entropy (may be NULL) as mc_logits_score gives them.  Skipped
+ * rows and rows with nothing left have gradient 0; where the token is outside the model weights[r] is not read.
+ * out_grad may be the logits themselves when those are contiguous; it must not overlap them otherwise. */
+int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
+                       int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
+                       int64_t token_outer_stride, int64_t token_inner_stride, double temperature,
+                       const float *weights, int64_t weight_outer_stride, int64_t weight_inner_stride,
+                       const float *entropy_weights, int64_t entropy_outer_stride, int64_t entropy_inner_stride,
+                       float *out_ml2p, float *out_entropy, void *out_grad, void *stream);
+/* One draw from every row by inversion, as pick_expand: the first token whose running sum C_i of exp((x_i - max x) / T)
+ * exceeds u * C_(vocab-1), decided as sums in 64 bits decide it; out_token and its out_ml2p.  u = uniforms[row] in
+ * [0, 1) (below: 0, above: the last token with any probability, NaN: 0), or, with uniforms NULL, the uniform
+ * (seed, first_id + row, draw) of the stream mc_sample uses.  live (may be NULL): rows whose byte is 0 are not read
+ * (samples that have ended): MC_TOKEN_SKIP, 0. */
+int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows, uint64_t vocab, int64_t row_stride,
+                   double temperature, const double *uniforms, uint64_t seed, uint64_t first_id, uint32_t draw,
+                   const uint8_t *live, int32_t *out_token, float *out_ml2p, void *stream);
+/* -log2 p of whole passwords, the keys of mc_rank_build: the sum in 64 bits of a password's ml2p; 1022.0 where one of
+ * them is +inf (as mc_score), 0.0 for no symbols.  Packed: password t is ml2p[offsets[t] .. offsets[t+1]) of `longest`
+ * values in all (a pair of offsets that does not ascend within them names nothing).  Padded (offsets NULL):
+ * ml2p[t * stride + 0 .. lengths[t]), lengths of 4 or 8 bytes cut to 0 .. longest, or NULL: `longest` each. */
+int mc_logits_keys(const float *ml2p, const int64_t *offsets, const void *lengths, uint32_t length_bytes,
+                   uint64_t count, int64_t stride, uint64_t longest, double *out_keys, void *stream);
+
 /* ---- sharded estimation: the one collective of the path -------------------------------------------*/
 /* SURVEY.md §8(b)/(e).  The reference is single-process and has no counterpart; what is summed is the
  * `positions[idx - 1]` of ml2p2rank (lib4mc/MonteCarloLib.py:31-32) when every rank holds a shard of the

@@ -74,6 +74,13 @@ def _load() -> C.CDLL:
     sig = {
         "mc_abi_version": (C.c_int, []),
         "mc_last_error": (C.c_char_p, []),
+        "mc_logits_score": (C.c_int, [vp, C.c_uint32] + [C.c_uint64] * 3 + [C.c_int64] * 2 + [vp, C.c_uint32] + [C.c_int64] * 2
+                            + [C.c_double, vp, vp, C.c_uint32, vp, vp, vp]),
+        "mc_logits_gradient": (C.c_int, [vp, C.c_uint32] + [C.c_uint64] * 3 + [C.c_int64] * 2 + [vp, C.c_uint32]
+                               + [C.c_int64] * 2 + [C.c_double] + [vp, C.c_int64, C.c_int64] * 2 + [vp] * 4),
+        "mc_logits_draw": (C.c_int, [vp, C.c_uint32, C.c_uint64, C.c_uint64, C.c_int64, C.c_double, vp, C.c_uint64,
+                                     C.c_uint64, C.c_uint32, vp, vp, vp, vp]),
+        "mc_logits_keys": (C.c_int, [vp, vp, vp, C.c_uint32, C.c_uint64, C.c_int64, C.c_uint64, vp, vp]),
         "mc_table_compile": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(vp)]),
         "mc_table_free": (None, [vp]),
         "mc_table_array": (C.c_int64, [vp, C.c_int, vp, C.c_size_t]),
@@ -201,7 +208,8 @@ EXPORTS = ["mc_abi_version", "mc_last_error", "mc_table_compile", "mc_table_free
            "mc_enum_free", "mc_rank_runs_workspace_bytes", "mc_rank_runs_capacity", "mc_rank_runs_max_keys", "mc_rank_runs_build",
            "mc_rank_runs_forget", "mc_rank_runs_check", "mc_rank_runs_query", "mc_rank_runs_expand", "mc_rank_runs_debug_phases",
            "mc_score_words_debug_kernel", "mc_score_bpe_debug_kernel",
-           "mc_rank_runs_debug_groups", "mc_rank_runs_guess_numbers"]
+           "mc_rank_runs_debug_groups", "mc_rank_runs_guess_numbers", "mc_logits_score", "mc_logits_gradient", "mc_logits_draw",
+           "mc_logits_keys"]
 
 
 def check(rc: int) -> int:

@@ -21,6 +21,7 @@
 #include <new>
 
 #include "mc_internal.h"
+#include "mc_philox.h"
 
 #define HIP_TRY(expr)                                                                        \
     do {                                                                                     \
@@ -115,30 +116,6 @@ __device__ __forceinline__ void carry_copy(const uint4 *__restrict__ src, uint4 
         for (int u = 0; u < U; ++u) dst[i + u * stride] = v[u];
     }
     for (; i < n16; i += stride) dst[i] = src[i];
-}
-
-constexpr uint32_t PH_M0 = 0xD2511F53u, PH_M1 = 0xCD9E8D57u, PH_W0 = 0x9E3779B9u, PH_W1 = 0xBB67AE85u;
-
-// Philox4x32-10; same bits as oracle/philox.py
-__device__ __forceinline__ void philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0,
-                                               uint32_t k1, uint32_t &o0, uint32_t &o1, uint32_t &o2, uint32_t &o3) {
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const unsigned long long p0 = (unsigned long long)PH_M0 * c0, p1 = (unsigned long long)PH_M1 * c2;
-        const uint32_t hi0 = (uint32_t)(p0 >> 32), lo0 = (uint32_t)p0;
-        const uint32_t hi1 = (uint32_t)(p1 >> 32), lo1 = (uint32_t)p1;
-        uint32_t n0 = hi1 ^ c1 ^ k0, n2 = hi0 ^ c3 ^ k1;
-        c0 = n0;
-        c1 = lo1;
-        c2 = n2;
-        c3 = lo0;
-        k0 += PH_W0;
-        k1 += PH_W1;
-    }
-    o0 = c0;
-    o1 = c1;
-    o2 = c2;
-    o3 = c3;
 }
 
 struct alignas(16) DrawRec {

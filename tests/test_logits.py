@@ -1,0 +1,103 @@
+"""The operators on logits without a GPU: the definitions against differences, and what the C ABI refuses."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from montecarlo_amd import _native as nv
+from montecarlo_amd import logits as lg
+from tests.logits_ref import OUTSIDE, SKIP, Row
+
+
+@pytest.mark.parametrize("vocab,temperature,tok", [(1, 1.0, 0), (5, 0.7, 3), (17, 1.6, 0), (17, 1.0, OUTSIDE), (6, 1.0, SKIP)])
+def test_gradient_formula_is_the_differences(vocab, temperature, tok):
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(size=vocab) * 2
+    a, b, h = 0.7, -0.4, 1e-5
+
+    def loss(v):
+        r = Row(v, temperature)
+        m = r.score(tok)[0]
+        return (a * m if math.isfinite(m) else 0.0) + b * r.h(tok)[0]
+
+    got = Row(x, temperature).grad(tok, a, b, 0.0, 0.0)[0]
+    for i in range(vocab):
+        d = np.zeros(vocab)
+        d[i] = h
+        # (the central difference is off by h^2 / 6 times the third derivative, and by the losses' rounding over h)
+        assert abs((loss(x + d) - loss(x - d)) / (2 * h) - got[i]) < 1e-8
+
+
+def _score(**over):
+    a = dict(logits=None, dtype=0, outer=1, inner=1, vocab=8, os=0, is_=8, tokens=None, tb=8, tos=0, tis=1, t=1.0, ml2p=None,
+             ent=None, top=0, ids=None, vals=None, stream=None)
+    a.update(over)
+    return nv.lib.mc_logits_score(*a.values())
+
+
+BUF = (C.c_char * 4096)()
+ADDR = C.addressof(BUF) & ~63 | 0
+
+
+@pytest.mark.parametrize("over", [
+    dict(),                                                     # no logits
+    dict(logits=ADDR),                                          # no tokens
+    dict(logits=ADDR, tokens=ADDR),                             # no output
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, dtype=3),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, vocab=0),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, vocab=1 << 31),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, outer=1 << 20, inner=1 << 20),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, outer=1 << 63, inner=2),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, tb=2),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, t=0.0),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, t=-1.0),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, t=math.nan),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, t=math.inf),
+    dict(logits=ADDR + 2, tokens=ADDR, ml2p=ADDR),              # float32 at an odd half word
+    dict(logits=ADDR + 1, tokens=ADDR, ml2p=ADDR, dtype=2),
+    dict(logits=ADDR, tokens=ADDR + 4, ml2p=ADDR),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, top=65, ids=ADDR, vals=ADDR, vocab=100),
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, top=9, ids=ADDR, vals=ADDR),      # more than tokens
+    dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, top=2, ids=ADDR),
+])
+def test_score_refuses(over):
+    assert _score(**over) == -1
+    assert nv.lib.mc_last_error().startswith(b"mc_logits_score: ")
+
+
+@pytest.mark.parametrize("name,args", [
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, None, 0, 1, None, 0, 0, ADDR, None, ADDR, None]),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, None, None]),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR + 2, None]),
+    ("mc_logits_gradient", [ADDR, 7, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, None]),
+    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, None, ADDR, None]),
+    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 0.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
+    ("mc_logits_draw", [ADDR, 0, 1 << 31, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
+    ("mc_logits_draw", [None, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
+    ("mc_logits_keys", [ADDR, ADDR, ADDR, 8, 1, 0, 1, ADDR, None]),
+    ("mc_logits_keys", [ADDR, None, ADDR, 2, 1, 0, 1, ADDR, None]),
+    ("mc_logits_keys", [None, None, None, 0, 1, 4, 4, ADDR, None]),
+    ("mc_logits_keys", [ADDR, None, None, 0, 1, 4, 4, None, None]),
+    ("mc_logits_keys", [ADDR, None, None, 0, 1 << 50, 4, 4, ADDR, None]),
+])
+def test_the_others_refuse(name, args):
+    assert getattr(nv.lib, name)(*args) == -1
+    assert nv.lib.mc_last_error().startswith(name.encode() + b": ")
+
+
+def test_nothing_to_do_is_fine_without_a_gpu():
+    assert _score(inner=0) == 0
+    assert _score(outer=0, inner=5) == 0
+    assert nv.lib.mc_logits_draw(None, 0, 0, 8, 8, 1.0, None, 0, 0, 0, None, None, None, None) == 0
+    assert nv.lib.mc_logits_keys(None, None, None, 0, 0, 0, 0, None, None) == 0
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x = torch.zeros(3, 5)
+    t = torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: lg.logits_score(x, t), lambda: lg.logits_gradient(x, t, torch.ones(3)),
+                 lambda: lg.logits_draw(x, seed=1), lambda: lg.logits_keys(x)):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
