@@ -82,6 +82,7 @@ __device__ __forceinline__ int token_of(const Rows &a, u32 row) {
 // one workgroup a row: a grid of two dimensions, since one holds at most 2^32 work items
 constexpr u32 GRID_X = 1u << 20;
 __device__ __forceinline__ u32 row_of_block() { return blockIdx.y * GRID_X + blockIdx.x; }
+u32 rows_to_blocks(u32 rows, u32 group) { return (u32)(((u64)rows * group + BLOCK - 1) / BLOCK); }
 dim3 grid_of(u32 rows) { return rows <= GRID_X ? dim3(rows) : dim3(GRID_X, (rows + GRID_X - 1) / GRID_X); }
 
 template <int DT>
@@ -165,22 +166,22 @@ __device__ __forceinline__ u32 pack2(float lo, float hi) {
 }
 
 template <int DT>
-__device__ __forceinline__ void store_vec(char *row, u32 v, u32 vocab, const float *g) {
+__device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const float *g) {
     constexpr u32 N = VEC<DT>;
-    if ((u64)v * N + N <= vocab) {
+    if ((u64)from + N <= vocab) {
         raw4 q;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (Elt<DT>::BYTES == 4) q[j] = __float_as_uint(g[j]);
             else q[j] = pack2<DT>(g[2 * j], g[2 * j + 1]);
         }
-        *(raw4_at2 *)(row + (u64)v * 16) = q;
+        *(raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES) = q;
     } else {
 #pragma unroll
         for (u32 j = 0; j < N; ++j) {
-            if ((u64)v * N + j < vocab) {
-                if constexpr (Elt<DT>::BYTES == 4) *(float *)(row + ((u64)v * N + j) * 4) = g[j];
-                else *(unsigned short *)(row + ((u64)v * N + j) * 2) = (unsigned short)pack2<DT>(g[j], 0.f);
+            if (from + j < vocab) {
+                if constexpr (Elt<DT>::BYTES == 4) *(float *)(row + ((u64)from + j) * 4) = g[j];
+                else *(unsigned short *)(row + ((u64)from + j) * 2) = (unsigned short)pack2<DT>(g[j], 0.f);
             }
         }
     }
@@ -312,6 +313,142 @@ __device__ __forceinline__ float ml2p_of(int tok, const Stat &st, float x, float
 
 __device__ __forceinline__ float entropy_of(int tok, const Stat &st) {
     return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : log2f(st.s) - st.e / st.s;
+}
+
+// ---- rows of few tokens: a group of G lanes a row, several rows a wave, the row in registers ---------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+    __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
+};
+
+// the same bits in every lane of the group: each step joins two halves that hold one value each
+template <int G, typename Op>
+__device__ __forceinline__ float group_all(float x, Op op) {
+    if constexpr (G >= 2) x = op(x, dpp<0xB1>(x));    // quad_perm 1 0 3 2
+    if constexpr (G >= 4) x = op(x, dpp<0x4E>(x));    // quad_perm 2 3 0 1
+    if constexpr (G >= 8) x = op(x, dpp<0x141>(x));   // half rows mirrored
+    if constexpr (G >= 16) x = op(x, dpp<0x140>(x));  // rows mirrored
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return x;
+}
+
+template <int G, typename Op>
+__device__ __forceinline__ double group_all(double x, Op op) {
+#pragma unroll
+    for (int d = 1; d < G; d <<= 1) x = op(x, __shfl_xor(x, d));
+    return x;
+}
+
+// inclusive prefix sum over the lanes of a group
+template <int G, typename A>
+__device__ __forceinline__ A group_scan(A x) {
+#pragma unroll
+    for (int d = 1; d < G; d <<= 1) {
+        const A o = __shfl_up(x, d, G);
+        if ((threadIdx.x & (G - 1)) >= (u32)d) x += o;
+    }
+    return x;
+}
+
+constexpr int SUB_NV = 8;  // vectors a lane holds at most
+
+// Vector v of a row, 16 bytes whole: the last one of a row that is no multiple of it reaches back into the one before it.
+// `from`: its first element's number; `own`: the first that is not the vector's before it.
+template <int DT>
+__device__ __forceinline__ raw4 load_sub(const char *row, u32 v, u32 nvec, u32 vocab, u32 &from, u32 &own) {
+    constexpr u32 N = VEC<DT>;
+    raw4 q = {Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF};
+    from = own = v * N;
+    if (v < nvec) {
+        if (vocab < N) {
+            q = load_vec<DT>(row, v, nvec, vocab);
+        } else {
+            from = min(own, vocab - N);
+            q = *(const raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES);
+        }
+    }
+    return q;
+}
+
+// the vector with -inf in the places that are another one's
+template <int DT>
+__device__ __forceinline__ raw4 masked(raw4 q, u32 from, u32 own) {
+    if (from == own) return q;
+    const u32 n = own - from;
+#pragma unroll
+    for (u32 w = 0; w < 4; ++w) {
+        u32 m;
+        if constexpr (Elt<DT>::BYTES == 4) m = w < n ? 0xFFFFFFFFu : 0u;
+        else m = (2 * w < n ? 0xFFFFu : 0u) | (2 * w + 1 < n ? 0xFFFF0000u : 0u);
+        q[w] = (q[w] & ~m) | (Elt<DT>::NEG_INF & m);
+    }
+    return q;
+}
+
+template <int DT>
+struct SubRow {
+    raw4 q[SUB_NV];      // as loaded
+    u32 from, own;       // of the lane's last vector (the others' are whole)
+    u32 nv;              // vectors a lane holds, the same in the whole grid
+};
+
+template <int DT, int G>
+__device__ __forceinline__ void load_row(SubRow<DT> &r, const char *p, const Rows &a, bool read) {
+    const u32 lane = threadIdx.x & (G - 1);
+    r.nv = (a.nvec + G - 1) / G;
+    r.from = r.own = 0;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) r.q[i] = load_sub<DT>(p, i * G + lane, read ? a.nvec : 0u, a.vocab, r.from, r.own);
+    }
+}
+
+template <int DT, int G>
+__device__ __forceinline__ raw4 vec_of(const SubRow<DT> &r, int i) {
+    return i + 1 == (int)r.nv ? masked<DT>(r.q[i], r.from, r.own) : r.q[i];
+}
+
+template <int DT, int G, bool ENT>
+__device__ __forceinline__ Stat sub_stat(const SubRow<DT> &r, float c) {
+    float m = LOWEST;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT, G>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) m = fmaxf(m, unpack<DT>(q, j));
+        }
+    }
+    m = group_all<G>(m, Max());
+    float s = 0.f, e = 0.f;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT, G>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float y = (unpack<DT>(q, j) - m) * c, w = exp2_(y);
+                s += w;
+                if (ENT) e += w * fmaxf(y, FAR);
+            }
+        }
+    }
+    return Stat{m, group_all<G>(s, Add()), ENT ? group_all<G>(e, Add()) : 0.f};
 }
 
 // ---- top alternatives ------------------------------------------------------------------------------------------
@@ -508,6 +645,67 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score(Rows a, ScoreOut out) {
     }
 }
 
+// The k largest of a row in registers, one after the other: the largest that comes behind the last one in the order (logit
+// descending, index ascending).
+template <int DT, int G>
+__device__ __forceinline__ void sub_top(const SubRow<DT> &r, const Rows &a, const Stat &st, const ScoreOut &out, u32 row, bool writes, int fill,
+                                        float fill_value) {
+    const u32 lane = threadIdx.x & (G - 1);
+    const float lz = log2f(st.s);
+    float last = INFINITY;
+    u32 last_i = 0xFFFFFFFFu;
+    for (u32 k = 0; k < out.k; ++k) {
+        float best = -INFINITY;
+        u32 best_i = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < SUB_NV; ++i) {
+            if (i < (int)r.nv) {
+                const raw4 q = vec_of<DT, G>(r, i);
+                const u32 from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) {
+                    const float x = unpack<DT>(q, j);
+                    const bool open = x < last || (x == last && from + j > last_i);
+                    if (open && x > best) best = x, best_i = from + j;
+                }
+            }
+        }
+        const float top = group_all<G>(best, Max());
+        u32 at = best == top ? best_i : 0xFFFFFFFFu;
+#pragma unroll
+        for (int d = 1; d < G; d <<= 1) at = min(at, (u32)__shfl_xor(at, d));
+        const float v = lz - (top - st.m) * a.c;
+        const bool there = fill == 0 && top > -INFINITY && v < INFINITY;
+        if (writes && lane == 0) {
+            out.top[(u64)row * out.k + k] = there ? (int)at : fill == 0 ? MC_TOKEN_OUTSIDE : fill;
+            out.top_ml2p[(u64)row * out.k + k] = there ? v : fill == 0 ? INFINITY : fill_value;
+        }
+        last = top;
+        last_i = at;
+    }
+}
+
+template <int DT, int G, bool ENT>
+__global__ __launch_bounds__(BLOCK) void k_logits_score_sub(Rows a, ScoreOut out) {
+    const u32 row = row_of_block() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows;
+    const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    if (there && lane == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+    }
+    if (out.k) {
+        const bool bad = !(st.s == st.s);
+        sub_top<DT, G>(r, a, st, out, row, there, tok == MC_TOKEN_SKIP ? MC_TOKEN_SKIP : bad ? MC_TOKEN_OUTSIDE : 0,
+                       tok == MC_TOKEN_SKIP ? 0.f : st.s);
+    }
+}
+
 // ---- gradient ------------------------------------------------------------------------------------------------------
 struct GradOut {
     View weights, entropy_weights;  // entropy_weights.p may be null
@@ -557,7 +755,46 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient(Rows a, GradOut out) 
                 if ((int)(v * VEC<DT> + j) == tok) g[j] -= A;
             }
         }
-        store_vec<DT>(gp, v, a.vocab, g);
+        store_at<DT>(gp, v * VEC<DT>, a.vocab, g);
+    }
+}
+
+template <int DT, int G, bool ENT>
+__global__ __launch_bounds__(BLOCK) void k_logits_gradient_sub(Rows a, GradOut out) {
+    const u32 row = row_of_block() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows;
+    const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const float A = tok >= 0 ? *(const float *)at(out.weights, a.inner, row) * a.c : 0.f;
+    const float B = ENT && there ? *(const float *)at(out.entropy_weights, a.inner, row) * out.inv_t : 0.f;
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    if (!there) return;
+    if (lane == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+    }
+    const bool none = tok == MC_TOKEN_SKIP || st.s == 0.f;
+    const float inv = none ? 0.f : 1.f / st.s, off = ENT ? entropy_of(tok, st) - log2f(st.s) : 0.f;
+    char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv && i * G + lane < a.nvec) {
+            // (a last vector that reaches back computes and stores what the one before it does)
+            const u32 from = none || a.vocab < VEC<DT> ? min((i * G + lane) * VEC<DT>, a.vocab < VEC<DT> ? 0u : a.vocab - VEC<DT>)
+                             : i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+            float g[VEC<DT>];
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float y = (unpack<DT>(r.q[i], j) - st.m) * a.c, pr = exp2_(y) * inv;
+                g[j] = ENT ? pr * (A - B * (fmaxf(y, FAR) + off)) : pr * A;
+                if ((int)(from + j) == tok) g[j] -= A;
+                if (none) g[j] = 0.f;
+            }
+            store_at<DT>(gp, from, a.vocab, g);
+        }
     }
 }
 
@@ -566,7 +803,7 @@ struct DrawArgs {
     const double *uniforms;  // or null: Philox
     u64 seed, first_id;
     u32 draw;
-    double t;
+    double t, eps;
     const unsigned char *live;
     int *token;
     float *ml2p;
@@ -677,6 +914,95 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw(Rows a, DrawArgs d) {
     }
 }
 
+// draw_row for a group's row in registers: running sums in the order of the index, vector by vector of the lanes
+template <int DT, int G, typename A>
+__device__ __forceinline__ bool draw_sub(const SubRow<DT> &r, const Rows &a, const DrawArgs &d, float m, double u, double eps, u32 &token) {
+    const u32 lane = threadIdx.x & (G - 1);
+    A s[SUB_NV], z = 0;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        s[i] = 0;
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT, G>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) s[i] += weight<A>(unpack<DT>(q, j), m, a.c, d.t);
+            z += s[i];
+        }
+    }
+    z = group_all<G>(z, Add());
+    const double target = u * (double)z;
+    // the vector step whose running sum passes the target, or the last one with any weight
+    double before = 0., run = 0.;
+    A mine = 0;
+    raw4 q = r.q[0];
+    u32 from = lane * VEC<DT>;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const double step = (double)group_all<G>(s[i], Add());
+            if (!found && step > 0.) {
+                before = run;
+                mine = s[i];
+                q = vec_of<DT, G>(r, i);
+                from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+                found = run + step > target;
+            }
+            run += step;
+        }
+    }
+    const A inc = group_scan<G>(mine);
+    const double lo = before + (double)(inc - mine);
+    const u32 shift = threadIdx.x & 63 & ~(G - 1);
+    const u64 all = G == 64 ? ~0ull : (1ull << (G & 63)) - 1;
+    const u64 passes = (__ballot(before + (double)inc > target) >> shift) & all, some = (__ballot(mine > 0) >> shift) & all;
+    // (a sum that passes by a rounding only, or none: the last lane with any weight)
+    const bool hit = found && passes;
+    const u32 who = hit ? (u32)__ffsll((unsigned long long)passes) - 1 : some ? 63u - (u32)__clzll((long long)some) : 0u;
+    double at_lo = lo;
+    u32 got = 0xFFFFFFFFu, last = 0;
+    bool ok = false;
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) {
+        const A w = weight<A>(unpack<DT>(q, j), m, a.c, d.t);
+        const double next = at_lo + (double)w;
+        if (w > 0) {
+            last = from + j;
+            if (got == 0xFFFFFFFFu && next > target) {
+                got = from + j;
+                ok = hit && target - at_lo >= eps * (double)z && next - target >= eps * (double)z;
+            }
+        }
+        at_lo = next;
+    }
+    if (!hit || got == 0xFFFFFFFFu) got = last;
+    token = __shfl(got, who, G);
+    return __shfl((int)ok, who, G) || eps == 0.;
+}
+
+template <int DT, int G>
+__global__ __launch_bounds__(BLOCK) void k_logits_draw_sub(Rows a, DrawArgs d) {
+    const u32 row = row_of_block() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows, live = there && (!d.live || d.live[row]);
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, live);
+    const double u = there ? uniform_of(d, row) : 0.;
+    const Stat st = sub_stat<DT, G, false>(r, a.c);
+    u32 token = 0;
+    bool sure = draw_sub<DT, G, float>(r, a, d, st.m, u, d.eps, token);
+    if (!(st.s > 0.f)) sure = true, token = 0;
+    if (__ballot(!sure)) {  // (a few rows in a million: the whole wave decides again in 64 bits)
+        u32 again;
+        draw_sub<DT, G, double>(r, a, d, st.m, u, 0., again);
+        if (!sure) token = again;
+    }
+    if (there && lane == 0) {
+        d.token[row] = !live ? MC_TOKEN_SKIP : st.s > 0.f ? (int)token : MC_TOKEN_OUTSIDE;
+        d.ml2p[row] = !live ? 0.f : st.s > 0.f ? ml2p_of(0, st, element<DT>(p, token), a.c) : st.s == 0.f ? INFINITY : st.s;
+    }
+}
+
 // ---- keys ----------------------------------------------------------------------------------------------------------
 // one lane a password
 __global__ __launch_bounds__(BLOCK) void k_logits_keys(const float *ml2p, const i64 *offsets, const void *lengths, u32 length_bytes,
@@ -698,6 +1024,21 @@ __global__ __launch_bounds__(BLOCK) void k_logits_keys(const float *ml2p, const 
         out[i] = s == INFINITY ? 1022.0 : s;
     }
 }
+
+// A group of lanes a row while a row's vectors fit the registers of 64 lanes (4096 tokens of two bytes), else a workgroup.
+constexpr u32 SUB_VECS = 64 * SUB_NV;
+
+#define BY_GROUP(nvec, ...)                              \
+    if ((nvec) <= 4 * SUB_NV) { constexpr int G = 4; __VA_ARGS__; }        \
+    else if ((nvec) <= 8 * SUB_NV) { constexpr int G = 8; __VA_ARGS__; }   \
+    else if ((nvec) <= 16 * SUB_NV) { constexpr int G = 16; __VA_ARGS__; } \
+    else if ((nvec) <= 32 * SUB_NV) { constexpr int G = 32; __VA_ARGS__; } \
+    else { constexpr int G = 64; __VA_ARGS__; }
+
+// How far off a running sum of weights in 32 bits may be as a share of the whole: the weights' own errors (the exponent's
+// three roundings weigh at most 2.1 log2 V of half a step in the sum, the power's own 2) and one half step for each of
+// the additions behind each other (a lane's vectors, then the joining of lanes); twice, since the target is such a sum too.
+double error_of_sums(const Rows &a) { return 0x1p-24 * 2. * (SUB_NV * 8 + 16 + 8 + 2.1 * std::log2((double)a.vocab)); }
 
 int bad(const char *who, const char *why) {
     mc_set_error("%s: %s", who, why);
@@ -741,11 +1082,11 @@ int tokens_of(const char *who, Rows &a, const void *tokens, uint32_t token_bytes
 
 }  // namespace
 
-#define BY_TYPE(dtype, call)                            \
+#define BY_TYPE(dtype, ...)                            \
     switch (dtype) {                                    \
-        case MC_LOGITS_F32: { constexpr int DT = MC_LOGITS_F32; call; break; }   \
-        case MC_LOGITS_F16: { constexpr int DT = MC_LOGITS_F16; call; break; }   \
-        default: { constexpr int DT = MC_LOGITS_BF16; call; break; }             \
+        case MC_LOGITS_F32: { constexpr int DT = MC_LOGITS_F32; __VA_ARGS__; break; }   \
+        case MC_LOGITS_F16: { constexpr int DT = MC_LOGITS_F16; __VA_ARGS__; break; }   \
+        default: { constexpr int DT = MC_LOGITS_BF16; __VA_ARGS__; break; }             \
     }
 
 extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
@@ -763,7 +1104,12 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
     if (!out_ml2p || (top && (!out_top || !out_top_ml2p))) return bad(who, "no output");
     ScoreOut out{out_ml2p, out_entropy, out_top_ml2p, out_top, top};
     hipStream_t s = (hipStream_t)stream;
-    if (top) {
+    if (a.nvec <= SUB_VECS) {
+        BY_TYPE(dtype, BY_GROUP(a.nvec, {
+                    if (out_entropy) hipLaunchKernelGGL((k_logits_score_sub<DT, G, true>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                    else hipLaunchKernelGGL((k_logits_score_sub<DT, G, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                }));
+    } else if (top) {
         BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_score<DT, true>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out));
     } else {
         BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_score<DT, false>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out));
@@ -791,7 +1137,12 @@ extern "C" int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t o
     GradOut out{View{(const char *)weights, weight_outer_stride * 4, weight_inner_stride * 4},
                 View{(const char *)entropy_weights, entropy_outer_stride * 4, entropy_inner_stride * 4},
                 (float)(1.0 / temperature), out_ml2p, out_entropy, (char *)out_grad};
-    BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_gradient<DT>), grid_of(a.rows), dim3(BLOCK), 0, (hipStream_t)stream, a, out));
+    if (a.nvec <= SUB_VECS) {
+        BY_TYPE(dtype, BY_GROUP(a.nvec, {
+                    if (entropy_weights) hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, true>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, (hipStream_t)stream, a, out);
+                    else hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, (hipStream_t)stream, a, out);
+                }));
+    } else BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_gradient<DT>), grid_of(a.rows), dim3(BLOCK), 0, (hipStream_t)stream, a, out));
     HIP_TRY(hipGetLastError());
     return MC_OK;
 }
@@ -804,8 +1155,10 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (int rc = rows_of(who, a, logits, dtype, 1, rows, vocab, 0, row_stride, temperature, true)) return rc;
     if (a.rows == 0) return MC_OK;
     if (!out_token || !out_ml2p) return bad(who, "no output");
-    DrawArgs d{uniforms, seed, first_id, draw, temperature, live, out_token, out_ml2p};
-    BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(BLOCK), 0, (hipStream_t)stream, a, d));
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, error_of_sums(a), live, out_token, out_ml2p};
+    if (a.nvec <= SUB_VECS) {
+        BY_TYPE(dtype, BY_GROUP(a.nvec, hipLaunchKernelGGL((k_logits_draw_sub<DT, G>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, (hipStream_t)stream, a, d)));
+    } else BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(BLOCK), 0, (hipStream_t)stream, a, d));
     HIP_TRY(hipGetLastError());
     return MC_OK;
 }
