@@ -555,7 +555,8 @@ int mc_rank_query(const double *keys_sorted, const double *positions, uint64_t n
  * ELEMENTS, consecutive tokens adjacent; any strides (a slice of a longer sequence, rows that overlap or repeat), any
  * alignment of the element's own.  Tokens and weights come with strides of their own for the same (outer, inner); outputs
  * are contiguous [outer * inner].  Sums are held in 32 bits (the draw decides in 64).  All calls are asynchronous on
- * `stream`, allocate nothing and may be captured into a graph.  Temperatures 1e-30 .. 1e30.
+ * `stream`, allocate nothing and may be captured into a graph.  A workspace (16-byte aligned, mc_logits_*_workspace_bytes;
+ * NULL where that is 0) holds nothing between calls, but calls that may overlap need one each.  Temperatures 1e-30 .. 1e30.
  *   token ids   0 .. vocab - 1; MC_TOKEN_SKIP: the row is not read (padding), its outputs are 0; anything else is a token
  *               outside the model, as MC_TOKEN_OUTSIDE: impossible (+inf)
  *   -inf        a token switched off: probability 0.  A row with nothing left: ml2p +inf, entropy 0, no alternatives, no
@@ -569,29 +570,35 @@ enum { MC_LOGITS_F32 = 0, MC_LOGITS_F16 = 1, MC_LOGITS_BF16 = 2 };
  * `top` most probable tokens (<= MC_LOGITS_MAX_TOP and <= vocab) in descending order, equal logits by the lower id:
  * out_top[rows][top] and their -log2 p out_top_ml2p[rows][top]; where fewer have any probability the rest is
  * MC_TOKEN_OUTSIDE / +inf, in a skipped row MC_TOKEN_SKIP / 0. */
+size_t mc_logits_score_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab, uint32_t top);
 int mc_logits_score(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
                     int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
                     int64_t token_outer_stride, int64_t token_inner_stride, double temperature, float *out_ml2p,
-                    float *out_entropy, uint32_t top, int32_t *out_top, float *out_top_ml2p, void *stream);
+                    float *out_entropy, uint32_t top, int32_t *out_top, float *out_top_ml2p, void *workspace,
+                    size_t workspace_bytes, void *stream);
 /* out_grad[rows][vocab] (contiguous, the logits' type, one rounding) = the gradient of
  *     sum over rows of weights[r] * ml2p[r] + entropy_weights[r] * entropy[r]
- * (entropy_weights may be NULL) for the logits, with ml2p and entropy (may be NULL) as mc_logits_score gives them.  Skipped
- * rows and rows with nothing left have gradient 0; where the token is outside the model weights[r] is not read.
+ * (entropy_weights may be NULL) for the logits, with ml2p and entropy as mc_logits_score gives them (out_entropy may be NULL
+ * without entropy_weights, and is then not written).  Skipped rows and rows with nothing left have gradient 0; where the token is outside the model weights[r] is not read.
  * out_grad may be the logits themselves when those are contiguous; it must not overlap them otherwise. */
+size_t mc_logits_gradient_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab);
 int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
                        int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
                        int64_t token_outer_stride, int64_t token_inner_stride, double temperature,
                        const float *weights, int64_t weight_outer_stride, int64_t weight_inner_stride,
                        const float *entropy_weights, int64_t entropy_outer_stride, int64_t entropy_inner_stride,
-                       float *out_ml2p, float *out_entropy, void *out_grad, void *stream);
+                       float *out_ml2p, float *out_entropy, void *out_grad, void *workspace, size_t workspace_bytes,
+                       void *stream);
 /* One draw from every row by inversion, as pick_expand: the first token whose running sum C_i of exp((x_i - max x) / T)
  * exceeds u * C_(vocab-1), decided as sums in 64 bits decide it; out_token and its out_ml2p.  u = uniforms[row] in
  * [0, 1) (below: 0, above: the last token with any probability, NaN: 0), or, with uniforms NULL, the uniform
  * (seed, first_id + row, draw) of the stream mc_sample uses.  live (may be NULL): rows whose byte is 0 are not read
  * (samples that have ended): MC_TOKEN_SKIP, 0. */
+size_t mc_logits_draw_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab);
 int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows, uint64_t vocab, int64_t row_stride,
                    double temperature, const double *uniforms, uint64_t seed, uint64_t first_id, uint32_t draw,
-                   const uint8_t *live, int32_t *out_token, float *out_ml2p, void *stream);
+                   const uint8_t *live, int32_t *out_token, float *out_ml2p, void *workspace, size_t workspace_bytes,
+                   void *stream);
 /* -log2 p of whole passwords, the keys of mc_rank_build: the sum in 64 bits of a password's ml2p; 1022.0 where one of
  * them is +inf (as mc_score), 0.0 for no symbols.  Packed: password t is ml2p[offsets[t] .. offsets[t+1]) of `longest`
  * values in all (a pair of offsets that does not ascend within them names nothing).  Padded (offsets NULL):

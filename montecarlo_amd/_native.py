@@ -75,11 +75,14 @@ def _load() -> C.CDLL:
         "mc_abi_version": (C.c_int, []),
         "mc_last_error": (C.c_char_p, []),
         "mc_logits_score": (C.c_int, [vp, C.c_uint32] + [C.c_uint64] * 3 + [C.c_int64] * 2 + [vp, C.c_uint32] + [C.c_int64] * 2
-                            + [C.c_double, vp, vp, C.c_uint32, vp, vp, vp]),
+                            + [C.c_double, vp, vp, C.c_uint32, vp, vp, vp, C.c_size_t, vp]),
         "mc_logits_gradient": (C.c_int, [vp, C.c_uint32] + [C.c_uint64] * 3 + [C.c_int64] * 2 + [vp, C.c_uint32]
-                               + [C.c_int64] * 2 + [C.c_double] + [vp, C.c_int64, C.c_int64] * 2 + [vp] * 4),
+                               + [C.c_int64] * 2 + [C.c_double] + [vp, C.c_int64, C.c_int64] * 2 + [vp] * 4 + [C.c_size_t, vp]),
         "mc_logits_draw": (C.c_int, [vp, C.c_uint32, C.c_uint64, C.c_uint64, C.c_int64, C.c_double, vp, C.c_uint64,
-                                     C.c_uint64, C.c_uint32, vp, vp, vp, vp]),
+                                     C.c_uint64, C.c_uint32, vp, vp, vp, vp, C.c_size_t, vp]),
+        "mc_logits_score_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint32]),
+        "mc_logits_gradient_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint64, C.c_uint64]),
+        "mc_logits_draw_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint64, C.c_uint64]),
         "mc_logits_keys": (C.c_int, [vp, vp, vp, C.c_uint32, C.c_uint64, C.c_int64, C.c_uint64, vp, vp]),
         "mc_table_compile": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(vp)]),
         "mc_table_free": (None, [vp]),
@@ -209,7 +212,7 @@ EXPORTS = ["mc_abi_version", "mc_last_error", "mc_table_compile", "mc_table_free
            "mc_rank_runs_forget", "mc_rank_runs_check", "mc_rank_runs_query", "mc_rank_runs_expand", "mc_rank_runs_debug_phases",
            "mc_score_words_debug_kernel", "mc_score_bpe_debug_kernel",
            "mc_rank_runs_debug_groups", "mc_rank_runs_guess_numbers", "mc_logits_score", "mc_logits_gradient", "mc_logits_draw",
-           "mc_logits_keys"]
+           "mc_logits_keys", "mc_logits_score_workspace_bytes", "mc_logits_gradient_workspace_bytes", "mc_logits_draw_workspace_bytes"]
 
 
 def check(rc: int) -> int:

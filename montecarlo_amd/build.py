@@ -14,8 +14,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmi355mc.so")
-SOURCES = ["mc_table.cpp", "mc_train.cpp", "mc_ingest.cpp", "mc_device.hip", "mc_rank.hip", "mc_sort.hip", "mc_runs.hip", "mc_gn.hip", "mc_enum.hip", "mc_logits.hip", "mc_comm.cpp"]
+SOURCES = ["mc_table.cpp", "mc_train.cpp", "mc_ingest.cpp", "mc_device.hip", "mc_rank.hip", "mc_sort.hip", "mc_runs.hip", "mc_gn.hip", "mc_enum.hip", "mc_logits_score.hip",
+           "mc_logits_gradient.hip", "mc_logits_draw.hip", "mc_comm.cpp"]
 HEADERS = [os.path.join(CSRC, "mc_internal.h"), os.path.join(CSRC, "mc_sort.h"), os.path.join(CSRC, "mc_philox.h"),
+           os.path.join(CSRC, "mc_logits.h"),
            os.path.join(os.path.dirname(HERE), "include", "mi355mc.h")]
 # (packed float32 instructions stay off: some of their forms have given wrong results on this hardware; the host pass
 # does not know the feature and would say so for every file)

@@ -1,0 +1,608 @@
+// What the kernels on logits share (device code; mc_logits_score.hip says what they compute).
+//
+// With c = log2(e) / T a token's exponent is y = x c - M, where M = m c is the largest logit's: one multiply-add, one power
+// and the sums an element.  M may be off by a rounding; every use of it subtracts the same number, so that cancels.  That
+// holds while |M| <= 2^15 (the largest weight is then 2^(2^-9) at most).  Parts of a row whose own maximum lies lower take
+// -2^15 for it; a ROW whose M is beyond, whose weights all vanish that way, or that holds a NaN or +inf is summed again
+// with y = (x - m) c (`exact`): a row of the type's lowest value, temperatures near 0, rows with nothing left.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cmath>
+
+#include "mc_internal.h"
+
+#define HIP_TRY(expr)                                                                        \
+    do {                                                                                     \
+        hipError_t e_ = (expr);                                                              \
+        if (e_ != hipSuccess) {                                                              \
+            mc_set_error("%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
+            return MC_ERR_HIP;                                                               \
+        }                                                                                    \
+    } while (0)
+
+namespace {
+
+typedef unsigned long long u64;
+typedef unsigned int u32;
+typedef long long i64;
+
+constexpr int BLOCK = 256;
+constexpr float LOWEST = -FLT_MAX;
+constexpr double LOG2E = 1.4426950408889634074;
+constexpr float FAR = 32768.f;
+
+// A division by the same number for every row, as a multiplication: exact for row numbers below 2^31.
+struct Div {
+    u32 d, mul, shift;
+};
+
+// Something with a value (or a row of values) for every row, addressed by (row / inner, row % inner); strides in bytes.
+struct View {
+    const char *p;
+    i64 os, is;
+};
+
+struct Rows {
+    View logits, tokens;
+    Div inner;
+    u32 rows, vocab, nvec, full, token_bytes;  // nvec: vectors of 16 bytes a row; full: those that are whole
+    float c;                                   // log2(e) / T
+};
+
+__device__ __forceinline__ const char *at(const View &v, const Div &inner, u32 row) {
+    const u32 o = __umulhi(row << 1, inner.mul) >> inner.shift;
+    return v.p + (i64)o * v.os + (i64)(row - o * inner.d) * v.is;
+}
+
+// A token id as the kernels use it: [0, V), MC_TOKEN_SKIP, or MC_TOKEN_OUTSIDE for everything else.
+__device__ __forceinline__ int token_of(const Rows &a, u32 row) {
+    const char *p = at(a.tokens, a.inner, row);
+    const i64 t = a.token_bytes == 8 ? *(const i64 *)p : (i64) * (const int *)p;
+    return t == MC_TOKEN_SKIP ? MC_TOKEN_SKIP : (t >= 0 && t < (i64)a.vocab) ? (int)t : MC_TOKEN_OUTSIDE;
+}
+
+// workgroups in a grid of two dimensions, since one holds at most 2^32 work items
+constexpr u32 GRID_X = 1u << 20;
+__device__ __forceinline__ u32 block_id() { return blockIdx.y * GRID_X + blockIdx.x; }
+inline dim3 grid_of(u32 blocks) { return blocks <= GRID_X ? dim3(blocks) : dim3(GRID_X, (blocks + GRID_X - 1) / GRID_X); }
+
+template <int DT>
+struct Elt;
+template <>
+struct Elt<MC_LOGITS_F32> {
+    static constexpr int BYTES = 4;
+    static constexpr u32 NEG_INF = 0xFF800000u;
+};
+template <>
+struct Elt<MC_LOGITS_F16> {
+    static constexpr int BYTES = 2;
+    static constexpr u32 NEG_INF = 0xFC00FC00u;
+};
+template <>
+struct Elt<MC_LOGITS_BF16> {
+    static constexpr int BYTES = 2;
+    static constexpr u32 NEG_INF = 0xFF80FF80u;
+};
+
+template <int DT>
+constexpr int VEC = 16 / Elt<DT>::BYTES;
+
+// 16 bytes of a row; rows begin where they like (an odd number of 2-byte tokens), which the loads take as they are
+typedef u32 raw4 __attribute__((ext_vector_type(4)));
+typedef raw4 raw4_at2 __attribute__((aligned(2)));
+
+template <int DT>
+__device__ __forceinline__ float to_float(u32 word, int half) {
+    if constexpr (DT == MC_LOGITS_F32) return __uint_as_float(word);
+    if constexpr (DT == MC_LOGITS_BF16) return __uint_as_float(half ? word & 0xFFFF0000u : word << 16);
+    if constexpr (DT == MC_LOGITS_F16) {
+        const unsigned short h = (unsigned short)(half ? word >> 16 : word);
+        return (float)__builtin_bit_cast(_Float16, h);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float element(const char *row, u32 i) {
+    if constexpr (Elt<DT>::BYTES == 4) return *(const float *)(row + 4 * (u64)i);
+    else return to_float<DT>(*(const unsigned short *)(row + 2 * (u64)i), 0);
+}
+
+// element j of a vector of raw words
+template <int DT>
+__device__ __forceinline__ float unpack(const raw4 &q, int j) {
+    if constexpr (Elt<DT>::BYTES == 4) return to_float<DT>(q[j], 0);
+    else return to_float<DT>(q[j >> 1], j & 1);
+}
+
+template <int DT>
+__device__ __forceinline__ raw4 nothing() {
+    return raw4{Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF};
+}
+
+// vector v of a row; what lies behind the row's end, or in vectors from `end` on, is -inf
+template <int DT>
+__device__ __forceinline__ raw4 load_vec(const char *row, const Rows &a, u32 v, u32 end) {
+    constexpr u32 N = VEC<DT>;
+    raw4 q = nothing<DT>();
+    if (v < min(end, a.full)) {
+        q = *(const raw4_at2 *)(row + (u64)v * 16);
+    } else if (v < end) {
+#pragma unroll
+        for (u32 j = 0; j < N; ++j) {
+            if (v * N + j < a.vocab) {
+                if constexpr (Elt<DT>::BYTES == 4) {
+                    q[j] = *(const u32 *)(row + ((u64)v * N + j) * 4);
+                } else {
+                    const u32 h = *(const unsigned short *)(row + ((u64)v * N + j) * 2);
+                    q[j >> 1] = (j & 1) ? (q[j >> 1] & 0xFFFFu) | (h << 16) : (q[j >> 1] & 0xFFFF0000u) | h;
+                }
+            }
+        }
+    }
+    return q;
+}
+
+// one rounding to the logits' type, to nearest even
+template <int DT>
+__device__ __forceinline__ u32 pack2(float lo, float hi) {
+    if constexpr (DT == MC_LOGITS_BF16)
+        return (u32)__builtin_bit_cast(unsigned short, (__bf16)lo) | ((u32)__builtin_bit_cast(unsigned short, (__bf16)hi) << 16);
+    else
+        return (u32)__builtin_bit_cast(unsigned short, (_Float16)lo) | ((u32)__builtin_bit_cast(unsigned short, (_Float16)hi) << 16);
+}
+
+// the elements from `from` on that the row has room for
+template <int DT>
+__device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const float *g) {
+    constexpr u32 N = VEC<DT>;
+    if ((u64)from + N <= vocab) {
+        raw4 q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (Elt<DT>::BYTES == 4) q[j] = __float_as_uint(g[j]);
+            else q[j] = pack2<DT>(g[2 * j], g[2 * j + 1]);
+        }
+        *(raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES) = q;
+    } else {
+#pragma unroll
+        for (u32 j = 0; j < N; ++j) {
+            if (from + j < vocab) {
+                if constexpr (Elt<DT>::BYTES == 4) *(float *)(row + ((u64)from + j) * 4) = g[j];
+                else *(unsigned short *)(row + ((u64)from + j) * 2) = (unsigned short)pack2<DT>(g[j], 0.f);
+            }
+        }
+    }
+}
+
+// the larger of two logits, NaN if one is (an instruction that takes three and, unlike fmaxf's, quiets nothing first)
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A row's (or a part's) largest logit m, the sum s of 2^y and the sum e of 2^y y; `exact` says how y is meant.
+struct Stat {
+    float m, s, e;
+    bool exact;
+};
+
+__device__ __forceinline__ float scaled(float m, float c) { return fmaxf(m * c, -FAR); }
+
+// the exponent of a logit under a row's statistics
+struct Expo {
+    float m, c, M;
+    bool exact;
+    __device__ __forceinline__ Expo(const Stat &st, float c_) : m(fmaxf(st.m, LOWEST)), c(c_), M(scaled(st.m, c_)), exact(st.exact) {}
+    __device__ __forceinline__ float fast(float x) const { return __builtin_fmaf(x, c, -M); }
+    __device__ __forceinline__ float operator()(float x) const { return exact ? (x - m) * c : fast(x); }
+};
+
+// whether a row's fast sums stand
+__device__ __forceinline__ bool doubtful(const Stat &st, float c) { return !(fabsf(scaled(st.m, c)) <= FAR && st.m * c > -FAR && st.s > 0.f); }
+
+// what a row's statistics say about its token
+__device__ __forceinline__ float ml2p_of(int tok, const Stat &st, float x, float c) {
+    if (tok == MC_TOKEN_SKIP) return 0.f;
+    if (!(st.s == st.s)) return st.s;
+    return tok >= 0 && st.s > 0.f ? log2f(st.s) - Expo(st, c)(x) : INFINITY;
+}
+
+__device__ __forceinline__ float entropy_of(int tok, const Stat &st) {
+    return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : log2f(st.s) - st.e / st.s;
+}
+
+// ---- reductions over groups of lanes and over workgroups ---------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Add {
+    template <typename A>
+    __device__ __forceinline__ A operator()(A a, A b) const {
+        return a + b;
+    }
+};
+
+// the same bits in every lane of the group: each step joins two halves that hold one value each
+template <int G, typename Op>
+__device__ __forceinline__ float group_all(float x, Op op) {
+    if constexpr (G >= 2) x = op(x, dpp<0xB1>(x));    // quad_perm 1 0 3 2
+    if constexpr (G >= 4) x = op(x, dpp<0x4E>(x));    // quad_perm 2 3 0 1
+    if constexpr (G >= 8) x = op(x, dpp<0x141>(x));   // half rows mirrored
+    if constexpr (G >= 16) x = op(x, dpp<0x140>(x));  // rows mirrored
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return x;
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    const float lo = dpp<CTRL>(__int_as_float(__double2loint(x))), hi = dpp<CTRL>(__int_as_float(__double2hiint(x)));
+    return __hiloint2double(__float_as_int(hi), __float_as_int(lo));
+}
+
+template <int G, typename Op>
+__device__ __forceinline__ double group_all(double x, Op op) {
+    if constexpr (G >= 2) x = op(x, dpp<0xB1>(x));
+    if constexpr (G >= 4) x = op(x, dpp<0x4E>(x));
+    if constexpr (G >= 8) x = op(x, dpp<0x141>(x));
+    if constexpr (G >= 16) x = op(x, dpp<0x140>(x));
+    if constexpr (G >= 32) x = op(x, __shfl_xor(x, 16));
+    if constexpr (G >= 64) x = op(x, __shfl_xor(x, 32));
+    return x;
+}
+
+// inclusive prefix sum over the lanes of a group
+template <int G, typename A>
+__device__ __forceinline__ A group_scan(A x) {
+#pragma unroll
+    for (int d = 1; d < G; d <<= 1) {
+        const A o = __shfl_up(x, d, G);
+        if ((threadIdx.x & (G - 1)) >= (u32)d) x += o;
+    }
+    return x;
+}
+
+// the lanes of a group joined: the common maximum, the sums scaled to it
+template <int G, bool ENT>
+__device__ __forceinline__ Stat group_stat(Stat st, float c) {
+    const float mine = scaled(st.m, c);
+    st.m = group_all<G>(st.m, Max());
+    const float d = mine - scaled(st.m, c), f = exp2_(d);
+    if (ENT) st.e = group_all<G>(__builtin_fmaf(d, st.s, st.e) * f, Add());
+    st.s = group_all<G>(st.s * f, Add());
+    return st;
+}
+
+// the whole workgroup's, in every thread
+template <int T, bool ENT>
+__device__ __forceinline__ Stat block_stat(Stat st, float c) {
+    __shared__ float pm[T / 64], ps[T / 64], pe[T / 64];
+    st = group_stat<64, ENT>(st, c);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        pm[threadIdx.x >> 6] = st.m;
+        ps[threadIdx.x >> 6] = st.s;
+        if (ENT) pe[threadIdx.x >> 6] = st.e;
+    }
+    __syncthreads();
+    const u32 w = threadIdx.x & (T / 64 - 1);  // (every group of as many lanes as there are waves joins the waves once more)
+    return group_stat<T / 64, ENT>(Stat{pm[w], ps[w], ENT ? pe[w] : 0.f, false}, c);
+}
+
+template <int T>
+__device__ __forceinline__ u32 block_sum(u32 v) {
+    __shared__ u32 part[T / 64];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) v += part[w];
+    return v;
+}
+
+template <int T>
+__device__ __forceinline__ float block_max(float v) {
+    __shared__ float part[T / 64];
+    v = group_all<64>(v, Max());
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) v = fmaxf(v, part[w]);
+    return v;
+}
+
+// exclusive prefix sum over the workgroup and the total
+template <int T, typename A>
+__device__ __forceinline__ A block_scan(A v, A &total) {
+    __shared__ A part[T / 64];
+    const A inc = group_scan<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    A base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+        if (w < (int)(threadIdx.x >> 6)) base += part[w];
+        total += part[w];
+    }
+    return base + inc - v;
+}
+
+template <int T>
+__device__ __forceinline__ u32 block_min(u32 v) {
+    __shared__ u32 part[T / 64];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = min(v, (u32)__shfl_xor(v, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) v = min(v, part[w]);
+    return v;
+}
+
+// ---- rows of few tokens: a group of G lanes a row, several rows a wave, the row in registers ---------------------------------
+constexpr int SUB_NV = 8;                    // vectors a lane holds at most
+constexpr u32 SUB_VECS = 64 * SUB_NV;        // vectors a group of 64 lanes holds: 4096 tokens of two bytes
+
+template <int DT>
+struct SubRow {
+    raw4 q[SUB_NV];      // as loaded
+    u32 from, own;       // of the lane's last vector (the others' are whole)
+    u32 nv;              // vectors a lane holds, the same in the whole grid
+};
+
+// Vector v of a row, 16 bytes whole: the last one of a row that is no multiple of it reaches back into the one before it.
+// `from`: its first element's number; `own`: the first that is not the vector's before it.
+template <int DT>
+__device__ __forceinline__ raw4 load_sub(const char *row, const Rows &a, u32 v, bool read, u32 &from, u32 &own) {
+    constexpr u32 N = VEC<DT>;
+    raw4 q = nothing<DT>();
+    from = own = v * N;
+    if (read && v < a.nvec) {
+        if (a.vocab < N) {
+            q = load_vec<DT>(row, a, v, a.nvec);
+        } else {
+            from = min(own, a.vocab - N);
+            q = *(const raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES);
+        }
+    }
+    return q;
+}
+
+// the vector with -inf in the places that are another one's
+template <int DT>
+__device__ __forceinline__ raw4 masked(raw4 q, u32 from, u32 own) {
+    if (from == own) return q;
+    const u32 n = own - from;
+#pragma unroll
+    for (u32 w = 0; w < 4; ++w) {
+        u32 m;
+        if constexpr (Elt<DT>::BYTES == 4) m = w < n ? 0xFFFFFFFFu : 0u;
+        else m = (2 * w < n ? 0xFFFFu : 0u) | (2 * w + 1 < n ? 0xFFFF0000u : 0u);
+        q[w] = (q[w] & ~m) | (Elt<DT>::NEG_INF & m);
+    }
+    return q;
+}
+
+template <int DT, int G>
+__device__ __forceinline__ void load_row(SubRow<DT> &r, const char *p, const Rows &a, bool read) {
+    const u32 lane = threadIdx.x & (G - 1);
+    r.nv = (a.nvec + G - 1) / G;
+    r.from = r.own = 0;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) r.q[i] = load_sub<DT>(p, a, i * G + lane, read, r.from, r.own);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ raw4 vec_of(const SubRow<DT> &r, int i) {
+    return i + 1 == (int)r.nv ? masked<DT>(r.q[i], r.from, r.own) : r.q[i];
+}
+
+template <int DT, int G, bool ENT, bool EXACT>
+__device__ __forceinline__ Stat sub_sums(const SubRow<DT> &r, float m, float c) {
+    Stat st{m, 0.f, 0.f, EXACT};
+    const Expo y_of(st, c);
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float x = unpack<DT>(q, j), y = EXACT ? (x - y_of.m) * c : y_of.fast(x), w = exp2_(y);
+                st.s += w;
+                if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
+            }
+        }
+    }
+    st.s = group_all<G>(st.s, Add());
+    if (ENT) st.e = group_all<G>(st.e, Add());
+    return st;
+}
+
+// The words of a row as if just loaded: what the next pass makes of them is made again from the packed words, where the
+// compiler would keep the unpacked numbers of all vectors in registers (145 instead of 64-80: three waves instead of six).
+template <int DT>
+__device__ __forceinline__ void forget(SubRow<DT> &r) {
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) asm("" : "+v"(r.q[i]));
+}
+
+template <int DT, int G, bool ENT>
+__device__ __forceinline__ Stat sub_stat(SubRow<DT> &r, float c) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) m = maximum(m, unpack<DT>(q, j));
+        }
+    }
+    m = group_all<G>(m, Max());
+    forget(r);
+    Stat st = sub_sums<DT, G, ENT, false>(r, m, c);
+    const bool again = doubtful(st, c);
+    forget(r);
+    if (__ballot(again)) {
+        const Stat ex = sub_sums<DT, G, ENT, true>(r, m, c);
+        if (again) st = ex;
+    }
+    return st;
+}
+
+// ---- rows of many tokens: workgroups that stream a row or a part of it ---------------------------------------------------
+constexpr int UNROLL = 4;  // vectors of a thread in flight
+
+// a chunk joins a thread's running statistics; returns the chunk's largest logit
+template <int DT, bool ENT>
+__device__ __forceinline__ float take(Stat &st, const raw4 (&q)[UNROLL], float c) {
+    constexpr int N = VEC<DT>;
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = maximum(m, unpack<DT>(q[u], j));
+    const float old = scaled(st.m, c);
+    st.m = maximum(st.m, m);
+    const float M = scaled(st.m, c), d = old - M, f = exp2_(d);
+    if (ENT) st.e = __builtin_fmaf(d, st.s, st.e) * f;
+    st.s *= f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float y = __builtin_fmaf(unpack<DT>(q[u], j), c, -M), w = exp2_(y);
+            st.s += w;
+            if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
+        }
+    return m;
+}
+
+// the vectors base + u * STRIDE + lane of a row, as far as they are below `end`
+template <int DT, int STRIDE>
+__device__ __forceinline__ void load_chunk(raw4 (&q)[UNROLL], const char *p, const Rows &a, u32 base, u32 lane, u32 end) {
+    if (base + UNROLL * STRIDE <= min(end, a.full)) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) q[u] = *(const raw4_at2 *)(p + (u64)(base + u * STRIDE + lane) * 16);
+    } else {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) q[u] = load_vec<DT>(p, a, base + u * STRIDE + lane, end);
+    }
+}
+
+// A doubtful row's statistics (every thread of the workgroup calls): m is its largest logit.
+template <int DT, int T, bool ENT>
+__device__ __forceinline__ Stat exact_stat(const char *p, const Rows &a, float m) {
+    Stat st{m, 0.f, 0.f, true};
+    m = fmaxf(m, LOWEST);
+    for (u32 v = threadIdx.x; v < a.nvec; v += T) {
+        const raw4 q = load_vec<DT>(p, a, v, a.nvec);
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) {
+            const float y = (unpack<DT>(q, j) - m) * a.c, w = exp2_(y);
+            st.s += w;
+            st.e += w * fmaxf(y, -FAR);
+        }
+    }
+    __shared__ float ps[T / 64], pe[T / 64];
+    st.s = group_all<64>(st.s, Add());
+    st.e = group_all<64>(st.e, Add());
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        ps[threadIdx.x >> 6] = st.s;
+        pe[threadIdx.x >> 6] = st.e;
+    }
+    __syncthreads();
+    const u32 w = threadIdx.x & (T / 64 - 1);
+    st.s = group_all<T / 64>(ps[w], Add());
+    st.e = group_all<T / 64>(pe[w], Add());
+    return st;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+inline int bad(const char *who, const char *why) {
+    mc_set_error("%s: %s", who, why);
+    return MC_ERR_ARG;
+}
+
+inline Div make_div(u64 d) {
+    Div r{(u32)d, 0, 0};
+    while ((1ull << r.shift) < d) ++r.shift;
+    r.mul = (u32)((((u64)1 << (31 + r.shift)) + d - 1) / d);
+    return r;
+}
+
+inline bool one_run(uint64_t inner, int64_t outer_stride, int64_t inner_stride) { return outer_stride == (int64_t)inner * inner_stride; }
+
+// the arguments that every entry point on logits shares (`flat`: everything else that a row has lies as one run too)
+inline int rows_of(const char *who, Rows &a, const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
+                   int64_t outer_stride, int64_t inner_stride, double temperature, bool flat) {
+    if (dtype > MC_LOGITS_BF16) return bad(who, "unknown element type");
+    if (vocab == 0 || vocab >= (1ull << 31) - 64) return bad(who, "the vocabulary holds 1 .. 2^31 - 65 tokens");
+    if (outer >= (1ull << 31) || inner >= (1ull << 31) || outer * inner >= (1ull << 31)) return bad(who, "at most 2^31 - 1 rows");
+    if (!(temperature >= 1e-30 && temperature <= 1e30)) return bad(who, "the temperature is a positive number (1e-30 .. 1e30)");
+    if (outer * inner && !logits) return bad(who, "no logits");
+    const int bytes = dtype == MC_LOGITS_F32 ? 4 : 2;
+    if ((uintptr_t)logits % bytes) return bad(who, "logits that are not aligned to their type");
+    a.rows = (u32)(outer * inner);
+    if (outer > 1 && flat && one_run(inner, outer_stride, inner_stride)) {
+        inner *= outer;
+        outer = 1;
+    }
+    a.logits = View{(const char *)logits, outer_stride * bytes, inner_stride * bytes};
+    a.inner = make_div(inner ? inner : 1);
+    a.vocab = (u32)vocab;
+    a.full = (u32)(vocab / (16 / bytes));
+    a.nvec = (u32)((vocab + 16 / bytes - 1) / (16 / bytes));
+    a.c = (float)(LOG2E / temperature);
+    return MC_OK;
+}
+
+inline int tokens_of(const char *who, Rows &a, const void *tokens, uint32_t token_bytes, int64_t outer_stride, int64_t inner_stride,
+                     uint64_t rows) {
+    if (token_bytes != 4 && token_bytes != 8) return bad(who, "token ids of 4 or 8 bytes");
+    if (rows && !tokens) return bad(who, "no tokens");
+    if ((uintptr_t)tokens % token_bytes) return bad(who, "tokens that are not aligned to their type");
+    a.token_bytes = token_bytes;
+    a.tokens = View{(const char *)tokens, outer_stride * (i64)token_bytes, inner_stride * (i64)token_bytes};
+    return MC_OK;
+}
+
+inline u32 rows_to_blocks(u32 rows, u32 group) { return (u32)(((u64)rows * group + BLOCK - 1) / BLOCK); }
+
+}  // namespace
+
+#define BY_TYPE(dtype, ...)                                                            \
+    switch (dtype) {                                                                   \
+        case MC_LOGITS_F32: { constexpr int DT = MC_LOGITS_F32; __VA_ARGS__; break; }  \
+        case MC_LOGITS_F16: { constexpr int DT = MC_LOGITS_F16; __VA_ARGS__; break; }  \
+        default: { constexpr int DT = MC_LOGITS_BF16; __VA_ARGS__; break; }            \
+    }
+
+// a group of as few lanes as hold a row
+#define BY_GROUP(nvec, ...)                                                 \
+    if ((nvec) <= 4 * SUB_NV) { constexpr int G = 4; __VA_ARGS__; }         \
+    else if ((nvec) <= 8 * SUB_NV) { constexpr int G = 8; __VA_ARGS__; }    \
+    else if ((nvec) <= 16 * SUB_NV) { constexpr int G = 16; __VA_ARGS__; }  \
+    else if ((nvec) <= 32 * SUB_NV) { constexpr int G = 32; __VA_ARGS__; }  \
+    else { constexpr int G = 64; __VA_ARGS__; }

@@ -1,0 +1,524 @@
+// Draws from rows of logits by inversion, and the keys of whole passwords (formulas: mc_logits_score.hip).
+//
+// The draw is defined by running sums in 64 bits, and these are what has to be computed: a vocabulary of 10^5 tokens puts
+// 10^5 ends of intervals into [0, Z), so that sums known to 10^-7 would leave the token open in every other row.  Weights
+// come from a polynomial that is right to 4e-11 (sixteen operations an element, which this GPU does at the rate of 32
+// bits); where u Z lies within 1e-10 Z of an end (a row in 10^5) the row is summed again with the library's exponential.
+// Exponents of 64 bits reach far enough that no maximum has to be known first: one pass.
+#include "mc_logits.h"
+#include "mc_philox.h"
+
+namespace {
+
+// 2^(x c) for x c in [-1000, 900]; lower ones as 2^-1000 (so far below any sum that `good` lets pass that it changes
+// nothing), NaN for NaN.  The whole part n goes to the exponent; on [-1/2, 1/2] the polynomial of degree 7 that
+// approximates 2^f best relative to its value (found by exchange of the extremal points; largest error 4.03e-11).
+struct Power {
+    double c;
+    float lo;
+    __device__ __forceinline__ double operator()(float x) const {
+        const double y = (double)maximum(x, lo) * c, t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+        double p = 0x1.fe1786b50da52p-17;
+        p = __builtin_fma(p, f, 0x1.446a1fdd54f3ap-13);
+        p = __builtin_fma(p, f, 0x1.5d8a7085cddb8p-10);
+        p = __builtin_fma(p, f, 0x1.3b29dc40d2ec5p-7);
+        p = __builtin_fma(p, f, 0x1.c6b08aaf3156ep-5);
+        p = __builtin_fma(p, f, 0x1.ebfbe0a4be886p-3);
+        p = __builtin_fma(p, f, 0x1.62e42ff11627ap-1);
+        p = __builtin_fma(p, f, 0x1.ffffffffabbccp-1);
+        return __hiloint2double(__double2hiint(p) + (int)((u32)__double2loint(t) << 20), __double2loint(p));
+    }
+};
+constexpr double MARGIN = 1e-10;
+
+// The draw's own weights: exp((x - m) / T) in 64 bits, m the row's largest logit.
+struct Definition {
+    double t, m;
+    __device__ __forceinline__ double operator()(float x) const { return exp(((double)x - m) / t); }
+};
+
+// whether sums of Power stand: no exponent was too large, not all were too small, and no NaN
+__device__ __forceinline__ bool good(double z, float m, double c) { return z >= 0x1p-900 && (double)m * c <= 900.; }
+
+// -log2 p of a token drawn under sums of Power
+__device__ __forceinline__ float ml2p_under(double z, double c, float x) {
+    int e;
+    const double m = frexp(z, &e);
+    return (float)(((double)e - (double)x * c) + (double)log2f((float)m));
+}
+
+struct DrawArgs {
+    const double *uniforms;  // or null: Philox
+    u64 seed, first_id;
+    u32 draw;
+    double t;
+    Power power;
+    const unsigned char *live;
+    int *token;
+    float *ml2p;
+};
+
+__device__ __forceinline__ double uniform_of(const DrawArgs &d, u32 row) {
+    if (d.uniforms) {
+        const double u = d.uniforms[row];
+        return u > 0. ? u : 0.;
+    }
+    const u64 id = d.first_id + row;
+    u32 o0, o1, o2, o3;
+    philox4x32_10((u32)id, (u32)(id >> 32), d.draw >> 1, 0u, (u32)d.seed, (u32)(d.seed >> 32), o0, o1, o2, o3);
+    const u32 a = d.draw & 1 ? o2 : o0, b = d.draw & 1 ? o3 : o1;
+    return (double)((u64)(a >> 5) << 26 | b >> 6) * 0x1p-53;
+}
+
+// ---- rows of few tokens --------------------------------------------------------------------------------------------------
+// The token of a group's row in registers: running sums in the order of the index, vector step by vector step.  False when
+// u Z lies within `margin` Z of an end of the token's interval (0 takes any answer).
+template <int DT, int G, typename W>
+__device__ __forceinline__ bool draw_sub(SubRow<DT> &r, const W &weight, double u, double margin, u32 &token, float &x, double &z, float &m) {
+    const u32 lane = threadIdx.x & (G - 1);
+    double s[SUB_NV];
+    z = 0.;
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        s[i] = 0.;
+        if (i < (int)r.nv) {
+            const raw4 q = vec_of<DT>(r, i);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float e = unpack<DT>(q, j);
+                m = maximum(m, e);
+                s[i] += weight(e);
+            }
+            z += s[i];
+        }
+    }
+    m = group_all<G>(m, Max());
+    z = group_all<G>(z, Add());
+    const double target = u * z;
+    // the vector step whose running sum passes the target, or the last one with any weight
+    double before = 0., run = 0., mine = 0.;
+    raw4 q = r.q[0];
+    u32 from = lane * VEC<DT>;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        if (i < (int)r.nv) {
+            const double step = group_all<G>(s[i], Add());
+            if (!found && step > 0.) {
+                before = run;
+                mine = s[i];
+                q = vec_of<DT>(r, i);
+                from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+                found = run + step > target;
+            }
+            run += step;
+        }
+    }
+    const double inc = group_scan<G>(mine), lo = before + (inc - mine);
+    const u32 shift = threadIdx.x & 63 & ~(G - 1);
+    const u64 all = G == 64 ? ~0ull : (1ull << (G & 63)) - 1;
+    const u64 passes = (__ballot(before + inc > target) >> shift) & all, some = (__ballot(mine > 0.) >> shift) & all;
+    // (a sum that passes by a rounding only, or none: the last lane with any weight)
+    const bool hit = found && passes;
+    const u32 who = hit ? (u32)__ffsll((unsigned long long)passes) - 1 : some ? 63u - (u32)__clzll((long long)some) : 0u;
+    double at_lo = lo;
+    u32 got = 0xFFFFFFFFu, last = 0;
+    float got_x = 0.f, last_x = 0.f;
+    bool ok = false;
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) {
+        const float e = unpack<DT>(q, j);
+        const double w = weight(e), next = at_lo + w;
+        if (w > 0.) {
+            last = from + j;
+            last_x = e;
+            if (got == 0xFFFFFFFFu && next > target) {
+                got = from + j;
+                got_x = e;
+                ok = hit && target - at_lo >= margin * z && next - target >= margin * z;
+            }
+        }
+        at_lo = next;
+    }
+    if (!hit || got == 0xFFFFFFFFu) got = last, got_x = last_x;
+    token = __shfl(got, who, G);
+    x = __shfl(got_x, who, G);
+    return __shfl((int)ok, who, G) || margin == 0.;
+}
+
+template <int DT, int G>
+__global__ __launch_bounds__(BLOCK) void k_logits_draw_sub(Rows a, DrawArgs d) {
+    const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows, live = there && (!d.live || d.live[row]);
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, live);
+    const double u = there ? uniform_of(d, row) : 0.;
+    u32 token;
+    float x, m;
+    double z;
+    bool sure = draw_sub<DT, G>(r, d.power, u, MARGIN, token, x, z, m) && good(z, m, d.power.c);
+    float ml2p = ml2p_under(z, d.power.c, x);
+    if (!live) sure = true, token = (u32)MC_TOKEN_SKIP, ml2p = 0.f;
+    if (__ballot(!sure)) {  // the whole wave decides again, from the definition
+        forget(r);
+        const Stat st = sub_stat<DT, G, false>(r, a.c);
+        u32 again;
+        float x_again, m_again;
+        double z_again;
+        draw_sub<DT, G>(r, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u, 0., again, x_again, z_again, m_again);
+        if (!sure) {
+            token = st.s > 0.f ? again : (u32)MC_TOKEN_OUTSIDE;
+            ml2p = ml2p_of(0, st, x_again, a.c);
+        }
+    }
+    if (there && lane == 0) {
+        d.token[row] = (int)token;
+        d.ml2p[row] = ml2p;
+    }
+}
+
+// ---- rows of many tokens ---------------------------------------------------------------------------------------------------
+constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 8;
+
+// The token by the definition's weights (every thread of the workgroup calls).
+template <int DT>
+__device__ __forceinline__ u32 draw_exact(const char *p, const Rows &a, const Definition &weight, double u) {
+    double mine = 0., total;
+    for (u32 v = threadIdx.x; v < a.nvec; v += WIDE) {
+#pragma unroll 1
+        for (u32 i = v * VEC<DT>; i < min((v + 1) * VEC<DT>, a.vocab); ++i) mine += weight(element<DT>(p, i));
+    }
+    block_scan<WIDE>(mine, total);
+    const double target = u * total;
+    double before = 0.;
+    u32 last = 0;
+    __shared__ u32 hit;
+    for (u32 base = 0; base < a.nvec; base += WIDE) {
+        const u32 from = (base + threadIdx.x) * VEC<DT>, to = min(from + VEC<DT>, a.vocab);
+        double s = 0., step;
+#pragma unroll 1
+        for (u32 i = from; i < to; ++i) {
+            const double w = weight(element<DT>(p, i));
+            if (w > 0.) last = i;
+            s += w;
+        }
+        const double lo = before + block_scan<WIDE>(s, step);
+        const u32 first = block_min<WIDE>(lo + s > target ? threadIdx.x : 0xFFFFFFFFu);
+        if (first != 0xFFFFFFFFu) {
+            if (threadIdx.x == first) {
+                double run = lo;
+                u32 got = 0xFFFFFFFFu;
+#pragma unroll 1
+                for (u32 i = from; i < to; ++i) {
+                    const double w = weight(element<DT>(p, i));
+                    run += w;
+                    if (got == 0xFFFFFFFFu && w > 0. && run > target) got = i;
+                }
+                hit = got != 0xFFFFFFFFu ? got : last;  // (the vector's sum exceeds the target, its running sum by a rounding not)
+            }
+            __syncthreads();
+            return hit;
+        }
+        before += step;
+    }
+    // u Z at or behind the last running sum: the last token with any weight
+    return 0xFFFFFFFFu - block_min<WIDE>(0xFFFFFFFFu - last);
+}
+
+struct LocateShared {
+    double sums[STEPS * WIDE_WAVES];
+    u32 token;
+    float x;
+    int sure;
+};
+
+// The token among vectors v0 .. v1, whose running sums begin at `before`: rounds of STEPS vectors a thread, of which every
+// wave's sum of every step is compared.
+template <int DT>
+__device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Rows &a, const Power &weight, u32 v0, u32 v1, double before,
+                                       double target, double margin, u32 &token, float &x) {
+    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (u32 base = v0; base < v1; base += WIDE * STEPS) {
+        raw4 q[STEPS];
+        double s[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(p, a, base + i * WIDE + threadIdx.x, v1);
+        if (threadIdx.x == 0) sh.sure = 0;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            s[i] = 0.;
+            if (base + i * WIDE < v1) {
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(q[i], j));
+            }
+            const double all = group_all<64>(s[i], Add());
+            if (lane == 0) sh.sums[i * WIDE_WAVES + wave] = all;
+        }
+        __syncthreads();
+        static_assert(STEPS * WIDE_WAVES == 64, "one lane for each sum");
+        const double mine = sh.sums[lane], inc = group_scan<64>(mine);
+        const u64 passes = __ballot(before + inc > target);
+        if (passes) {
+            const u32 which = (u32)__ffsll((unsigned long long)passes) - 1;
+            const double start = before + __shfl(inc - mine, which);
+            if (which % WIDE_WAVES == wave) {
+                const u32 step = which / WIDE_WAVES;
+                raw4 mq = q[0];
+                double ms = s[0];
+#pragma unroll
+                for (int i = 1; i < STEPS; ++i) {
+                    if (i == (int)step) mq = q[i], ms = s[i];
+                }
+                const double minc = group_scan<64>(ms);
+                const u64 over = __ballot(start + minc > target);
+                const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u;
+                if (lane == who) {
+                    double run = start + (minc - ms);
+                    int sure = 0;
+                    u32 got = 0;
+                    float got_x = 0.f;
+#pragma unroll
+                    for (int j = 0; j < VEC<DT>; ++j) {
+                        const float e = unpack<DT>(mq, j);
+                        const double next = run + weight(e);
+                        if (!sure && over && target - run >= margin && next - target >= margin) {
+                            sure = 1;
+                            got = (base + step * WIDE + threadIdx.x) * VEC<DT> + j;
+                            got_x = e;
+                        }
+                        run = next;
+                    }
+                    sh.token = got;
+                    sh.x = got_x;
+                    sh.sure = sure;
+                }
+            }
+            __syncthreads();
+            token = sh.token;
+            x = sh.x;
+            return sh.sure;
+        }
+        before += __shfl(inc, 63);
+        __syncthreads();
+    }
+    return false;
+}
+
+// How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose sums another launch joins.
+struct Split {
+    u32 shift, vecs;
+    double2 *stats;  // [row][part]: the sum, the largest logit
+};
+
+// the wave's sum and largest logit over its share of vectors v0 .. v1
+template <int DT, int STRIDE>
+__device__ __forceinline__ void sum_vecs(const char *p, const Rows &a, const Power &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
+    s = 0.;
+    m = -INFINITY;
+    for (u32 v = v0; v < v1; v += STRIDE * UNROLL) {
+        raw4 q[UNROLL];
+        load_chunk<DT, STRIDE>(q, p, a, v, lane, v1);
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float e = unpack<DT>(q[i], j);
+                m = maximum(m, e);
+                s += weight(e);
+            }
+    }
+    s = group_all<64>(s, Add());
+    m = group_all<64>(m, Max());
+}
+
+// the sums of the parts of a row
+template <int DT>
+__global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, Split sp) {
+    __shared__ double ps[BLOCK / 64];
+    __shared__ float pm[BLOCK / 64];
+    const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
+    if (row >= a.rows || (d.live && !d.live[row])) return;
+    const char *p = at(a.logits, a.inner, row);
+    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    double s;
+    float m;
+    sum_vecs<DT, BLOCK>(p, a, d.power, v0, v1, threadIdx.x, s, m);
+    if ((threadIdx.x & 63) == 0) {
+        ps[threadIdx.x >> 6] = s;
+        pm[threadIdx.x >> 6] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < BLOCK / 64; ++w) {
+            s += ps[w];
+            m = maximum(m, pm[w]);
+        }
+        sp.stats[id] = make_double2(s, (double)m);
+    }
+}
+
+// One workgroup a row: its waves' (or the parts') sums say in which of them the token lies; that part is looked at again.
+template <int DT, bool PART>
+__global__ __launch_bounds__(WIDE) void k_logits_draw(Rows a, DrawArgs d, Split sp) {
+    __shared__ LocateShared sh;
+    __shared__ double ps[WIDE_WAVES];
+    __shared__ float pm[WIDE_WAVES];
+    const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (row >= a.rows) return;
+    if (d.live && !d.live[row]) {
+        if (threadIdx.x == 0) {
+            d.token[row] = MC_TOKEN_SKIP;
+            d.ml2p[row] = 0.f;
+        }
+        return;
+    }
+    const char *p = at(a.logits, a.inner, row);
+    const double u = uniform_of(d, row);
+    u32 share;
+    double mine = 0.;
+    float m = -INFINITY;
+    if constexpr (PART) {
+        share = sp.vecs;
+        if (lane < (1u << sp.shift)) {
+            const double2 f = sp.stats[((u64)row << sp.shift) + lane];
+            mine = f.x;
+            m = (float)f.y;
+        }
+    } else {
+        share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES;
+        const u32 v0 = min(wave * share, a.nvec), v1 = min(a.nvec, v0 + share);
+        double s;
+        sum_vecs<DT, 64>(p, a, d.power, v0, v1, lane, s, m);
+        if (lane == 0) {
+            ps[wave] = s;
+            pm[wave] = m;
+        }
+        __syncthreads();
+        if (lane < WIDE_WAVES) mine = ps[lane];
+        m = lane < WIDE_WAVES ? pm[lane] : -INFINITY;
+    }
+    // lane i holds part i
+    m = group_all<64>(m, Max());
+    const double inc = group_scan<64>(mine), z = __shfl(inc, 63), target = u * z;
+    const u64 passes = __ballot(inc > target);
+    u32 token = 0;
+    float x = 0.f;
+    bool sure = false;
+    if (good(z, m, d.power.c) && passes) {
+        const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
+        sure = locate<DT>(sh, p, a, d.power, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
+    }
+    if (sure) {
+        if (threadIdx.x == 0) {
+            d.token[row] = (int)token;
+            d.ml2p[row] = ml2p_under(z, d.power.c, x);
+        }
+        return;
+    }
+    float top = -INFINITY;
+    for (u32 v = threadIdx.x; v < a.nvec; v += WIDE) {
+        const raw4 q = load_vec<DT>(p, a, v, a.nvec);
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) top = fmaxf(top, unpack<DT>(q, j));
+    }
+    const Stat st = exact_stat<DT, WIDE, false>(p, a, block_max<WIDE>(top));
+    if (st.s > 0.f) token = draw_exact<DT>(p, a, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u);
+    if (threadIdx.x == 0) {
+        d.token[row] = st.s > 0.f ? (int)token : MC_TOKEN_OUTSIDE;
+        d.ml2p[row] = ml2p_of(0, st, st.s > 0.f ? element<DT>(p, token) : 0.f, a.c);
+    }
+}
+
+// Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
+u32 split_shift(u32 rows, u32 nvec) {
+    if (nvec <= SUB_VECS) return 0;
+    u32 shift = 0;
+    while (shift < 6 && ((u64)rows << shift) < 512 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+    return shift;
+}
+
+size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * 16 : 0; }
+
+// ---- keys ----------------------------------------------------------------------------------------------------------
+// one lane a password
+__global__ __launch_bounds__(BLOCK) void k_logits_keys(const float *ml2p, const i64 *offsets, const void *lengths, u32 length_bytes,
+                                                       u64 count, i64 stride, u64 longest, double *out) {
+    for (u64 i = (u64)blockIdx.x * BLOCK + threadIdx.x; i < count; i += (u64)gridDim.x * BLOCK) {
+        u64 from = 0, to = 0;
+        const float *p = ml2p;
+        if (offsets) {
+            // (offsets that do not ascend or leave the array name no symbols: nothing is read through them)
+            const i64 lo = offsets[i], hi = offsets[i + 1];
+            if (lo >= 0 && hi > lo && (u64)hi <= longest) from = (u64)lo, to = (u64)hi;
+        } else {
+            p += (i64)i * stride;
+            const i64 n = length_bytes == 8 ? ((const i64 *)lengths)[i] : length_bytes == 4 ? (i64)((const int *)lengths)[i] : (i64)longest;
+            to = n < 0 ? 0 : (u64)n > longest ? longest : (u64)n;
+        }
+        double s = 0.;
+        for (u64 k = from; k < to; ++k) s += (double)p[k];
+        out[i] = s == INFINITY ? 1022.0 : s;
+    }
+}
+
+}  // namespace
+
+extern "C" size_t mc_logits_draw_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab) {
+    if (dtype > MC_LOGITS_BF16 || rows >= (1ull << 31) || vocab >= (1ull << 31)) return 0;
+    const u64 per = dtype == MC_LOGITS_F32 ? 4 : 8;
+    return split_bytes((u32)rows, split_shift((u32)rows, (u32)((vocab + per - 1) / per)));
+}
+
+extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows, uint64_t vocab, int64_t row_stride,
+                              double temperature, const double *uniforms, uint64_t seed, uint64_t first_id, uint32_t draw,
+                              const uint8_t *live, int32_t *out_token, float *out_ml2p, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+    const char *who = "mc_logits_draw";
+    Rows a{};
+    if (int rc = rows_of(who, a, logits, dtype, 1, rows, vocab, 0, row_stride, temperature, true)) return rc;
+    if (a.rows == 0) return MC_OK;
+    if (!out_token || !out_ml2p) return bad(who, "no output");
+    hipStream_t s = (hipStream_t)stream;
+    const double c = LOG2E / temperature;
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
+    if (a.nvec <= SUB_VECS) {
+        BY_TYPE(dtype, BY_GROUP(a.nvec, hipLaunchKernelGGL((k_logits_draw_sub<DT, G>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
+    } else {
+        Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
+        if (sp.shift) {
+            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
+                mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);
+                return MC_ERR_WORKSPACE;
+            }
+            const u32 each = (a.nvec + (1u << sp.shift) - 1) >> sp.shift;
+            sp.vecs = (each + BLOCK - 1) / BLOCK * BLOCK;
+            sp.stats = (double2 *)workspace;
+                BY_TYPE(dtype, {
+                hipLaunchKernelGGL((k_logits_draw_sums<DT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, d, sp);
+                hipLaunchKernelGGL((k_logits_draw<DT, true>), grid_of(a.rows), dim3(WIDE), 0, s, a, d, sp);
+            });
+        } else {
+                BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT, false>), grid_of(a.rows), dim3(WIDE), 0, s, a, d, sp));
+        }
+    }
+    HIP_TRY(hipGetLastError());
+    return MC_OK;
+}
+
+extern "C" int mc_logits_keys(const float *ml2p, const int64_t *offsets, const void *lengths, uint32_t length_bytes,
+                              uint64_t count, int64_t stride, uint64_t longest, double *out_keys, void *stream) {
+    const char *who = "mc_logits_keys";
+    if (count >= (1ull << 40)) return bad(who, "too many passwords");
+    if (offsets && lengths) return bad(who, "offsets or lengths, not both");
+    if (lengths && length_bytes != 4 && length_bytes != 8) return bad(who, "lengths of 4 or 8 bytes");
+    if (count == 0) return MC_OK;
+    if (!out_keys || (longest && !ml2p)) return bad(who, "null pointer");
+    const u64 blocks = (count + BLOCK - 1) / BLOCK;
+    hipLaunchKernelGGL(k_logits_keys, dim3((u32)(blocks < 65536 ? blocks : 65536)), dim3(BLOCK), 0, (hipStream_t)stream, ml2p,
+                       (const i64 *)offsets, lengths, lengths ? length_bytes : 0u, (u64)count, (i64)stride, (u64)longest, out_keys);
+    HIP_TRY(hipGetLastError());
+    return MC_OK;
+}

@@ -1,0 +1,316 @@
+// The gradient of weights * (-log2 p of the given token) + entropy weights * entropy for the logits, with both values
+// (formulas: mc_logits_score.hip).  A row is read once and its gradient written once while its vectors fit the registers
+// of a group of lanes or of one workgroup of up to 1024 lanes (131072 tokens of two bytes); longer rows, and
+// rows too few to fill the GPU, are summed part by part by one launch and written by a second one.
+#include "mc_logits.h"
+
+namespace {
+
+struct GradOut {
+    View weights, entropy_weights;  // entropy_weights.p may be null
+    float inv_t;
+    float *ml2p, *entropy;
+    char *grad;
+};
+
+// what the elements of a row's gradient need
+struct Slope {
+    float A, B, inv, off;
+    bool none;
+    int tok;
+};
+
+template <bool ENT>
+__device__ __forceinline__ Slope slope_of(const Rows &a, const GradOut &out, u32 row, int tok, const Stat &st) {
+    Slope s;
+    s.none = tok == MC_TOKEN_SKIP || st.s == 0.f;
+    s.A = tok >= 0 ? *(const float *)at(out.weights, a.inner, row) * a.c : 0.f;
+    s.B = ENT ? *(const float *)at(out.entropy_weights, a.inner, row) * out.inv_t : 0.f;
+    s.inv = s.none ? 0.f : 1.f / st.s;
+    s.off = ENT && !s.none ? entropy_of(tok, st) - log2f(st.s) : 0.f;  // log2 p + H = y + off
+    s.tok = tok;
+    return s;
+}
+
+template <int DT, bool ENT, bool EXACT>
+__device__ __forceinline__ void slope_vec(const raw4 &q, u32 from, const Slope &s, const Expo &y_of, float *g) {
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) {
+        const float x = unpack<DT>(q, j), y = EXACT ? y_of(x) : y_of.fast(x), p = exp2_(y) * s.inv;
+        g[j] = ENT ? p * (s.A - s.B * (fmaxf(y, -FAR) + s.off)) : p * s.A;
+    }
+    const u32 t = (u32)s.tok - from;
+    if (t < (u32)VEC<DT>) {
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) g[j] -= t == (u32)j ? s.A : 0.f;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void put_zeros(char *gp, u32 from, u32 vocab) {
+    float g[VEC<DT>];
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
+    store_at<DT>(gp, from, vocab, g);
+}
+
+template <int DT, int G, bool ENT>
+__global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOut out) {
+    const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows;
+    const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    if (!there) return;
+    if (lane == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+    }
+    const Slope s = slope_of<ENT>(a, out, row, tok, st);
+    const Expo y_of(st, a.c);
+    char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
+#pragma unroll
+    for (int i = 0; i < SUB_NV; ++i) {
+        const u32 v = i * G + lane;
+        if (i < (int)r.nv && v < a.nvec) {
+            // (a last vector that reaches back computes and stores there what the one before it does)
+            const u32 from = a.vocab < VEC<DT> ? 0u : min(v * VEC<DT>, a.vocab - VEC<DT>);
+            if (s.none) {
+                put_zeros<DT>(gp, from, a.vocab);
+            } else {
+                float g[VEC<DT>];
+                slope_vec<DT, ENT, true>(r.q[i], from, s, y_of, g);
+                store_at<DT>(gp, from, a.vocab, g);
+            }
+        }
+    }
+}
+
+// one workgroup a row, the row in its registers
+constexpr int HELD = 8;  // vectors a lane holds
+
+template <int DT, int T, bool ENT>
+__global__ __launch_bounds__(T, 8) void k_logits_gradient_held(Rows a, GradOut out) {
+    const u32 row = block_id();
+    if (row >= a.rows) return;
+    const int tok = token_of(a, row);
+    const char *p = at(a.logits, a.inner, row);
+    char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
+    const u32 nv = (a.nvec + T - 1) / T;
+    if (tok == MC_TOKEN_SKIP) {
+        if (threadIdx.x == 0) {
+            out.ml2p[row] = 0.f;
+            if (ENT) out.entropy[row] = 0.f;
+        }
+        for (u32 v = threadIdx.x; v < a.nvec; v += T) put_zeros<DT>(gp, v * VEC<DT>, a.vocab);
+        return;
+    }
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    raw4 q[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (i < (int)nv) q[i] = load_vec<DT>(p, a, i * T + threadIdx.x, a.nvec);
+    }
+    Stat st{-INFINITY, 0.f, 0.f, false};
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (i < (int)nv) {
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) st.m = maximum(st.m, unpack<DT>(q[i], j));
+        }
+    }
+    {
+        const Expo y_of(st, a.c);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            asm("" : "+v"(q[i]));  // (see forget)
+            if (i < (int)nv) {
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) {
+                    const float y = y_of.fast(unpack<DT>(q[i], j)), w = exp2_(y);
+                    st.s += w;
+                    if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
+                }
+            }
+        }
+    }
+    st = block_stat<T, ENT>(st, a.c);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) asm("" : "+v"(q[i]));
+    if (doubtful(st, a.c)) st = exact_stat<DT, T, ENT>(p, a, st.m);
+    if (threadIdx.x == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+    }
+    const Slope s = slope_of<ENT>(a, out, row, tok, st);
+    const Expo y_of(st, a.c);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const u32 v = i * T + threadIdx.x;
+        if (i < (int)nv && v < a.nvec) {
+            float g[VEC<DT>];
+            if (s.none) {
+                put_zeros<DT>(gp, v * VEC<DT>, a.vocab);
+                continue;
+            }
+            if (st.exact) slope_vec<DT, ENT, true>(q[i], v * VEC<DT>, s, y_of, g);
+            else slope_vec<DT, ENT, false>(q[i], v * VEC<DT>, s, y_of, g);
+            store_at<DT>(gp, v * VEC<DT>, a.vocab, g);
+        }
+    }
+}
+
+// 2^shift workgroups of `vecs` vectors a row
+struct Split {
+    u32 shift, vecs;
+    float4 *stats;  // [row][part]: m, s, e
+};
+
+template <int DT, bool ENT>
+__global__ __launch_bounds__(BLOCK) void k_logits_gradient_sums(Rows a, Split sp) {
+    const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
+    if (row >= a.rows || token_of(a, row) == MC_TOKEN_SKIP) return;
+    const char *p = at(a.logits, a.inner, row);
+    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    Stat st{-INFINITY, 0.f, 0.f, false};
+    for (u32 v = v0; v < v1; v += BLOCK * UNROLL) {
+        raw4 q[UNROLL];
+        load_chunk<DT, BLOCK>(q, p, a, v, threadIdx.x, v1);
+        take<DT, ENT>(st, q, a.c);
+    }
+    st = block_stat<BLOCK, ENT>(st, a.c);
+    if (threadIdx.x == 0) sp.stats[id] = make_float4(st.m, st.s, st.e, 0.f);
+}
+
+// A row's statistics joined into its first part's place, and its outputs: before any part of the row is written, since
+// the gradient may take the logits' place.
+template <int DT, bool ENT>
+__global__ __launch_bounds__(BLOCK) void k_logits_gradient_join(Rows a, GradOut out, Split sp) {
+    const u32 row = block_id(), lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
+    const int tok = token_of(a, row);
+    const char *p = at(a.logits, a.inner, row);
+    Stat st{-INFINITY, 0.f, 0.f, false};
+    if (tok != MC_TOKEN_SKIP) {
+        if (lane < (1u << sp.shift)) {
+            const float4 f = sp.stats[((u64)row << sp.shift) + lane];
+            st = Stat{f.x, f.y, f.z, false};
+        }
+        st = group_stat<64, ENT>(st, a.c);
+        if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+    }
+    __syncthreads();  // (every wave has read the parts)
+    if (threadIdx.x == 0) {
+        sp.stats[(u64)row << sp.shift] = make_float4(st.m, st.s, st.e, st.exact ? 1.f : 0.f);
+        out.ml2p[row] = ml2p_of(tok, st, tok >= 0 ? element<DT>(p, tok) : 0.f, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+    }
+}
+
+template <int DT, bool ENT>
+__global__ __launch_bounds__(BLOCK) void k_logits_gradient_parts(Rows a, GradOut out, Split sp) {
+    const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
+    if (row >= a.rows) return;
+    const int tok = token_of(a, row);
+    const char *p = at(a.logits, a.inner, row);
+    char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
+    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    const float4 f = sp.stats[(u64)row << sp.shift];
+    const Stat st{f.x, f.y, f.z, f.w != 0.f};
+    const Slope s = slope_of<ENT>(a, out, row, tok, st);
+    const Expo y_of(st, a.c);
+    for (u32 v = v0; v < v1; v += BLOCK * UNROLL) {
+        raw4 q[UNROLL];
+        if (!s.none) load_chunk<DT, BLOCK>(q, p, a, v, threadIdx.x, v1);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const u32 mine = v + u * BLOCK + threadIdx.x;
+            if (mine >= v1) continue;
+            float g[VEC<DT>];
+            if (s.none) {
+                put_zeros<DT>(gp, mine * VEC<DT>, a.vocab);
+                continue;
+            }
+            if (st.exact) slope_vec<DT, ENT, true>(q[u], mine * VEC<DT>, s, y_of, g);
+            else slope_vec<DT, ENT, false>(q[u], mine * VEC<DT>, s, y_of, g);
+            store_at<DT>(gp, mine * VEC<DT>, a.vocab, g);
+        }
+    }
+}
+
+// Parts while there are too few rows to fill the GPU with one workgroup each, or a row is longer than one holds.
+u32 split_shift(u32 rows, u32 nvec) {
+    if (nvec <= SUB_VECS) return 0;
+    u32 shift = 0;
+    while (shift < 6 && ((u64)rows << shift) < 256 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+    while (shift < 6 && nvec > 1024 * HELD && (nvec >> shift) > 1024 * HELD / 2) ++shift;
+    return shift;
+}
+
+size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * 16 : 0; }
+
+template <int DT, bool ENT>
+void launch(const Rows &a, const GradOut &out, const Split &sp, hipStream_t s) {
+    if (a.nvec <= SUB_VECS) {
+        BY_GROUP(a.nvec, hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, ENT>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out));
+    } else if (sp.shift) {
+        hipLaunchKernelGGL((k_logits_gradient_sums<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, sp);
+        hipLaunchKernelGGL((k_logits_gradient_join<DT, ENT>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_gradient_parts<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, out, sp);
+    } else if (a.nvec <= 256 * HELD) {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 256, ENT>), grid_of(a.rows), dim3(256), 0, s, a, out);
+    } else if (a.nvec <= 512 * HELD) {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 512, ENT>), grid_of(a.rows), dim3(512), 0, s, a, out);
+    } else {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 1024, ENT>), grid_of(a.rows), dim3(1024), 0, s, a, out);
+    }
+}
+
+}  // namespace
+
+extern "C" size_t mc_logits_gradient_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab) {
+    if (dtype > MC_LOGITS_BF16 || rows >= (1ull << 31) || vocab >= (1ull << 31)) return 0;
+    const u64 per = dtype == MC_LOGITS_F32 ? 4 : 8;
+    return split_bytes((u32)rows, split_shift((u32)rows, (u32)((vocab + per - 1) / per)));
+}
+
+extern "C" int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
+                                  int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
+                                  int64_t token_outer_stride, int64_t token_inner_stride, double temperature,
+                                  const float *weights, int64_t weight_outer_stride, int64_t weight_inner_stride,
+                                  const float *entropy_weights, int64_t entropy_outer_stride, int64_t entropy_inner_stride,
+                                  float *out_ml2p, float *out_entropy, void *out_grad, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+    const char *who = "mc_logits_gradient";
+    Rows a{};
+    if (int rc = tokens_of(who, a, tokens, token_bytes, token_outer_stride, token_inner_stride, outer * inner)) return rc;
+    const bool flat = one_run(inner, token_outer_stride, token_inner_stride) && one_run(inner, weight_outer_stride, weight_inner_stride) &&
+                      (!entropy_weights || one_run(inner, entropy_outer_stride, entropy_inner_stride));
+    if (int rc = rows_of(who, a, logits, dtype, outer, inner, vocab, outer_stride, inner_stride, temperature, flat)) return rc;
+    if (a.rows == 0) return MC_OK;
+    if (!weights) return bad(who, "no weights");
+    if (!out_ml2p || !out_grad || (entropy_weights && !out_entropy)) return bad(who, "no output");
+    if ((uintptr_t)out_grad % (dtype == MC_LOGITS_F32 ? 4 : 2)) return bad(who, "a gradient that is not aligned to its type");
+    GradOut out{View{(const char *)weights, weight_outer_stride * 4, weight_inner_stride * 4},
+                View{(const char *)entropy_weights, entropy_outer_stride * 4, entropy_inner_stride * 4},
+                (float)(1.0 / temperature), out_ml2p, out_entropy, (char *)out_grad};
+    Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
+    if (sp.shift) {
+        if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
+            mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);
+            return MC_ERR_WORKSPACE;
+        }
+        const u32 each = (a.nvec + (1u << sp.shift) - 1) >> sp.shift;
+        sp.vecs = (each + BLOCK - 1) / BLOCK * BLOCK;
+        sp.stats = (float4 *)workspace;
+    }
+    BY_TYPE(dtype, {
+        if (entropy_weights) launch<DT, true>(a, out, sp, (hipStream_t)stream);
+        else launch<DT, false>(a, out, sp, (hipStream_t)stream);
+    });
+    HIP_TRY(hipGetLastError());
+    return MC_OK;
+}

@@ -1,0 +1,460 @@
+// A language model's answer -- a row of logits x over V tokens for every place -- turned into what the Monte Carlo
+// path works on (gfx950): the score of given tokens (calc_ml2p), with entropy and the most probable alternatives; the
+// gradient of that score (mc_logits_gradient.hip); draws with their probability (pick_expand, lib4mc/ProbLib.py:31-43) and
+// the float64 keys of whole passwords (mc_logits_draw.hip).  With c = log2(e) / T, m the row's largest logit,
+// y = (x - m) c <= 0, w = 2^y and Z the sum of w:
+//
+//   score      -log2 p_t = log2 Z - y_t,   H = log2 Z - (sum of w y) / Z          (bits)
+//   gradient   d/dx_i of a * (-log2 p_t) + b * H = (a (p_i - [i = t]) / ln 2 - b p_i (log2 p_i + H)) / T
+//   draw       the first token whose running sum of weights exceeds u Z
+//   keys       the sum of a password's -log2 p in 64 bits
+//
+// A row holds 10^2 .. 10^5 numbers that are read once: every kernel here is bound by HBM, then by the eight to ten
+// operations an element takes.  One pass keeps the running maximum, the sum scaled to it and the sum of w y in 32 bits
+// (all terms are positive or all negative: no cancellation); a change of the maximum scales both.
+#include "mc_logits.h"
+
+namespace {
+
+struct ScoreOut {
+    float *ml2p, *entropy, *top_ml2p;
+    int *top;
+    u32 k;
+};
+
+// The order of alternatives is that of the logits themselves (equal logits: the lower index), so it never depends on a
+// rounding.  A logit as a word whose unsigned order is the numbers' (both zeros alike):
+__device__ __forceinline__ u32 order_of(float x) {
+    const u32 b = __float_as_uint(x + 0.0f);
+    return b ^ ((u32)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(u32 o) { return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu)); }
+constexpr u32 ORDER_NEG_INF = 0x007FFFFFu;
+
+// a candidate: larger for a larger logit and, among equals, for a lower index; 0: none
+__device__ __forceinline__ u64 key_of(u32 order, u32 index) { return (u64)order << 32 | (0xFFFFFFFFu - index); }
+__device__ __forceinline__ u32 index_of(u64 key) { return 0xFFFFFFFFu - (u32)key; }
+
+// one alternative's outputs
+__device__ __forceinline__ void put_top(const ScoreOut &out, u32 row, u32 rank, u64 key, const Stat &st, float c) {
+    const float v = log2f(st.s) - Expo(st, c)(value_of((u32)(key >> 32)));
+    out.top[(u64)row * out.k + rank] = v < INFINITY ? (int)index_of(key) : MC_TOKEN_OUTSIDE;
+    out.top_ml2p[(u64)row * out.k + rank] = v < INFINITY ? v : INFINITY;
+}
+
+// ---- rows of few tokens --------------------------------------------------------------------------------------------------
+// The k largest of a row in registers, one after the other: the largest that comes behind the last one in the order.
+template <int DT, int G>
+__device__ __forceinline__ void sub_top(SubRow<DT> &r, const Rows &a, const Stat &st, const ScoreOut &out, u32 row, bool writes, int tok) {
+    const u32 lane = threadIdx.x & (G - 1);
+    const bool blank = tok == MC_TOKEN_SKIP || !(st.s > 0.f);
+    float last = INFINITY;
+    u32 last_i = 0xFFFFFFFFu;
+    for (u32 k = 0; k < out.k; ++k) {
+        forget(r);
+        float best = -INFINITY;
+        u32 best_i = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < SUB_NV; ++i) {
+            if (i < (int)r.nv) {
+                const raw4 q = vec_of<DT>(r, i);
+                const u32 from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) {
+                    const float x = unpack<DT>(q, j);
+                    const bool open = x < last || (x == last && from + j > last_i);
+                    if (open && x > best) best = x, best_i = from + j;
+                }
+            }
+        }
+        const float top = group_all<G>(best, Max());
+        u32 at = best == top ? best_i : 0xFFFFFFFFu;
+#pragma unroll
+        for (int d = 1; d < G; d <<= 1) at = min(at, (u32)__shfl_xor(at, d));
+        if (writes && lane == 0) {
+            if (!blank && top > -INFINITY) {
+                put_top(out, row, k, key_of(order_of(top), at), st, a.c);
+            } else {
+                out.top[(u64)row * out.k + k] = tok == MC_TOKEN_SKIP ? MC_TOKEN_SKIP : MC_TOKEN_OUTSIDE;
+                out.top_ml2p[(u64)row * out.k + k] = tok == MC_TOKEN_SKIP ? 0.f : st.s == st.s ? INFINITY : st.s;
+            }
+        }
+        last = top;
+        last_i = at;
+    }
+}
+
+template <int DT, int G, bool ENT, bool TOP>
+__global__ __launch_bounds__(BLOCK, TOP ? 6 : 8) void k_logits_score_sub(Rows a, ScoreOut out) {
+    const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
+    const bool there = row < a.rows;
+    const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
+    const char *p = there ? at(a.logits, a.inner, row) : nullptr;
+    SubRow<DT> r;
+    load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    if (there && lane == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT && out.entropy) out.entropy[row] = entropy_of(tok, st);
+    }
+    if constexpr (TOP) sub_top<DT, G>(r, a, st, out, row, there, tok);
+}
+
+// ---- rows of many tokens ---------------------------------------------------------------------------------------------------
+constexpr int CELL_ROWS = 16;  // cells of a thread
+constexpr u32 LIST_CAP = 256, CAND_CAP = 512;
+
+// A pass over the row keeps, beside its sums, the largest logit of every cell (one thread's vectors of some chunks) and,
+// by lane, of all threads of that lane.  The k-th largest of these 64 is a lower bound of the k-th largest of all (about 64
+// ln(64 / (64 - k)) logits of a random row reach it): only the cells that do are looked at again.
+struct TopShared {
+    float lanes[BLOCK];
+    u64 cand[CAND_CAP];
+    u32 list[LIST_CAP];
+    u32 n_list, n_cand;
+};
+
+// An order word among the wave's 64 that at least k of them reach: the least that reaches the k-th's first 16 bits.
+__device__ __forceinline__ u32 bound_of(u32 o, u32 k) {
+    u32 b = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const u32 t = b | (1u << bit);
+        if ((u32)__popcll(__ballot(o >= t)) >= k) b = t;
+    }
+    u32 least = o >= b ? o : 0xFFFFFFFFu;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) least = min(least, (u32)__shfl_xor(least, d));
+    return least;
+}
+
+template <int DT>
+__device__ __forceinline__ u32 count_from(const char *row, const Rows &a, u32 v0, u32 v1, u32 order) {
+    u32 n = 0;
+    for (u32 v = v0 + threadIdx.x; v < v1; v += BLOCK) {
+        const raw4 q = load_vec<DT>(row, a, v, v1);
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) n += order_of(unpack<DT>(q, j)) >= order;
+    }
+    return block_sum<BLOCK>(n);
+}
+
+// The k largest when the candidates do not fit (rows of equal logits, orders made to defeat the cells): the k-th largest
+// value by bits, unless `bound` is it already; then one pass in order of the index.
+template <int DT>
+__device__ __forceinline__ u32 select_by_bits(TopShared &sh, const char *row, const Rows &a, u32 v0, u32 v1, u32 k, u32 bound) {
+    u32 kth = bound, above;
+    if (bound <= ORDER_NEG_INF) {  // fewer than k lanes hold anything: there may be fewer than k candidates
+        k = min(k, count_from<DT>(row, a, v0, v1, ORDER_NEG_INF + 1));
+        if (k == 0) return 0;
+        above = 0xFFFFFFFFu;
+    } else {
+        above = count_from<DT>(row, a, v0, v1, bound + 1);
+    }
+    if (above >= k) {
+        kth = 0;
+        for (int b = 31; b >= 0; --b) {
+            const u32 t = kth | (1u << b);
+            if (count_from<DT>(row, a, v0, v1, t) >= k) kth = t;
+        }
+        above = count_from<DT>(row, a, v0, v1, kth + 1);
+    }
+    const u32 equal = k - above;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n_cand = equal;  // (those above come behind the equal ones, in any order)
+    __syncthreads();
+    u32 found = 0, base = v0;
+    for (; base < v1 && found < equal; base += BLOCK) {
+        const u32 v = base + threadIdx.x;
+        const raw4 q = load_vec<DT>(row, a, v, v1);
+        u32 n = 0;
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) n += order_of(unpack<DT>(q, j)) == kth;
+        u32 total, place = found + block_scan<BLOCK>(n, total);
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) {
+            const u32 o = order_of(unpack<DT>(q, j)), i = v * VEC<DT> + j;
+            if (o == kth && place < equal) sh.cand[place] = key_of(o, i);
+            place += o == kth;
+            if (o > kth) sh.cand[atomicAdd(&sh.n_cand, 1u)] = key_of(o, i);
+        }
+        found += total;
+    }
+    if (above) {
+        for (u32 v = base + threadIdx.x; v < v1; v += BLOCK) {
+            const raw4 q = load_vec<DT>(row, a, v, v1);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const u32 o = order_of(unpack<DT>(q, j));
+                if (o > kth) sh.cand[atomicAdd(&sh.n_cand, 1u)] = key_of(o, v * VEC<DT> + j);
+            }
+        }
+    }
+    __syncthreads();
+    return k;
+}
+
+// candidates for the k largest of vectors v0 .. v1 into sh.cand: their number (sh.lanes holds the threads' largest)
+template <int DT>
+__device__ __forceinline__ u32 select(TopShared &sh, const float *cells, const char *row, const Rows &a, u32 v0, u32 v1, u32 k, u32 per_cell) {
+    if (threadIdx.x == 0) sh.n_list = sh.n_cand = 0;
+    __syncthreads();
+    float lm = sh.lanes[threadIdx.x & 63];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; ++w) lm = fmaxf(lm, sh.lanes[w * 64 + (threadIdx.x & 63)]);
+    const u32 bound = bound_of(order_of(lm), k);
+    const u32 cell_vecs = per_cell * UNROLL;
+    for (u32 r = 0; v0 + r * cell_vecs * BLOCK < v1; ++r) {
+        const float m = cells[r * BLOCK + threadIdx.x];
+        if (m > -INFINITY && order_of(m) >= bound) {
+            const u32 n = atomicAdd(&sh.n_list, 1u);
+            if (n < LIST_CAP) sh.list[n] = r * BLOCK + threadIdx.x;
+        }
+    }
+    __syncthreads();
+    const u32 n_list = sh.n_list;
+    if (n_list <= LIST_CAP) {
+        for (u32 i = threadIdx.x; i < n_list * cell_vecs; i += BLOCK) {
+            const u32 cell = sh.list[i / cell_vecs], u = i % cell_vecs;
+            const u32 v = v0 + ((cell / BLOCK) * cell_vecs + u) * BLOCK + cell % BLOCK;
+            const raw4 q = load_vec<DT>(row, a, v, v1);
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float x = unpack<DT>(q, j);
+                if (x > -INFINITY && order_of(x) >= bound) {
+                    const u32 n = atomicAdd(&sh.n_cand, 1u);
+                    if (n < CAND_CAP) sh.cand[n] = key_of(order_of(x), v * VEC<DT> + j);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const u32 n = sh.n_cand;
+    if (n_list <= LIST_CAP && n <= CAND_CAP) return n;
+    return select_by_bits<DT>(sh, row, a, v0, v1, k, bound);
+}
+
+// How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose statistics (and candidates, by place and part)
+// another launch joins.
+struct Split {
+    u32 shift, vecs;
+    float4 *stats;  // [row][part]: m, s, e
+    u64 *keys;      // [row][place][part]
+};
+
+__device__ __forceinline__ void put_skipped(const ScoreOut &out, u32 row) {
+    if (threadIdx.x == 0) {
+        out.ml2p[row] = 0.f;
+        if (out.entropy) out.entropy[row] = 0.f;
+    }
+    if (threadIdx.x < out.k) {
+        out.top[(u64)row * out.k + threadIdx.x] = MC_TOKEN_SKIP;
+        out.top_ml2p[(u64)row * out.k + threadIdx.x] = 0.f;
+    }
+}
+
+// a row's statistics are known (to all threads): its outputs, with n candidates for the alternatives
+__device__ __forceinline__ void put_row(const ScoreOut &out, u32 row, int tok, float x, const Stat &st, float c, const u64 *cand, u32 n) {
+    if (threadIdx.x == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, c);
+        if (out.entropy) out.entropy[row] = entropy_of(tok, st);
+    }
+    if (!out.k) return;
+    if (!(st.s > 0.f)) n = 0;
+    for (u32 i = threadIdx.x; i < n; i += BLOCK) {
+        const u64 key = cand[i];
+        u32 rank = 0;
+        for (u32 j = 0; j < n; ++j) rank += cand[j] > key;
+        if (rank < out.k) put_top(out, row, rank, key, st, c);
+    }
+    for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) {
+        out.top[(u64)row * out.k + i] = MC_TOKEN_OUTSIDE;
+        out.top_ml2p[(u64)row * out.k + i] = st.s == st.s ? INFINITY : st.s;
+    }
+}
+
+template <int DT, bool ENT, bool TOP, bool PART>
+__global__ __launch_bounds__(BLOCK, 8) void k_logits_score(Rows a, ScoreOut out, Split sp) {
+    __shared__ typename std::conditional<TOP, TopShared, int>::type sh;
+    extern __shared__ float cells[];
+    const u32 id = block_id(), row = PART ? id >> sp.shift : id, part = PART ? id & ((1u << sp.shift) - 1) : 0;
+    if (row >= a.rows) return;
+    const int tok = token_of(a, row);
+    if (tok == MC_TOKEN_SKIP) {
+        if (!PART) put_skipped(out, row);
+        return;
+    }
+    const char *p = at(a.logits, a.inner, row);
+    const float x = !PART && tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const u32 v0 = PART ? min(part * sp.vecs, a.nvec) : 0, v1 = PART ? min(a.nvec, v0 + sp.vecs) : a.nvec;
+    const u32 chunks = (v1 - v0 + BLOCK * UNROLL - 1) / (BLOCK * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
+    Stat st{-INFINITY, 0.f, 0.f, false};
+    float cell = -INFINITY;
+    for (u32 ch = 0, in = 0, r = 0; ch < chunks; ++ch) {
+        raw4 q[UNROLL];
+        load_chunk<DT, BLOCK>(q, p, a, v0 + ch * BLOCK * UNROLL, threadIdx.x, v1);
+        const float m = take<DT, ENT>(st, q, a.c);
+        if constexpr (TOP) {
+            cell = maximum(cell, m);
+            if (++in == per_cell || ch + 1 == chunks) {
+                cells[r++ * BLOCK + threadIdx.x] = cell;
+                cell = -INFINITY;
+                in = 0;
+            }
+        }
+    }
+    if constexpr (TOP) sh.lanes[threadIdx.x] = st.m;
+    st = block_stat<BLOCK, ENT>(st, a.c);
+    if constexpr (PART) {
+        if (threadIdx.x == 0) sp.stats[id] = make_float4(st.m, st.s, st.e, 0.f);
+        if constexpr (TOP) {
+            const u32 n = select<DT>(sh, cells, p, a, v0, v1, out.k, per_cell);
+            u64 *keys = sp.keys + ((u64)row * out.k << sp.shift) + part;
+            for (u32 i = threadIdx.x; i < n; i += BLOCK) {
+                const u64 key = sh.cand[i];
+                u32 rank = 0;
+                for (u32 j = 0; j < n; ++j) rank += sh.cand[j] > key;
+                if (rank < out.k) keys[rank << sp.shift] = key;
+            }
+            for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) keys[i << sp.shift] = 0;
+        }
+    } else {
+        if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+        u32 n = 0;
+        const u64 *cand = nullptr;
+        if constexpr (TOP) {
+            if (st.s > 0.f) n = select<DT>(sh, cells, p, a, v0, v1, out.k, per_cell);
+            cand = sh.cand;
+        }
+        put_row(out, row, tok, x, st, a.c, cand, n);
+    }
+}
+
+// the parts of a row joined
+template <int DT, bool ENT, bool TOP>
+__global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut out, Split sp) {
+    __shared__ typename std::conditional<TOP, TopShared, int>::type sh;
+    const u32 row = block_id();
+    if (row >= a.rows) return;
+    const int tok = token_of(a, row);
+    if (tok == MC_TOKEN_SKIP) {
+        put_skipped(out, row);
+        return;
+    }
+    const char *p = at(a.logits, a.inner, row);
+    const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
+    const u32 parts = 1u << sp.shift, lane = threadIdx.x & 63;
+    Stat st{-INFINITY, 0.f, 0.f, false};
+    if (lane < parts) {
+        const float4 f = sp.stats[((u64)row << sp.shift) + lane];
+        st = Stat{f.x, f.y, f.z, false};
+    }
+    st = group_stat<64, ENT>(st, a.c);
+    if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+    u32 n = 0;
+    const u64 *cand = nullptr;
+    if constexpr (TOP) {
+        const u32 total = out.k << sp.shift;
+        const u64 *keys = sp.keys + (u64)row * total;
+        u32 lm = 0;
+        for (u32 i = threadIdx.x; i < total; i += BLOCK) lm = max(lm, (u32)(keys[i] >> 32));
+        if (threadIdx.x == 0) sh.n_cand = 0;
+        sh.lanes[threadIdx.x] = __uint_as_float(lm);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < BLOCK / 64; ++w) lm = max(lm, __float_as_uint(sh.lanes[w * 64 + lane]));
+        const u32 bound = bound_of(lm, out.k);
+        for (u32 i = threadIdx.x; i < total; i += BLOCK) {
+            const u64 key = keys[i];
+            if (key && (u32)(key >> 32) >= bound) {
+                const u32 at = atomicAdd(&sh.n_cand, 1u);
+                if (at < CAND_CAP) sh.cand[at] = key;
+            }
+        }
+        __syncthreads();
+        n = sh.n_cand;
+        if (n > CAND_CAP) n = select_by_bits<DT>(sh, p, a, 0, a.nvec, out.k, bound);
+        cand = sh.cand;
+    }
+    put_row(out, row, tok, x, st, a.c, cand, n);
+}
+
+// Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
+u32 split_shift(u32 rows, u32 nvec) {
+    if (nvec <= SUB_VECS) return 0;
+    u32 shift = 0;
+    while (shift < 6 && ((u64)rows << shift) < 1024 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+    return shift;
+}
+
+u32 split_vecs(u32 nvec, u32 shift) {
+    const u32 each = (nvec + (1u << shift) - 1) >> shift;
+    return (each + BLOCK * UNROLL - 1) / (BLOCK * UNROLL) * (BLOCK * UNROLL);
+}
+
+size_t split_bytes(u32 rows, u32 shift, u32 top) { return shift ? ((size_t)rows << shift) * (16 + 8 * (size_t)top) : 0; }
+
+template <int DT, bool ENT, bool TOP>
+void launch(const Rows &a, const ScoreOut &out, Split sp, hipStream_t s) {
+    const u32 chunks = ((sp.shift ? sp.vecs : a.nvec) + BLOCK * UNROLL - 1) / (BLOCK * UNROLL);
+    const u32 per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
+    const size_t lds = TOP ? (chunks + per_cell - 1) / per_cell * BLOCK * sizeof(float) : 0;
+    if (sp.shift) {
+        hipLaunchKernelGGL((k_logits_score<DT, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK), lds, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_score_join<DT, ENT, TOP>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
+    } else {
+        hipLaunchKernelGGL((k_logits_score<DT, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), lds, s, a, out, sp);
+    }
+}
+
+}  // namespace
+
+extern "C" size_t mc_logits_score_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab, uint32_t top) {
+    if (dtype > MC_LOGITS_BF16 || rows >= (1ull << 31) || vocab >= (1ull << 31) || top > MC_LOGITS_MAX_TOP) return 0;
+    const u64 per = dtype == MC_LOGITS_F32 ? 4 : 8;
+    return split_bytes((u32)rows, split_shift((u32)rows, (u32)((vocab + per - 1) / per)), top);
+}
+
+extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
+                               int64_t outer_stride, int64_t inner_stride, const void *tokens, uint32_t token_bytes,
+                               int64_t token_outer_stride, int64_t token_inner_stride, double temperature, float *out_ml2p,
+                               float *out_entropy, uint32_t top, int32_t *out_top, float *out_top_ml2p, void *workspace,
+                               size_t workspace_bytes, void *stream) {
+    const char *who = "mc_logits_score";
+    Rows a{};
+    if (int rc = tokens_of(who, a, tokens, token_bytes, token_outer_stride, token_inner_stride, outer * inner)) return rc;
+    if (int rc = rows_of(who, a, logits, dtype, outer, inner, vocab, outer_stride, inner_stride, temperature,
+                         one_run(inner, token_outer_stride, token_inner_stride)))
+        return rc;
+    if (top > MC_LOGITS_MAX_TOP || top > vocab) return bad(who, "top: at most 64 alternatives, and no more than tokens");
+    if (a.rows == 0) return MC_OK;
+    if (!out_ml2p || (top && (!out_top || !out_top_ml2p))) return bad(who, "no output");
+    ScoreOut out{out_ml2p, out_entropy, out_top_ml2p, out_top, top};
+    hipStream_t s = (hipStream_t)stream;
+    if (a.nvec <= SUB_VECS) {
+        BY_TYPE(dtype, BY_GROUP(a.nvec, {
+                    if (top) hipLaunchKernelGGL((k_logits_score_sub<DT, G, true, true>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                    else if (out_entropy) hipLaunchKernelGGL((k_logits_score_sub<DT, G, true, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                    else hipLaunchKernelGGL((k_logits_score_sub<DT, G, false, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                }));
+    } else {
+        Split sp{split_shift(a.rows, a.nvec), 0, nullptr, nullptr};
+        if (sp.shift) {
+            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift, top) || (uintptr_t)workspace % 16) {
+                mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift, top), workspace_bytes);
+                return MC_ERR_WORKSPACE;
+            }
+            sp.vecs = split_vecs(a.nvec, sp.shift);
+            sp.stats = (float4 *)workspace;
+            sp.keys = (u64 *)(sp.stats + ((size_t)a.rows << sp.shift));
+        }
+        BY_TYPE(dtype, {
+            if (top) launch<DT, true, true>(a, out, sp, s);
+            else if (out_entropy) launch<DT, true, false>(a, out, sp, s);
+            else launch<DT, false, false>(a, out, sp, s);
+        });
+    }
+    HIP_TRY(hipGetLastError());
+    return MC_OK;
+}

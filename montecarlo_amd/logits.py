@@ -85,6 +85,15 @@ def _call(device: torch.device, fn, *args):
             nv.check(fn(*args, stream))
 
 
+def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
+    """A call's own, held until its launches are queued; then its memory goes back to torch's pool of the current stream."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
 _INTS = (torch.int64, torch.int32)
 
 
@@ -108,9 +117,11 @@ def logits_score(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: flo
     ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
     ids = torch.empty((*rows, top), dtype=torch.int32, device=dev) if top else None
     vals = torch.empty((*rows, top), dtype=torch.float32, device=dev) if top else None
+    need = nv.lib.mc_logits_score_workspace_bytes(code, outer * inner, vocab, top)
+    ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_score, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
-          tokens.element_size(), tos, tis, temperature, ml2p.data_ptr(), ent.data_ptr() if entropy else None, top,
-          ids.data_ptr() if top else None, vals.data_ptr() if top else None)
+          tokens.element_size(), tos, tis, temperature, ml2p.data_ptr(), _ptr(ent), top, _ptr(ids), _ptr(vals),
+          _ptr(ws), need)
     return LogitScores(ml2p, ent, ids, vals)
 
 
@@ -144,10 +155,11 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
                 raise ValueError(f"out overlaps {name}")
     ml2p = torch.empty(rows, dtype=torch.float32, device=dev)
     ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy_weights is not None else None
+    need = nv.lib.mc_logits_gradient_workspace_bytes(code, outer * inner, vocab)
+    ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_gradient, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
-          tokens.element_size(), tos, tis, temperature, weights.data_ptr(), wos, wis,
-          entropy_weights.data_ptr() if entropy_weights is not None else None, eos, eis, ml2p.data_ptr(),
-          ent.data_ptr() if ent is not None else None, out.data_ptr())
+          tokens.element_size(), tos, tis, temperature, weights.data_ptr(), wos, wis, _ptr(entropy_weights), eos, eis,
+          ml2p.data_ptr(), _ptr(ent), out.data_ptr(), _ptr(ws), need)
     return LogitGradient(ml2p, ent, out)
 
 
@@ -174,10 +186,11 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
         live = live.contiguous()
     tokens = torch.empty(shape, dtype=torch.int32, device=dev)
     ml2p = torch.empty(shape, dtype=torch.float32, device=dev)
-    _call(dev, nv.lib.mc_logits_draw, logits.data_ptr(), code, rows, vocab, stride, temperature,
-          uniforms.data_ptr() if uniforms is not None else None, (seed or 0) & 0xFFFFFFFFFFFFFFFF,
-          first_id & 0xFFFFFFFFFFFFFFFF, draw & 0xFFFFFFFF, live.data_ptr() if live is not None else None,
-          tokens.data_ptr(), ml2p.data_ptr())
+    need = nv.lib.mc_logits_draw_workspace_bytes(code, rows, vocab)
+    ws = _workspace(need, dev)
+    _call(dev, nv.lib.mc_logits_draw, logits.data_ptr(), code, rows, vocab, stride, temperature, _ptr(uniforms),
+          (seed or 0) & 0xFFFFFFFFFFFFFFFF, first_id & 0xFFFFFFFFFFFFFFFF, draw & 0xFFFFFFFF, _ptr(live), tokens.data_ptr(),
+          ml2p.data_ptr(), _ptr(ws), need)
     return LogitDraws(tokens, ml2p)
 
 
@@ -212,7 +225,6 @@ def logits_keys(ml2p: torch.Tensor, lengths: Optional[torch.Tensor] = None, *,
         lengths = lengths.contiguous() if lengths is not None else None
         count, stride, longest = ml2p.shape[0], ml2p.stride(0), ml2p.shape[1]
     keys = torch.empty(count, dtype=torch.float64, device=dev)
-    _call(dev, nv.lib.mc_logits_keys, ml2p.data_ptr(), offsets.data_ptr() if offsets is not None else None,
-          lengths.data_ptr() if lengths is not None else None, lengths.element_size() if lengths is not None else 0, count,
-          stride, longest, keys.data_ptr())
+    _call(dev, nv.lib.mc_logits_keys, ml2p.data_ptr(), _ptr(offsets), _ptr(lengths),
+          lengths.element_size() if lengths is not None else 0, count, stride, longest, keys.data_ptr())
     return keys

@@ -32,7 +32,7 @@ def test_gradient_formula_is_the_differences(vocab, temperature, tok):
 
 def _score(**over):
     a = dict(logits=None, dtype=0, outer=1, inner=1, vocab=8, os=0, is_=8, tokens=None, tb=8, tos=0, tis=1, t=1.0, ml2p=None,
-             ent=None, top=0, ids=None, vals=None, stream=None)
+             ent=None, top=0, ids=None, vals=None, ws=None, wsb=0, stream=None)
     a.update(over)
     return nv.lib.mc_logits_score(*a.values())
 
@@ -68,14 +68,14 @@ def test_score_refuses(over):
 
 
 @pytest.mark.parametrize("name,args", [
-    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, None, 0, 1, None, 0, 0, ADDR, None, ADDR, None]),
-    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, None, None]),
-    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR + 2, None]),
-    ("mc_logits_gradient", [ADDR, 7, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, None]),
-    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, None, ADDR, None]),
-    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 0.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
-    ("mc_logits_draw", [ADDR, 0, 1 << 31, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
-    ("mc_logits_draw", [None, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None]),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, None, 0, 1, None, 0, 0, ADDR, None, ADDR, None, 0, None]),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, None, None, 0, None]),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR + 2, None, 0, None]),
+    ("mc_logits_gradient", [ADDR, 7, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, None, 0, None]),
+    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, None, ADDR, None, 0, None]),
+    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 0.0, None, 0, 0, 0, None, ADDR, ADDR, None, 0, None]),
+    ("mc_logits_draw", [ADDR, 0, 1 << 31, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None, 0, None]),
+    ("mc_logits_draw", [None, 0, 1, 8, 8, 1.0, None, 0, 0, 0, None, ADDR, ADDR, None, 0, None]),
     ("mc_logits_keys", [ADDR, ADDR, ADDR, 8, 1, 0, 1, ADDR, None]),
     ("mc_logits_keys", [ADDR, None, ADDR, 2, 1, 0, 1, ADDR, None]),
     ("mc_logits_keys", [None, None, None, 0, 1, 4, 4, ADDR, None]),
@@ -87,10 +87,25 @@ def test_the_others_refuse(name, args):
     assert nv.lib.mc_last_error().startswith(name.encode() + b": ")
 
 
+def test_a_workspace_that_is_too_small_is_refused():
+    need = nv.lib.mc_logits_score_workspace_bytes(0, 2, 100000, 5)
+    assert need > 0 and nv.lib.mc_logits_score_workspace_bytes(0, 2, 100, 5) == 0
+    big = dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, inner=2, vocab=100000, top=5, ids=ADDR, vals=ADDR)
+    for ws, size in ((None, need), (ADDR, need - 1), (ADDR + 8, need)):
+        assert _score(**big, ws=ws, wsb=size) == -6
+    need = nv.lib.mc_logits_gradient_workspace_bytes(2, 2, 100000)
+    assert need > 0
+    assert nv.lib.mc_logits_gradient(ADDR, 2, 1, 2, 100000, 0, 100000, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, ADDR,
+                                     need - 1, None) == -6
+    need = nv.lib.mc_logits_draw_workspace_bytes(1, 2, 100000)
+    assert need > 0
+    assert nv.lib.mc_logits_draw(ADDR, 1, 2, 100000, 100000, 1.0, None, 0, 0, 0, None, ADDR, ADDR, ADDR, need - 1, None) == -6
+
+
 def test_nothing_to_do_is_fine_without_a_gpu():
     assert _score(inner=0) == 0
     assert _score(outer=0, inner=5) == 0
-    assert nv.lib.mc_logits_draw(None, 0, 0, 8, 8, 1.0, None, 0, 0, 0, None, None, None, None) == 0
+    assert nv.lib.mc_logits_draw(None, 0, 0, 8, 8, 1.0, None, 0, 0, 0, None, None, None, None, 0, None) == 0
     assert nv.lib.mc_logits_keys(None, None, None, 0, 0, 0, 0, None, None) == 0
 
 
