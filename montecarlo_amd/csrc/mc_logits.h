@@ -154,10 +154,10 @@ __device__ __forceinline__ u32 pack2(float lo, float hi) {
 }
 
 // the elements from `from` on that the row has room for
-template <int DT>
+template <int DT, bool MAY_END = true>
 __device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const float *g) {
     constexpr u32 N = VEC<DT>;
-    if ((u64)from + N <= vocab) {
+    if (!MAY_END || (u64)from + N <= vocab) {
         raw4 q;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -221,6 +221,9 @@ __device__ __forceinline__ float dpp(float x) {
 struct Max {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
+struct Min {
+    __device__ __forceinline__ float operator()(float a, float b) const { return __uint_as_float(min(__float_as_uint(a), __float_as_uint(b))); }  // (of words)
+};
 struct Add {
     template <typename A>
     __device__ __forceinline__ A operator()(A a, A b) const {
@@ -261,6 +264,11 @@ __device__ __forceinline__ double group_all(double x, Op op) {
     if constexpr (G >= 32) x = op(x, __shfl_xor(x, 16));
     if constexpr (G >= 64) x = op(x, __shfl_xor(x, 32));
     return x;
+}
+
+template <int G>
+__device__ __forceinline__ u32 group_min(u32 x) {
+    return __float_as_uint(group_all<G>(__uint_as_float(x), Min()));
 }
 
 // inclusive prefix sum over the lanes of a group
@@ -359,79 +367,90 @@ __device__ __forceinline__ u32 block_min(u32 v) {
 }
 
 // ---- rows of few tokens: a group of G lanes a row, several rows a wave, the row in registers ---------------------------------
-constexpr int SUB_NV = 8;                    // vectors a lane holds at most
-constexpr u32 SUB_VECS = 64 * SUB_NV;        // vectors a group of 64 lanes holds: 4096 tokens of two bytes
+constexpr u32 SUB_VECS = 64 * 8;  // vectors that 64 lanes hold at most: 4096 tokens of two bytes
 
-template <int DT>
+// A row in the registers of G lanes, NV vectors each: vector i * G + lane; only a lane's last one may lie behind the row's
+// end.  NV = 0: a row shorter than a vector, in one lane's only vector.
+template <int DT, int NV>
 struct SubRow {
-    raw4 q[SUB_NV];      // as loaded
-    u32 from, own;       // of the lane's last vector (the others' are whole)
-    u32 nv;              // vectors a lane holds, the same in the whole grid
+    static constexpr int N = NV ? NV : 1;
+    raw4 q[N];           // as loaded
+    raw4 last;           // the lane's last vector with -inf in the places that are another vector's
+    u32 from;            // its first element's number
 };
 
-// Vector v of a row, 16 bytes whole: the last one of a row that is no multiple of it reaches back into the one before it.
-// `from`: its first element's number; `own`: the first that is not the vector's before it.
-template <int DT>
-__device__ __forceinline__ raw4 load_sub(const char *row, const Rows &a, u32 v, bool read, u32 &from, u32 &own) {
-    constexpr u32 N = VEC<DT>;
-    raw4 q = nothing<DT>();
-    from = own = v * N;
-    if (read && v < a.nvec) {
-        if (a.vocab < N) {
-            q = load_vec<DT>(row, a, v, a.nvec);
-        } else {
-            from = min(own, a.vocab - N);
-            q = *(const raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES);
+// The row's last vector is loaded whole, 16 bytes that end where the row does: when the row is no multiple of a vector it
+// reaches back into the one before it.
+template <int DT, int G, int NV>
+__device__ __forceinline__ void load_row(SubRow<DT, NV> &r, const char *p, const Rows &a, bool read) {
+    constexpr u32 E = VEC<DT>;
+    constexpr int N = SubRow<DT, NV>::N;
+    const u32 lane = threadIdx.x & (G - 1), v = (N - 1) * G + lane;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.q[i] = nothing<DT>();
+    r.from = v * E;
+    if (read) {
+#pragma unroll
+        for (int i = 0; i + 1 < N; ++i) r.q[i] = *(const raw4_at2 *)(p + (u64)(i * G + lane) * 16);
+        if (NV == 0) {
+            r.q[0] = load_vec<DT>(p, a, lane, a.nvec);
+        } else if (v < a.nvec) {
+            r.from = min(v * E, a.vocab - E);
+            r.q[N - 1] = *(const raw4_at2 *)(p + (u64)r.from * Elt<DT>::BYTES);
         }
     }
-    return q;
-}
-
-// the vector with -inf in the places that are another one's
-template <int DT>
-__device__ __forceinline__ raw4 masked(raw4 q, u32 from, u32 own) {
-    if (from == own) return q;
-    const u32 n = own - from;
+    r.last = r.q[N - 1];
+    const u32 n = v * E - r.from;  // places of the vector before it
+    if (n) {
 #pragma unroll
-    for (u32 w = 0; w < 4; ++w) {
-        u32 m;
-        if constexpr (Elt<DT>::BYTES == 4) m = w < n ? 0xFFFFFFFFu : 0u;
-        else m = (2 * w < n ? 0xFFFFu : 0u) | (2 * w + 1 < n ? 0xFFFF0000u : 0u);
-        q[w] = (q[w] & ~m) | (Elt<DT>::NEG_INF & m);
-    }
-    return q;
-}
-
-template <int DT, int G>
-__device__ __forceinline__ void load_row(SubRow<DT> &r, const char *p, const Rows &a, bool read) {
-    const u32 lane = threadIdx.x & (G - 1);
-    r.nv = (a.nvec + G - 1) / G;
-    r.from = r.own = 0;
-#pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
-        if (i < (int)r.nv) r.q[i] = load_sub<DT>(p, a, i * G + lane, read, r.from, r.own);
+        for (u32 w = 0; w < 4; ++w) {
+            u32 m;
+            if constexpr (Elt<DT>::BYTES == 4) m = w < n ? 0xFFFFFFFFu : 0u;
+            else m = (2 * w < n ? 0xFFFFu : 0u) | (2 * w + 1 < n ? 0xFFFF0000u : 0u);
+            r.last[w] = (r.last[w] & ~m) | (Elt<DT>::NEG_INF & m);
+        }
     }
 }
 
-template <int DT>
-__device__ __forceinline__ raw4 vec_of(const SubRow<DT> &r, int i) {
-    return i + 1 == (int)r.nv ? masked<DT>(r.q[i], r.from, r.own) : r.q[i];
+template <int DT, int NV>
+__device__ __forceinline__ raw4 vec_of(const SubRow<DT, NV> &r, int i) {
+    return i + 1 == SubRow<DT, NV>::N ? r.last : r.q[i];
 }
 
-template <int DT, int G, bool ENT, bool EXACT>
-__device__ __forceinline__ Stat sub_sums(const SubRow<DT> &r, float m, float c) {
+// `a` takes the value of b where `yes` (by words: a choice between vectors becomes one between their addresses, and the row
+// goes to memory for it)
+__device__ __forceinline__ void choose(raw4 &a, const raw4 &b, bool yes) {
+    const u32 m = yes ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) a[w] = (a[w] & ~m) | (b[w] & m);
+}
+
+// the number of vector i's first element
+template <int DT, int G, int NV>
+__device__ __forceinline__ u32 from_of(const SubRow<DT, NV> &r, int i) {
+    return i + 1 == SubRow<DT, NV>::N ? r.from : (i * G + (threadIdx.x & (G - 1))) * VEC<DT>;
+}
+
+// The words of a row as if just loaded: what comes next unpacks them again, where the compiler would keep the numbers of
+// all vectors in registers.  For code that seldom runs, and for rows of more than four vectors a lane.
+template <int DT, int NV>
+__device__ __forceinline__ void forget(SubRow<DT, NV> &r) {
+#pragma unroll
+    for (int i = 0; i + 1 < SubRow<DT, NV>::N; ++i) asm("" : "+v"(r.q[i]));
+    asm("" : "+v"(r.last));
+}
+
+template <int DT, int G, bool ENT, bool EXACT, int NV>
+__device__ __forceinline__ Stat sub_sums(const SubRow<DT, NV> &r, float m, float c) {
     Stat st{m, 0.f, 0.f, EXACT};
     const Expo y_of(st, c);
 #pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
-        if (i < (int)r.nv) {
-            const raw4 q = vec_of<DT>(r, i);
+    for (int i = 0; i < SubRow<DT, NV>::N; ++i) {
 #pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) {
-                const float x = unpack<DT>(q, j), y = EXACT ? (x - y_of.m) * c : y_of.fast(x), w = exp2_(y);
-                st.s += w;
-                if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
-            }
+        for (int j = 0; j < VEC<DT>; ++j) {
+            const float x = unpack<DT>(vec_of(r, i), j), y = EXACT ? (x - y_of.m) * c : y_of.fast(x), w = exp2_(y);
+            st.s += w;
+            if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
         }
     }
     st.s = group_all<G>(st.s, Add());
@@ -439,31 +458,25 @@ __device__ __forceinline__ Stat sub_sums(const SubRow<DT> &r, float m, float c) 
     return st;
 }
 
-// The words of a row as if just loaded: what the next pass makes of them is made again from the packed words, where the
-// compiler would keep the unpacked numbers of all vectors in registers (145 instead of 64-80: three waves instead of six).
-template <int DT>
-__device__ __forceinline__ void forget(SubRow<DT> &r) {
-#pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) asm("" : "+v"(r.q[i]));
-}
-
-template <int DT, int G, bool ENT>
-__device__ __forceinline__ Stat sub_stat(SubRow<DT> &r, float c) {
+template <int DT, int G, int NV>
+__device__ __forceinline__ float sub_max(const SubRow<DT, NV> &r) {
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
-        if (i < (int)r.nv) {
-            const raw4 q = vec_of<DT>(r, i);
+    for (int i = 0; i < SubRow<DT, NV>::N; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) m = maximum(m, unpack<DT>(q, j));
-        }
-    }
-    m = group_all<G>(m, Max());
-    forget(r);
+        for (int j = 0; j < VEC<DT>; ++j) m = maximum(m, unpack<DT>(vec_of(r, i), j));
+    return group_all<G>(m, Max());
+}
+
+// (a row that is not read has no doubts)
+template <int DT, int G, bool ENT, int NV>
+__device__ __forceinline__ Stat sub_stat(SubRow<DT, NV> &r, float c, bool read) {
+    const float m = sub_max<DT, G>(r);
+    if (NV > 4) forget(r);
     Stat st = sub_sums<DT, G, ENT, false>(r, m, c);
-    const bool again = doubtful(st, c);
-    forget(r);
+    const bool again = read && doubtful(st, c);
     if (__ballot(again)) {
+        forget(r);
         const Stat ex = sub_sums<DT, G, ENT, true>(r, m, c);
         if (again) st = ex;
     }
@@ -599,10 +612,44 @@ inline u32 rows_to_blocks(u32 rows, u32 group) { return (u32)(((u64)rows * group
         default: { constexpr int DT = MC_LOGITS_BF16; __VA_ARGS__; break; }            \
     }
 
-// a group of as few lanes as hold a row
-#define BY_GROUP(nvec, ...)                                                 \
-    if ((nvec) <= 4 * SUB_NV) { constexpr int G = 4; __VA_ARGS__; }         \
-    else if ((nvec) <= 8 * SUB_NV) { constexpr int G = 8; __VA_ARGS__; }    \
-    else if ((nvec) <= 16 * SUB_NV) { constexpr int G = 16; __VA_ARGS__; }  \
-    else if ((nvec) <= 32 * SUB_NV) { constexpr int G = 32; __VA_ARGS__; }  \
-    else { constexpr int G = 64; __VA_ARGS__; }
+// How many lanes share a row (G) and how many vectors each of them holds (NV).  Many rows: the fewest places for vectors, G
+// * NV, and the fewest lanes, since what is done once a row and lane costs as much as eight elements.  Few rows (less than
+// a wave for each of the 1024 SIMDs): the most lanes, since such a launch waits for its loads and its instructions (12 rows of
+// 97 tokens took 15.7 us with 4 lanes, 4.4 with 32).
+inline void group_of(u32 rows, u32 vocab, u32 nvec, u32 vec, int &g, int &nv) {
+    g = 4, nv = 0;
+    if (vocab < vec) return;
+    u32 best = 0xFFFFFFFFu;
+    for (int G = 4; G <= 64; G *= 2) {
+        const u32 n = (nvec + G - 1) / G;
+        if (n > (G == 64 ? 8u : 4u)) continue;
+        const bool few = (u64)rows * G <= 65536;
+        if (best == 0xFFFFFFFFu || n * G < best || (few && nv > 1)) best = n * G, g = G, nv = (int)n;
+    }
+}
+
+#define BY_LANES(...)                                              \
+    switch (g_) {                                                  \
+        case 4: { constexpr int G = 4; __VA_ARGS__; break; }       \
+        case 8: { constexpr int G = 8; __VA_ARGS__; break; }       \
+        case 16: { constexpr int G = 16; __VA_ARGS__; break; }     \
+        case 32: { constexpr int G = 32; __VA_ARGS__; break; }     \
+        default: { constexpr int G = 64; __VA_ARGS__; break; }     \
+    }
+
+#define BY_GROUP(a, ...)                                                            \
+    {                                                                               \
+        int g_, nv_;                                                                \
+        group_of((a).rows, (a).vocab, (a).nvec, VEC<DT>, g_, nv_);                  \
+        switch (nv_) {                                                              \
+            case 0: { constexpr int NV = 0, G = 4; __VA_ARGS__; break; }            \
+            case 1: { constexpr int NV = 1; BY_LANES(__VA_ARGS__) break; }          \
+            case 2: { constexpr int NV = 2; BY_LANES(__VA_ARGS__) break; }          \
+            case 3: { constexpr int NV = 3; BY_LANES(__VA_ARGS__) break; }          \
+            case 4: { constexpr int NV = 4; BY_LANES(__VA_ARGS__) break; }          \
+            case 5: { constexpr int NV = 5, G = 64; __VA_ARGS__; break; }           \
+            case 6: { constexpr int NV = 6, G = 64; __VA_ARGS__; break; }           \
+            case 7: { constexpr int NV = 7, G = 64; __VA_ARGS__; break; }           \
+            default: { constexpr int NV = 8, G = 64; __VA_ARGS__; break; }          \
+        }                                                                           \
+    }

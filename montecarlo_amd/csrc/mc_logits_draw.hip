@@ -1,10 +1,12 @@
 // Draws from rows of logits by inversion, and the keys of whole passwords (formulas: mc_logits_score.hip).
 //
-// The draw is defined by running sums in 64 bits, and these are what has to be computed: a vocabulary of 10^5 tokens puts
-// 10^5 ends of intervals into [0, Z), so that sums known to 10^-7 would leave the token open in every other row.  Weights
-// come from a polynomial that is right to 4e-11 (sixteen operations an element, which this GPU does at the rate of 32
-// bits); where u Z lies within 1e-10 Z of an end (a row in 10^5) the row is summed again with the library's exponential.
-// Exponents of 64 bits reach far enough that no maximum has to be known first: one pass.
+// The draw is defined by running sums in 64 bits.  Sums in 32 bits are known to e = a few parts in 10^6 and leave the token
+// open where u Z lies nearer than that to an end of its interval: at most a share 2 e V of the draws.  Rows of
+// up to 4096 tokens begin with them (a row in a thousand is open at V = 97) and take what is open again in 64 bits; a
+// vocabulary of 10^5 tokens has intervals as narrow as e, every other draw would be open, and wider rows begin with 64 bits.
+// Weights then come from a polynomial that is right to 4e-11 (sixteen operations an element, which this GPU does at the
+// rate of 32 bits), and where u Z lies within 1e-10 Z of an end (a row in 10^5) the row is summed once more with the library's
+// exponential.  Exponents of 64 bits reach far enough that no maximum has to be known first.
 #include "mc_logits.h"
 #include "mc_philox.h"
 
@@ -14,6 +16,7 @@ namespace {
 // nothing), NaN for NaN.  The whole part n goes to the exponent; on [-1/2, 1/2] the polynomial of degree 7 that
 // approximates 2^f best relative to its value (found by exchange of the extremal points; largest error 4.03e-11).
 struct Power {
+    typedef double Sum;
     double c;
     float lo;
     __device__ __forceinline__ double operator()(float x) const {
@@ -31,8 +34,16 @@ struct Power {
 };
 constexpr double MARGIN = 1e-10;
 
+// weights in 32 bits under the row's largest logit
+struct Fast {
+    typedef float Sum;
+    Expo y_of;
+    __device__ __forceinline__ float operator()(float x) const { return exp2_(y_of.fast(x)); }
+};
+
 // The draw's own weights: exp((x - m) / T) in 64 bits, m the row's largest logit.
 struct Definition {
+    typedef double Sum;
     double t, m;
     __device__ __forceinline__ double operator()(float x) const { return exp(((double)x - m) / t); }
 };
@@ -51,7 +62,7 @@ struct DrawArgs {
     const double *uniforms;  // or null: Philox
     u64 seed, first_id;
     u32 draw;
-    double t;
+    double t, margin;        // margin: how far off the running sums of Fast may be, as a share of Z
     Power power;
     const unsigned char *live;
     int *token;
@@ -73,70 +84,61 @@ __device__ __forceinline__ double uniform_of(const DrawArgs &d, u32 row) {
 // ---- rows of few tokens --------------------------------------------------------------------------------------------------
 // The token of a group's row in registers: running sums in the order of the index, vector step by vector step.  False when
 // u Z lies within `margin` Z of an end of the token's interval (0 takes any answer).
-template <int DT, int G, typename W>
-__device__ __forceinline__ bool draw_sub(SubRow<DT> &r, const W &weight, double u, double margin, u32 &token, float &x, double &z, float &m) {
-    const u32 lane = threadIdx.x & (G - 1);
-    double s[SUB_NV];
-    z = 0.;
-    m = -INFINITY;
+template <int DT, int G, typename W, int NV>
+__device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weight, double u, double margin, u32 &token, float &x, typename W::Sum &z) {
+    typedef typename W::Sum Sum;
+    constexpr int N = SubRow<DT, NV>::N;
+    Sum s[N];
+    z = 0;
 #pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
-        s[i] = 0.;
-        if (i < (int)r.nv) {
-            const raw4 q = vec_of<DT>(r, i);
+    for (int i = 0; i < N; ++i) {
+        s[i] = 0;
 #pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) {
-                const float e = unpack<DT>(q, j);
-                m = maximum(m, e);
-                s[i] += weight(e);
-            }
-            z += s[i];
-        }
+        for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(vec_of(r, i), j));
+        z += s[i];
     }
-    m = group_all<G>(m, Max());
     z = group_all<G>(z, Add());
-    const double target = u * z;
+    const double target = u * (double)z, near = margin * (double)z;
     // the vector step whose running sum passes the target, or the last one with any weight
-    double before = 0., run = 0., mine = 0.;
-    raw4 q = r.q[0];
-    u32 from = lane * VEC<DT>;
+    double before = 0., run = 0.;
+    Sum mine = 0;
+    raw4 q = vec_of(r, 0);
+    u32 from = from_of<DT, G>(r, 0);
     bool found = false;
 #pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
-        if (i < (int)r.nv) {
-            const double step = group_all<G>(s[i], Add());
-            if (!found && step > 0.) {
-                before = run;
-                mine = s[i];
-                q = vec_of<DT>(r, i);
-                from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
-                found = run + step > target;
-            }
-            run += step;
-        }
+    for (int i = 0; i < N; ++i) {
+        const double step = (double)group_all<G>(s[i], Add());
+        const bool here = !found && step > 0.;
+        before = here ? run : before;
+        mine = here ? s[i] : mine;
+        choose(q, vec_of(r, i), here);
+        from = here ? from_of<DT, G>(r, i) : from;
+        found = found || (here && run + step > target);
+        run += step;
     }
-    const double inc = group_scan<G>(mine), lo = before + (inc - mine);
+    const Sum inc = group_scan<G>(mine);
     const u32 shift = threadIdx.x & 63 & ~(G - 1);
     const u64 all = G == 64 ? ~0ull : (1ull << (G & 63)) - 1;
-    const u64 passes = (__ballot(before + inc > target) >> shift) & all, some = (__ballot(mine > 0.) >> shift) & all;
+    const u64 passes = (__ballot(before + (double)inc > target) >> shift) & all, some = (__ballot(mine > 0) >> shift) & all;
     // (a sum that passes by a rounding only, or none: the last lane with any weight)
     const bool hit = found && passes;
     const u32 who = hit ? (u32)__ffsll((unsigned long long)passes) - 1 : some ? 63u - (u32)__clzll((long long)some) : 0u;
-    double at_lo = lo;
+    double at_lo = before + (double)(inc - mine);
     u32 got = 0xFFFFFFFFu, last = 0;
     float got_x = 0.f, last_x = 0.f;
     bool ok = false;
 #pragma unroll
     for (int j = 0; j < VEC<DT>; ++j) {
         const float e = unpack<DT>(q, j);
-        const double w = weight(e), next = at_lo + w;
-        if (w > 0.) {
+        const Sum w = weight(e);
+        const double next = at_lo + (double)w;
+        if (w > 0) {
             last = from + j;
             last_x = e;
             if (got == 0xFFFFFFFFu && next > target) {
                 got = from + j;
                 got_x = e;
-                ok = hit && target - at_lo >= margin * z && next - target >= margin * z;
+                ok = hit && target - at_lo >= near && next - target >= near;
             }
         }
         at_lo = next;
@@ -147,30 +149,40 @@ __device__ __forceinline__ bool draw_sub(SubRow<DT> &r, const W &weight, double 
     return __shfl((int)ok, who, G) || margin == 0.;
 }
 
-template <int DT, int G>
-__global__ __launch_bounds__(BLOCK) void k_logits_draw_sub(Rows a, DrawArgs d) {
+template <int DT, int G, int NV>
+__global__ __launch_bounds__(BLOCK, 6) void k_logits_draw_sub(Rows a, DrawArgs d) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows, live = there && (!d.live || d.live[row]);
     const char *p = there ? at(a.logits, a.inner, row) : nullptr;
-    SubRow<DT> r;
+    SubRow<DT, NV> r;
     load_row<DT, G>(r, p, a, live);
     const double u = there ? uniform_of(d, row) : 0.;
+    Stat st{sub_max<DT, G>(r), 0.f, 0.f, false};
+    if (NV > 4) forget(r);
     u32 token;
-    float x, m;
-    double z;
-    bool sure = draw_sub<DT, G>(r, d.power, u, MARGIN, token, x, z, m) && good(z, m, d.power.c);
-    float ml2p = ml2p_under(z, d.power.c, x);
+    float x;
+    bool sure = draw_sub<DT, G>(r, Fast{Expo(st, a.c)}, u, d.margin, token, x, st.s) && !doubtful(st, a.c);
+    float ml2p = ml2p_of(0, st, x, a.c);
     if (!live) sure = true, token = (u32)MC_TOKEN_SKIP, ml2p = 0.f;
-    if (__ballot(!sure)) {  // the whole wave decides again, from the definition
+    if (__ballot(!sure)) {  // the whole wave decides again, in 64 bits
         forget(r);
-        const Stat st = sub_stat<DT, G, false>(r, a.c);
         u32 again;
-        float x_again, m_again;
-        double z_again;
-        draw_sub<DT, G>(r, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u, 0., again, x_again, z_again, m_again);
-        if (!sure) {
-            token = st.s > 0.f ? again : (u32)MC_TOKEN_OUTSIDE;
-            ml2p = ml2p_of(0, st, x_again, a.c);
+        float x_again;
+        double z;
+        bool now = draw_sub<DT, G>(r, d.power, u, MARGIN, again, x_again, z) && good(z, st.m, d.power.c);
+        if (!sure && now) {
+            token = again;
+            ml2p = ml2p_under(z, d.power.c, x_again);
+        }
+        now = now || sure;
+        if (__ballot(!now)) {  // and again, from the definition
+            forget(r);
+            st = sub_sums<DT, G, false, true>(r, st.m, a.c);
+            draw_sub<DT, G>(r, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u, 0., again, x_again, z);
+            if (!now) {
+                token = st.s > 0.f ? again : (u32)MC_TOKEN_OUTSIDE;
+                ml2p = ml2p_of(0, st, x_again, a.c);
+            }
         }
     }
     if (there && lane == 0) {
@@ -180,7 +192,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sub(Rows a, DrawArgs d) {
 }
 
 // ---- rows of many tokens ---------------------------------------------------------------------------------------------------
-constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 8;
+constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 4;
 
 // The token by the definition's weights (every thread of the workgroup calls).
 template <int DT>
@@ -257,8 +269,8 @@ __device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Ro
             if (lane == 0) sh.sums[i * WIDE_WAVES + wave] = all;
         }
         __syncthreads();
-        static_assert(STEPS * WIDE_WAVES == 64, "one lane for each sum");
-        const double mine = sh.sums[lane], inc = group_scan<64>(mine);
+        static_assert(STEPS * WIDE_WAVES <= 64, "one lane for each sum");
+        const double mine = lane < STEPS * WIDE_WAVES ? sh.sums[lane] : 0., inc = group_scan<64>(mine);
         const u64 passes = __ballot(before + inc > target);
         if (passes) {
             const u32 which = (u32)__ffsll((unsigned long long)passes) - 1;
@@ -269,7 +281,8 @@ __device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Ro
                 double ms = s[0];
 #pragma unroll
                 for (int i = 1; i < STEPS; ++i) {
-                    if (i == (int)step) mq = q[i], ms = s[i];
+                    choose(mq, q[i], i == (int)step);
+                    ms = i == (int)step ? s[i] : ms;
                 }
                 const double minc = group_scan<64>(ms);
                 const u64 over = __ballot(start + minc > target);
@@ -362,7 +375,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
 
 // One workgroup a row: its waves' (or the parts') sums say in which of them the token lies; that part is looked at again.
 template <int DT, bool PART>
-__global__ __launch_bounds__(WIDE) void k_logits_draw(Rows a, DrawArgs d, Split sp) {
+__global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d, Split sp) {
     __shared__ LocateShared sh;
     __shared__ double ps[WIDE_WAVES];
     __shared__ float pm[WIDE_WAVES];
@@ -442,6 +455,11 @@ u32 split_shift(u32 rows, u32 nvec) {
 
 size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * 16 : 0; }
 
+// How far off running sums of Fast over a row of few tokens may be, as a share of Z, in half steps of 32 bits: the weights (2
+// for the power; the exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions
+// in a vector, 8 over vectors, 6 over lanes, 2 where parts are joined; twice, since u Z is such a sum too.
+double margin_of(uint64_t vocab) { return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)vocab) + 24); }
+
 // ---- keys ----------------------------------------------------------------------------------------------------------
 // one lane a password
 __global__ __launch_bounds__(BLOCK) void k_logits_keys(const float *ml2p, const i64 *offsets, const void *lengths, u32 length_bytes,
@@ -483,9 +501,9 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (!out_token || !out_ml2p) return bad(who, "no output");
     hipStream_t s = (hipStream_t)stream;
     const double c = LOG2E / temperature;
-    DrawArgs d{uniforms, seed, first_id, draw, temperature, Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(vocab), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
     if (a.nvec <= SUB_VECS) {
-        BY_TYPE(dtype, BY_GROUP(a.nvec, hipLaunchKernelGGL((k_logits_draw_sub<DT, G>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
+        BY_TYPE(dtype, BY_GROUP(a, hipLaunchKernelGGL((k_logits_draw_sub<DT, G, NV>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
     } else {
         Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
         if (sp.shift) {

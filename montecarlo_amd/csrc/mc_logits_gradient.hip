@@ -54,16 +54,16 @@ __device__ __forceinline__ void put_zeros(char *gp, u32 from, u32 vocab) {
     store_at<DT>(gp, from, vocab, g);
 }
 
-template <int DT, int G, bool ENT>
+template <int DT, int G, int NV, bool ENT>
 __global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOut out) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows;
     const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
     const char *p = there ? at(a.logits, a.inner, row) : nullptr;
-    SubRow<DT> r;
+    SubRow<DT, NV> r;
     load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
-    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c, tok != MC_TOKEN_SKIP);
     if (!there) return;
     if (lane == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, a.c);
@@ -73,18 +73,19 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOu
     const Expo y_of(st, a.c);
     char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
 #pragma unroll
-    for (int i = 0; i < SUB_NV; ++i) {
+    for (int i = 0; i < SubRow<DT, NV>::N; ++i) {
         const u32 v = i * G + lane;
-        if (i < (int)r.nv && v < a.nvec) {
+        if (i + 1 < SubRow<DT, NV>::N || v < a.nvec) {
             // (a last vector that reaches back computes and stores there what the one before it does)
-            const u32 from = a.vocab < VEC<DT> ? 0u : min(v * VEC<DT>, a.vocab - VEC<DT>);
+            const u32 from = NV == 0 ? 0u : i + 1 < NV ? v * VEC<DT> : min(v * VEC<DT>, a.vocab - VEC<DT>);
+            float g[VEC<DT>];
+            if (st.exact) slope_vec<DT, ENT, true>(r.q[i], from, s, y_of, g);
+            else slope_vec<DT, ENT, false>(r.q[i], from, s, y_of, g);
             if (s.none) {
-                put_zeros<DT>(gp, from, a.vocab);
-            } else {
-                float g[VEC<DT>];
-                slope_vec<DT, ENT, true>(r.q[i], from, s, y_of, g);
-                store_at<DT>(gp, from, a.vocab, g);
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
             }
+            store_at<DT, NV == 0>(gp, from, a.vocab, g);
         }
     }
 }
@@ -255,7 +256,7 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 template <int DT, bool ENT>
 void launch(const Rows &a, const GradOut &out, const Split &sp, hipStream_t s) {
     if (a.nvec <= SUB_VECS) {
-        BY_GROUP(a.nvec, hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, ENT>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out));
+        BY_GROUP(a, hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, NV, ENT>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out));
     } else if (sp.shift) {
         hipLaunchKernelGGL((k_logits_gradient_sums<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, sp);
         hipLaunchKernelGGL((k_logits_gradient_join<DT, ENT>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);

@@ -36,44 +36,40 @@ __device__ __forceinline__ u64 key_of(u32 order, u32 index) { return (u64)order 
 __device__ __forceinline__ u32 index_of(u64 key) { return 0xFFFFFFFFu - (u32)key; }
 
 // one alternative's outputs
-__device__ __forceinline__ void put_top(const ScoreOut &out, u32 row, u32 rank, u64 key, const Stat &st, float c) {
-    const float v = log2f(st.s) - Expo(st, c)(value_of((u32)(key >> 32)));
+__device__ __forceinline__ void put_top(const ScoreOut &out, u32 row, u32 rank, u64 key, const Stat &st, float lz, float c) {
+    const float v = lz - Expo(st, c)(value_of((u32)(key >> 32)));
     out.top[(u64)row * out.k + rank] = v < INFINITY ? (int)index_of(key) : MC_TOKEN_OUTSIDE;
     out.top_ml2p[(u64)row * out.k + rank] = v < INFINITY ? v : INFINITY;
 }
 
 // ---- rows of few tokens --------------------------------------------------------------------------------------------------
 // The k largest of a row in registers, one after the other: the largest that comes behind the last one in the order.
-template <int DT, int G>
-__device__ __forceinline__ void sub_top(SubRow<DT> &r, const Rows &a, const Stat &st, const ScoreOut &out, u32 row, bool writes, int tok) {
+template <int DT, int G, int NV>
+__device__ __forceinline__ void sub_top(SubRow<DT, NV> &r, const Rows &a, const Stat &st, const ScoreOut &out, u32 row, bool writes, int tok) {
     const u32 lane = threadIdx.x & (G - 1);
     const bool blank = tok == MC_TOKEN_SKIP || !(st.s > 0.f);
+    const float lz = log2f(st.s);
     float last = INFINITY;
     u32 last_i = 0xFFFFFFFFu;
     for (u32 k = 0; k < out.k; ++k) {
-        forget(r);
+        if (NV > 1) forget(r);
         float best = -INFINITY;
         u32 best_i = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < SUB_NV; ++i) {
-            if (i < (int)r.nv) {
-                const raw4 q = vec_of<DT>(r, i);
-                const u32 from = i + 1 == (int)r.nv ? r.from : (i * G + lane) * VEC<DT>;
+        for (int i = 0; i < SubRow<DT, NV>::N; ++i) {
+            const u32 from = from_of<DT, G>(r, i);
 #pragma unroll
-                for (int j = 0; j < VEC<DT>; ++j) {
-                    const float x = unpack<DT>(q, j);
-                    const bool open = x < last || (x == last && from + j > last_i);
-                    if (open && x > best) best = x, best_i = from + j;
-                }
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float x = unpack<DT>(vec_of(r, i), j);
+                const bool open = x < last || (x == last && from + j > last_i);
+                if (open && x > best) best = x, best_i = from + j;
             }
         }
         const float top = group_all<G>(best, Max());
-        u32 at = best == top ? best_i : 0xFFFFFFFFu;
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) at = min(at, (u32)__shfl_xor(at, d));
+        const u32 at = group_min<G>(best == top ? best_i : 0xFFFFFFFFu);
         if (writes && lane == 0) {
             if (!blank && top > -INFINITY) {
-                put_top(out, row, k, key_of(order_of(top), at), st, a.c);
+                put_top(out, row, k, key_of(order_of(top), at), st, lz, a.c);
             } else {
                 out.top[(u64)row * out.k + k] = tok == MC_TOKEN_SKIP ? MC_TOKEN_SKIP : MC_TOKEN_OUTSIDE;
                 out.top_ml2p[(u64)row * out.k + k] = tok == MC_TOKEN_SKIP ? 0.f : st.s == st.s ? INFINITY : st.s;
@@ -84,16 +80,16 @@ __device__ __forceinline__ void sub_top(SubRow<DT> &r, const Rows &a, const Stat
     }
 }
 
-template <int DT, int G, bool ENT, bool TOP>
+template <int DT, int G, int NV, bool ENT, bool TOP>
 __global__ __launch_bounds__(BLOCK, TOP ? 6 : 8) void k_logits_score_sub(Rows a, ScoreOut out) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows;
     const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
     const char *p = there ? at(a.logits, a.inner, row) : nullptr;
-    SubRow<DT> r;
+    SubRow<DT, NV> r;
     load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
-    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c, tok != MC_TOKEN_SKIP);
     if (there && lane == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, a.c);
         if (ENT && out.entropy) out.entropy[row] = entropy_of(tok, st);
@@ -262,11 +258,12 @@ __device__ __forceinline__ void put_row(const ScoreOut &out, u32 row, int tok, f
     }
     if (!out.k) return;
     if (!(st.s > 0.f)) n = 0;
+    const float lz = log2f(st.s);
     for (u32 i = threadIdx.x; i < n; i += BLOCK) {
         const u64 key = cand[i];
         u32 rank = 0;
         for (u32 j = 0; j < n; ++j) rank += cand[j] > key;
-        if (rank < out.k) put_top(out, row, rank, key, st, c);
+        if (rank < out.k) put_top(out, row, rank, key, st, lz, c);
     }
     for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) {
         out.top[(u64)row * out.k + i] = MC_TOKEN_OUTSIDE;
@@ -433,10 +430,10 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
     ScoreOut out{out_ml2p, out_entropy, out_top_ml2p, out_top, top};
     hipStream_t s = (hipStream_t)stream;
     if (a.nvec <= SUB_VECS) {
-        BY_TYPE(dtype, BY_GROUP(a.nvec, {
-                    if (top) hipLaunchKernelGGL((k_logits_score_sub<DT, G, true, true>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
-                    else if (out_entropy) hipLaunchKernelGGL((k_logits_score_sub<DT, G, true, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
-                    else hipLaunchKernelGGL((k_logits_score_sub<DT, G, false, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+        BY_TYPE(dtype, BY_GROUP(a, {
+                    if (top) hipLaunchKernelGGL((k_logits_score_sub<DT, G, NV, true, true>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                    else if (out_entropy) hipLaunchKernelGGL((k_logits_score_sub<DT, G, NV, true, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
+                    else hipLaunchKernelGGL((k_logits_score_sub<DT, G, NV, false, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out);
                 }));
     } else {
         Split sp{split_shift(a.rows, a.nvec), 0, nullptr, nullptr};
