@@ -3,8 +3,9 @@
 // With c = log2(e) / T a token's exponent is y = x c - M, where M = m c is the largest logit's: one multiply-add, one power
 // and the sums an element.  M may be off by a rounding; every use of it subtracts the same number, so that cancels.  That
 // holds while |M| <= 2^15 (the largest weight is then 2^(2^-9) at most).  Parts of a row whose own maximum lies lower take
-// -2^15 for it; a ROW whose M is beyond, whose weights all vanish that way, or that holds a NaN or +inf is summed again
-// with y = (x - m) c (`exact`): a row of the type's lowest value, temperatures near 0, rows with nothing left.
+// -2^15 for it; a ROW whose M is beyond is summed again with y = (x - m) c (`exact`): a row of the type's lowest value,
+// temperatures near 0.  m says the rest: it is -inf where nothing is left (s is 0 then), NaN where the row holds a NaN and
+// +inf where it holds one (s is NaN then).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -198,8 +199,8 @@ struct Expo {
     __device__ __forceinline__ float operator()(float x) const { return exact ? (x - m) * c : fast(x); }
 };
 
-// whether a row's fast sums stand
-__device__ __forceinline__ bool doubtful(const Stat &st, float c) { return !(fabsf(scaled(st.m, c)) <= FAR && st.m * c > -FAR && st.s > 0.f); }
+// whether a row's fast sums do not stand
+__device__ __forceinline__ bool doubtful(float m, float c) { return fabsf(m) < INFINITY && fabsf(m * c) > FAR; }
 
 // what a row's statistics say about its token
 __device__ __forceinline__ float ml2p_of(int tok, const Stat &st, float x, float c) {
@@ -219,7 +220,7 @@ __device__ __forceinline__ float dpp(float x) {
 }
 
 struct Max {
-    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); }
 };
 struct Min {
     __device__ __forceinline__ float operator()(float a, float b) const { return __uint_as_float(min(__float_as_uint(a), __float_as_uint(b))); }  // (of words)
@@ -331,7 +332,7 @@ __device__ __forceinline__ float block_max(float v) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < T / 64; ++w) v = fmaxf(v, part[w]);
+    for (int w = 0; w < T / 64; ++w) v = maximum(v, part[w]);
     return v;
 }
 
@@ -468,13 +469,12 @@ __device__ __forceinline__ float sub_max(const SubRow<DT, NV> &r) {
     return group_all<G>(m, Max());
 }
 
-// (a row that is not read has no doubts)
 template <int DT, int G, bool ENT, int NV>
-__device__ __forceinline__ Stat sub_stat(SubRow<DT, NV> &r, float c, bool read) {
+__device__ __forceinline__ Stat sub_stat(SubRow<DT, NV> &r, float c) {
     const float m = sub_max<DT, G>(r);
     if (NV > 4) forget(r);
     Stat st = sub_sums<DT, G, ENT, false>(r, m, c);
-    const bool again = read && doubtful(st, c);
+    const bool again = doubtful(m, c);
     if (__ballot(again)) {
         forget(r);
         const Stat ex = sub_sums<DT, G, ENT, true>(r, m, c);

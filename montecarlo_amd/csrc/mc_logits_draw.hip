@@ -8,28 +8,46 @@
 // rate of 32 bits), and where u Z lies within 1e-10 Z of an end (a row in 10^5) the row is summed once more with the library's
 // exponential.  Exponents of 64 bits reach far enough that no maximum has to be known first.
 #include "mc_logits.h"
+
+#include <algorithm>
+
 #include "mc_philox.h"
 
 namespace {
 
-// 2^(x c) for x c in [-1000, 900]; lower ones as 2^-1000 (so far below any sum that `good` lets pass that it changes
-// nothing), NaN for NaN.  The whole part n goes to the exponent; on [-1/2, 1/2] the polynomial of degree 7 that
-// approximates 2^f best relative to its value (found by exchange of the extremal points; largest error 4.03e-11).
+// 2^y from y c's whole part n (as the low word of n + 1.5 * 2^52) and the rest f in [-1/2, 1/2]: the polynomial of degree 7
+// that approximates 2^f best relative to its value (found by exchange of the extremal points; largest error 4.03e-11).
+__device__ __forceinline__ double power_of(double n_word, double f) {
+    double p = 0x1.fe1786b50da52p-17;
+    p = __builtin_fma(p, f, 0x1.446a1fdd54f3ap-13);
+    p = __builtin_fma(p, f, 0x1.5d8a7085cddb8p-10);
+    p = __builtin_fma(p, f, 0x1.3b29dc40d2ec5p-7);
+    p = __builtin_fma(p, f, 0x1.c6b08aaf3156ep-5);
+    p = __builtin_fma(p, f, 0x1.ebfbe0a4be886p-3);
+    p = __builtin_fma(p, f, 0x1.62e42ff11627ap-1);
+    p = __builtin_fma(p, f, 0x1.ffffffffabbccp-1);
+    return __hiloint2double(__double2hiint(p) + (int)((u32)__double2loint(n_word) << 20), __double2loint(p));
+}
+
+// 2^(x c) for x c in [-1000, 900]; lower ones as 2^-1000: so far below any sum that `good` lets pass that it changes
+// nothing.
 struct Power {
     typedef double Sum;
     double c;
     float lo;
     __device__ __forceinline__ double operator()(float x) const {
-        const double y = (double)maximum(x, lo) * c, t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
-        double p = 0x1.fe1786b50da52p-17;
-        p = __builtin_fma(p, f, 0x1.446a1fdd54f3ap-13);
-        p = __builtin_fma(p, f, 0x1.5d8a7085cddb8p-10);
-        p = __builtin_fma(p, f, 0x1.3b29dc40d2ec5p-7);
-        p = __builtin_fma(p, f, 0x1.c6b08aaf3156ep-5);
-        p = __builtin_fma(p, f, 0x1.ebfbe0a4be886p-3);
-        p = __builtin_fma(p, f, 0x1.62e42ff11627ap-1);
-        p = __builtin_fma(p, f, 0x1.ffffffffabbccp-1);
-        return __hiloint2double(__double2hiint(p) + (int)((u32)__double2loint(t) << 20), __double2loint(p));
+        const double v = (double)maximum(x, lo), t = __builtin_fma(v, c, 0x1.8p52);
+        return power_of(t, __builtin_fma(v, c, 0x1.8p52 - t));
+    }
+};
+
+// 2^((x - m) c): for rows whose logits are too far from 0 for Power
+struct PowerBelow {
+    typedef double Sum;
+    double c, m;
+    __device__ __forceinline__ double operator()(float x) const {
+        const double y = fmax(((double)x - m) * c, -1000.), t = y + 0x1.8p52;
+        return power_of(t, y - (t - 0x1.8p52));
     }
 };
 constexpr double MARGIN = 1e-10;
@@ -48,14 +66,18 @@ struct Definition {
     __device__ __forceinline__ double operator()(float x) const { return exp(((double)x - m) / t); }
 };
 
-// whether sums of Power stand: no exponent was too large, not all were too small, and no NaN
-__device__ __forceinline__ bool good(double z, float m, double c) { return z >= 0x1p-900 && (double)m * c <= 900.; }
+// whether a row with this largest logit suits Power: no exponent too large, not all too small
+__device__ __forceinline__ bool good(float m, double c) { return fabs((double)m * c) <= 900.; }
 
-// -log2 p of a token drawn under sums of Power
-__device__ __forceinline__ float ml2p_under(double z, double c, float x) {
+// what a row gives that has no draw: nothing left, or a NaN or +inf
+__device__ __forceinline__ bool drawable(float m) { return fabsf(m) < INFINITY; }
+__device__ __forceinline__ float no_draw(float m) { return m == -INFINITY ? INFINITY : NAN; }
+
+// -log2 p of a token whose exponent is y, under a sum in 64 bits
+__device__ __forceinline__ float ml2p_under(double z, double y) {
     int e;
     const double m = frexp(z, &e);
-    return (float)(((double)e - (double)x * c) + (double)log2f((float)m));
+    return (float)(((double)e - y) + (double)log2f((float)m));
 }
 
 struct DrawArgs {
@@ -161,27 +183,27 @@ __global__ __launch_bounds__(BLOCK, 6) void k_logits_draw_sub(Rows a, DrawArgs d
     if (NV > 4) forget(r);
     u32 token;
     float x;
-    bool sure = draw_sub<DT, G>(r, Fast{Expo(st, a.c)}, u, d.margin, token, x, st.s) && !doubtful(st, a.c);
+    bool sure = draw_sub<DT, G>(r, Fast{Expo(st, a.c)}, u, d.margin, token, x, st.s) && !doubtful(st.m, a.c);
     float ml2p = ml2p_of(0, st, x, a.c);
+    if (!drawable(st.m)) sure = true, token = (u32)MC_TOKEN_OUTSIDE, ml2p = no_draw(st.m);
     if (!live) sure = true, token = (u32)MC_TOKEN_SKIP, ml2p = 0.f;
     if (__ballot(!sure)) {  // the whole wave decides again, in 64 bits
         forget(r);
+        const double m = (double)st.m;
         u32 again;
-        float x_again;
         double z;
-        bool now = draw_sub<DT, G>(r, d.power, u, MARGIN, again, x_again, z) && good(z, st.m, d.power.c);
-        if (!sure && now) {
+        bool now = draw_sub<DT, G>(r, PowerBelow{d.power.c, m}, u, MARGIN, again, x, z);
+        if (!sure) {
             token = again;
-            ml2p = ml2p_under(z, d.power.c, x_again);
+            ml2p = ml2p_under(z, ((double)x - m) * d.power.c);
         }
         now = now || sure;
-        if (__ballot(!now)) {  // and again, from the definition
+        if (__ballot(!now)) {  // and again, by the definition
             forget(r);
-            st = sub_sums<DT, G, false, true>(r, st.m, a.c);
-            draw_sub<DT, G>(r, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u, 0., again, x_again, z);
+            draw_sub<DT, G>(r, Definition{d.t, m}, u, 0., again, x, z);
             if (!now) {
-                token = st.s > 0.f ? again : (u32)MC_TOKEN_OUTSIDE;
-                ml2p = ml2p_of(0, st, x_again, a.c);
+                token = again;
+                ml2p = ml2p_under(z, ((double)x - m) * d.power.c);
             }
         }
     }
@@ -196,7 +218,7 @@ constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 4;
 
 // The token by the definition's weights (every thread of the workgroup calls).
 template <int DT>
-__device__ __forceinline__ u32 draw_exact(const char *p, const Rows &a, const Definition &weight, double u) {
+__device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token) {
     double mine = 0., total;
     for (u32 v = threadIdx.x; v < a.nvec; v += WIDE) {
 #pragma unroll 1
@@ -231,12 +253,14 @@ __device__ __forceinline__ u32 draw_exact(const char *p, const Rows &a, const De
                 hit = got != 0xFFFFFFFFu ? got : last;  // (the vector's sum exceeds the target, its running sum by a rounding not)
             }
             __syncthreads();
-            return hit;
+            token = hit;
+            return total;
         }
         before += step;
     }
     // u Z at or behind the last running sum: the last token with any weight
-    return 0xFFFFFFFFu - block_min<WIDE>(0xFFFFFFFFu - last);
+    token = 0xFFFFFFFFu - block_min<WIDE>(0xFFFFFFFFu - last);
+    return total;
 }
 
 struct LocateShared {
@@ -248,8 +272,8 @@ struct LocateShared {
 
 // The token among vectors v0 .. v1, whose running sums begin at `before`: rounds of STEPS vectors a thread, of which every
 // wave's sum of every step is compared.
-template <int DT>
-__device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Rows &a, const Power &weight, u32 v0, u32 v1, double before,
+template <int DT, typename W>
+__device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, double before,
                                        double target, double margin, u32 &token, float &x) {
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (u32 base = v0; base < v1; base += WIDE * STEPS) {
@@ -319,6 +343,19 @@ __device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Ro
     return false;
 }
 
+// The token, from the sums of a row's parts of `share` vectors (lane i holds part i's).
+template <int DT, typename W>
+__device__ __forceinline__ bool find(LocateShared &sh, const char *p, const Rows &a, const W &weight, double mine, u32 share, double u,
+                                     u32 &token, float &x, double &z) {
+    const double inc = group_scan<64>(mine);
+    z = __shfl(inc, 63);
+    const double target = u * z;
+    const u64 passes = __ballot(inc > target);
+    if (!passes) return false;
+    const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
+    return locate<DT>(sh, p, a, weight, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
+}
+
 // How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose sums another launch joins.
 struct Split {
     u32 shift, vecs;
@@ -326,8 +363,8 @@ struct Split {
 };
 
 // the wave's sum and largest logit over its share of vectors v0 .. v1
-template <int DT, int STRIDE>
-__device__ __forceinline__ void sum_vecs(const char *p, const Rows &a, const Power &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
+template <int DT, int STRIDE, typename W>
+__device__ __forceinline__ void sum_vecs(const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
     s = 0.;
     m = -INFINITY;
     for (u32 v = v0; v < v1; v += STRIDE * UNROLL) {
@@ -415,33 +452,37 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d, Spl
     }
     // lane i holds part i
     m = group_all<64>(m, Max());
-    const double inc = group_scan<64>(mine), z = __shfl(inc, 63), target = u * z;
-    const u64 passes = __ballot(inc > target);
-    u32 token = 0;
-    float x = 0.f;
-    bool sure = false;
-    if (good(z, m, d.power.c) && passes) {
-        const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
-        sure = locate<DT>(sh, p, a, d.power, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
-    }
-    if (sure) {
+    if (!drawable(m)) {
         if (threadIdx.x == 0) {
-            d.token[row] = (int)token;
-            d.ml2p[row] = ml2p_under(z, d.power.c, x);
+            d.token[row] = MC_TOKEN_OUTSIDE;
+            d.ml2p[row] = no_draw(m);
         }
         return;
     }
-    float top = -INFINITY;
-    for (u32 v = threadIdx.x; v < a.nvec; v += WIDE) {
-        const raw4 q = load_vec<DT>(p, a, v, a.nvec);
-#pragma unroll
-        for (int j = 0; j < VEC<DT>; ++j) top = fmaxf(top, unpack<DT>(q, j));
+    u32 token = 0;
+    float x = 0.f;
+    double z = 0., ref = 0.;
+    bool sure = false;
+    if (good(m, d.power.c)) {
+        sure = find<DT>(sh, p, a, d.power, mine, share, u, token, x, z);
+    } else {
+        const PowerBelow weight{d.power.c, ref = (double)m};
+        share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES;
+        double s;
+        sum_vecs<DT, 64>(p, a, weight, min(wave * share, a.nvec), min(a.nvec, (wave + 1) * share), lane, s, m);
+        __syncthreads();
+        if (lane == 0) ps[wave] = s;
+        __syncthreads();
+        sure = find<DT>(sh, p, a, weight, lane < WIDE_WAVES ? ps[lane] : 0., share, u, token, x, z);
     }
-    const Stat st = exact_stat<DT, WIDE, false>(p, a, block_max<WIDE>(top));
-    if (st.s > 0.f) token = draw_exact<DT>(p, a, Definition{d.t, (double)fmaxf(st.m, LOWEST)}, u);
+    if (!sure) {
+        ref = (double)block_max<WIDE>(m);
+        z = draw_exact<DT>(p, a, Definition{d.t, ref}, u, token);
+        x = element<DT>(p, token);
+    }
     if (threadIdx.x == 0) {
-        d.token[row] = st.s > 0.f ? (int)token : MC_TOKEN_OUTSIDE;
-        d.ml2p[row] = ml2p_of(0, st, st.s > 0.f ? element<DT>(p, token) : 0.f, a.c);
+        d.token[row] = (int)token;
+        d.ml2p[row] = ml2p_under(z, ((double)x - ref) * d.power.c);
     }
 }
 
@@ -461,24 +502,73 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 double margin_of(uint64_t vocab) { return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)vocab) + 24); }
 
 // ---- keys ----------------------------------------------------------------------------------------------------------
-// one lane a password
-__global__ __launch_bounds__(BLOCK) void k_logits_keys(const float *ml2p, const i64 *offsets, const void *lengths, u32 length_bytes,
-                                                       u64 count, i64 stride, u64 longest, double *out) {
-    for (u64 i = (u64)blockIdx.x * BLOCK + threadIdx.x; i < count; i += (u64)gridDim.x * BLOCK) {
-        u64 from = 0, to = 0;
-        const float *p = ml2p;
-        if (offsets) {
-            // (offsets that do not ascend or leave the array name no symbols: nothing is read through them)
-            const i64 lo = offsets[i], hi = offsets[i + 1];
-            if (lo >= 0 && hi > lo && (u64)hi <= longest) from = (u64)lo, to = (u64)hi;
-        } else {
-            p += (i64)i * stride;
-            const i64 n = length_bytes == 8 ? ((const i64 *)lengths)[i] : length_bytes == 4 ? (i64)((const int *)lengths)[i] : (i64)longest;
-            to = n < 0 ? 0 : (u64)n > longest ? longest : (u64)n;
-        }
+struct KeyArgs {
+    const float *ml2p;
+    const i64 *offsets;
+    const void *lengths;
+    u32 length_bytes;
+    u64 count, longest;
+    i64 stride;
+    double *out;
+};
+
+__device__ __forceinline__ double key_of(double sum) { return sum == INFINITY ? 1022.0 : sum; }
+
+// Password i's values p[0 .. n).  (Offsets that do not ascend or leave the array name none: nothing is read through them.)
+__device__ __forceinline__ u64 values_of(const KeyArgs &k, u64 i, u64 &from) {
+    from = 0;
+    if (k.offsets) {
+        const i64 lo = k.offsets[i], hi = k.offsets[i + 1];
+        if (lo < 0 || hi <= lo || (u64)hi > k.longest) return 0;
+        from = (u64)lo;
+        return (u64)(hi - lo);
+    }
+    from = (u64)((i64)i * k.stride);
+    const i64 n = k.length_bytes == 8 ? ((const i64 *)k.lengths)[i] : k.length_bytes == 4 ? (i64)((const int *)k.lengths)[i] : (i64)k.longest;
+    return n < 0 ? 0 : (u64)n > k.longest ? k.longest : (u64)n;
+}
+
+// a group of G lanes a password
+template <int G>
+__global__ __launch_bounds__(BLOCK) void k_logits_keys(KeyArgs k) {
+    const u32 lane = threadIdx.x & (G - 1);
+    const u64 step = (u64)gridDim.x * (BLOCK / G);
+    for (u64 first = (u64)blockIdx.x * (BLOCK / G); first < k.count; first += step) {
+        const u64 i = first + threadIdx.x / G;
+        u64 from = 0;
+        const u64 n = i < k.count ? values_of(k, i, from) : 0;
+        const float *p = k.ml2p + from;
         double s = 0.;
-        for (u64 k = from; k < to; ++k) s += (double)p[k];
-        out[i] = s == INFINITY ? 1022.0 : s;
+        for (u64 j = lane; j < n; j += G) s += (double)p[j];
+        s = group_all<G>(s, Add());
+        if (i < k.count && lane == 0) k.out[i] = key_of(s);
+    }
+}
+
+// Packed passwords of a few symbols, one lane a password: the workgroup's values lie side by side and go through LDS (a
+// lane that reads its own password's from memory touches a line of its own with every load: 71 us for 2e6 passwords of 12
+// symbols).  What does not fit the window is read from memory.
+constexpr u32 WINDOW = 4096;
+__global__ __launch_bounds__(BLOCK) void k_logits_keys_packed(KeyArgs k) {
+    __shared__ float win[WINDOW];
+    for (u64 first = (u64)blockIdx.x * BLOCK; first < k.count; first += (u64)gridDim.x * BLOCK) {
+        const u64 last = min(first + BLOCK, k.count), i = first + threadIdx.x;
+        const i64 lo = k.offsets[first], hi = k.offsets[last];
+        const u64 base = lo >= 0 && (u64)lo <= k.longest ? (u64)lo : 0;
+        const u32 n = hi > (i64)base && (u64)hi <= k.longest ? (u32)min((u64)hi - base, (u64)WINDOW) : 0u;
+        for (u32 j = threadIdx.x; j < n; j += BLOCK) win[j] = k.ml2p[base + j];
+        u64 from = 0;
+        const u64 m = i < k.count ? values_of(k, i, from) : 0;
+        __syncthreads();
+        double s = 0.;
+        if (from >= base && from + m <= base + n) {
+            const float *p = win + (u32)(from - base);
+            for (u32 j = 0; j < (u32)m; ++j) s += (double)p[j];
+        } else {
+            for (u64 j = 0; j < m; ++j) s += (double)k.ml2p[from + j];
+        }
+        if (i < k.count) k.out[i] = key_of(s);
+        __syncthreads();
     }
 }
 
@@ -534,9 +624,15 @@ extern "C" int mc_logits_keys(const float *ml2p, const int64_t *offsets, const v
     if (lengths && length_bytes != 4 && length_bytes != 8) return bad(who, "lengths of 4 or 8 bytes");
     if (count == 0) return MC_OK;
     if (!out_keys || (longest && !ml2p)) return bad(who, "null pointer");
-    const u64 blocks = (count + BLOCK - 1) / BLOCK;
-    hipLaunchKernelGGL(k_logits_keys, dim3((u32)(blocks < 65536 ? blocks : 65536)), dim3(BLOCK), 0, (hipStream_t)stream, ml2p,
-                       (const i64 *)offsets, lengths, lengths ? length_bytes : 0u, (u64)count, (i64)stride, (u64)longest, out_keys);
+    const KeyArgs k{ml2p, (const i64 *)offsets, lengths, lengths ? length_bytes : 0u, (u64)count, (u64)longest, (i64)stride, out_keys};
+    hipStream_t s = (hipStream_t)stream;
+    const u64 usual = offsets ? longest / count : longest;  // symbols of a password, or as many as it may have
+    const auto blocks = [&](u64 group) { return dim3((u32)std::min<u64>((count * group + BLOCK - 1) / BLOCK, 1u << 20)); };
+    if (offsets && usual <= 64 && count >= 4096) hipLaunchKernelGGL(k_logits_keys_packed, blocks(1), dim3(BLOCK), 0, s, k);
+    else if (usual <= 2) hipLaunchKernelGGL(k_logits_keys<1>, blocks(1), dim3(BLOCK), 0, s, k);
+    else if (usual <= 8) hipLaunchKernelGGL(k_logits_keys<4>, blocks(4), dim3(BLOCK), 0, s, k);
+    else if (usual <= 64) hipLaunchKernelGGL(k_logits_keys<16>, blocks(16), dim3(BLOCK), 0, s, k);
+    else hipLaunchKernelGGL(k_logits_keys<64>, blocks(64), dim3(BLOCK), 0, s, k);
     HIP_TRY(hipGetLastError());
     return MC_OK;
 }

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOu
     SubRow<DT, NV> r;
     load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
-    const Stat st = sub_stat<DT, G, ENT>(r, a.c, tok != MC_TOKEN_SKIP);
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
     if (!there) return;
     if (lane == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, a.c);
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(T, 8) void k_logits_gradient_held(Rows a, GradOut o
     st = block_stat<T, ENT>(st, a.c);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) asm("" : "+v"(q[i]));
-    if (doubtful(st, a.c)) st = exact_stat<DT, T, ENT>(p, a, st.m);
+    if (doubtful(st.m, a.c)) st = exact_stat<DT, T, ENT>(p, a, st.m);
     if (threadIdx.x == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, a.c);
         if (ENT) out.entropy[row] = entropy_of(tok, st);
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_join(Rows a, GradOut 
             st = Stat{f.x, f.y, f.z, false};
         }
         st = group_stat<64, ENT>(st, a.c);
-        if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
     }
     __syncthreads();  // (every wave has read the parts)
     if (threadIdx.x == 0) {

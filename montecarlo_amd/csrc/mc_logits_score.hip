@@ -89,7 +89,7 @@ __global__ __launch_bounds__(BLOCK, TOP ? 6 : 8) void k_logits_score_sub(Rows a,
     SubRow<DT, NV> r;
     load_row<DT, G>(r, p, a, tok != MC_TOKEN_SKIP);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
-    const Stat st = sub_stat<DT, G, ENT>(r, a.c, tok != MC_TOKEN_SKIP);
+    const Stat st = sub_stat<DT, G, ENT>(r, a.c);
     if (there && lane == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, a.c);
         if (ENT && out.entropy) out.entropy[row] = entropy_of(tok, st);
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_score(Rows a, ScoreOut out,
             for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) keys[i << sp.shift] = 0;
         }
     } else {
-        if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
         u32 n = 0;
         const u64 *cand = nullptr;
         if constexpr (TOP) {
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
         st = Stat{f.x, f.y, f.z, false};
     }
     st = group_stat<64, ENT>(st, a.c);
-    if (doubtful(st, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+    if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
     u32 n = 0;
     const u64 *cand = nullptr;
     if constexpr (TOP) {

@@ -113,10 +113,10 @@ def logits_score(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: flo
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top: 0 .. {min(MAX_TOP, vocab)} alternatives, not {top}")
     rows, dev = logits.shape[:-1], logits.device
-    ml2p = torch.empty(rows, dtype=torch.float32, device=dev)
-    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
-    ids = torch.empty((*rows, top), dtype=torch.int32, device=dev) if top else None
-    vals = torch.empty((*rows, top), dtype=torch.float32, device=dev) if top else None
+    ml2p = logits.new_empty(rows, dtype=torch.float32)
+    ent = logits.new_empty(rows, dtype=torch.float32) if entropy else None
+    ids = logits.new_empty((*rows, top), dtype=torch.int32) if top else None
+    vals = logits.new_empty((*rows, top), dtype=torch.float32) if top else None
     need = nv.lib.mc_logits_score_workspace_bytes(code, outer * inner, vocab, top)
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_score, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
@@ -141,7 +141,7 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
     temperature = _temperature(temperature)
     rows, dev = logits.shape[:-1], logits.device
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out = logits.new_empty(logits.shape)
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError("out: a contiguous tensor of the logits' shape, type and device is needed")
@@ -153,8 +153,8 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
             last = first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
             if first < hi and lo < last:
                 raise ValueError(f"out overlaps {name}")
-    ml2p = torch.empty(rows, dtype=torch.float32, device=dev)
-    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy_weights is not None else None
+    ml2p = logits.new_empty(rows, dtype=torch.float32)
+    ent = logits.new_empty(rows, dtype=torch.float32) if entropy_weights is not None else None
     need = nv.lib.mc_logits_gradient_workspace_bytes(code, outer * inner, vocab)
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_gradient, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
@@ -184,8 +184,8 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
     if live is not None:
         _beside("live", live, logits, (torch.bool,))
         live = live.contiguous()
-    tokens = torch.empty(shape, dtype=torch.int32, device=dev)
-    ml2p = torch.empty(shape, dtype=torch.float32, device=dev)
+    tokens = logits.new_empty(shape, dtype=torch.int32)
+    ml2p = logits.new_empty(shape, dtype=torch.float32)
     need = nv.lib.mc_logits_draw_workspace_bytes(code, rows, vocab)
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_draw, logits.data_ptr(), code, rows, vocab, stride, temperature, _ptr(uniforms),
@@ -224,7 +224,7 @@ def logits_keys(ml2p: torch.Tensor, lengths: Optional[torch.Tensor] = None, *,
             ml2p = ml2p.contiguous()
         lengths = lengths.contiguous() if lengths is not None else None
         count, stride, longest = ml2p.shape[0], ml2p.stride(0), ml2p.shape[1]
-    keys = torch.empty(count, dtype=torch.float64, device=dev)
+    keys = ml2p.new_empty(count, dtype=torch.float64)
     _call(dev, nv.lib.mc_logits_keys, ml2p.data_ptr(), _ptr(offsets), _ptr(lengths),
           lengths.element_size() if lengths is not None else 0, count, stride, longest, keys.data_ptr())
     return keys
