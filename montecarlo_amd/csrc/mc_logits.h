@@ -501,13 +501,17 @@ __device__ __forceinline__ float take(Stat &st, const raw4 (&q)[UNROLL], float c
     if (ENT) st.e = __builtin_fmaf(d, st.s, st.e) * f;
     st.s *= f;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+    for (int u = 0; u < UNROLL; ++u) {
+        float s = 0.f, e = 0.f;  // (a vector's own, so that fewer additions follow each other)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const float y = __builtin_fmaf(unpack<DT>(q[u], j), c, -M), w = exp2_(y);
-            st.s += w;
-            if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
+            s += w;
+            if (ENT) e = __builtin_fmaf(w, fmaxf(y, -FAR), e);
         }
+        st.s += s;
+        if (ENT) st.e += e;
+    }
     return m;
 }
 

@@ -1,12 +1,13 @@
 // Draws from rows of logits by inversion, and the keys of whole passwords (formulas: mc_logits_score.hip).
 //
 // The draw is defined by running sums in 64 bits.  Sums in 32 bits are known to e = a few parts in 10^6 and leave the token
-// open where u Z lies nearer than that to an end of its interval: at most a share 2 e V of the draws.  Rows of
-// up to 4096 tokens begin with them (a row in a thousand is open at V = 97) and take what is open again in 64 bits; a
-// vocabulary of 10^5 tokens has intervals as narrow as e, every other draw would be open, and wider rows begin with 64 bits.
-// Weights then come from a polynomial that is right to 4e-11 (sixteen operations an element, which this GPU does at the
-// rate of 32 bits), and where u Z lies within 1e-10 Z of an end (a row in 10^5) the row is summed once more with the library's
-// exponential.  Exponents of 64 bits reach far enough that no maximum has to be known first.
+// open where u Z lies nearer than that to an end of its interval: a share sum of min(p_i, 2 e) of the draws, one in a
+// thousand at V = 97, one in 20 at V = 32768, every third where 10^5 tokens are about equally likely.  Every row begins
+// with them (seven operations an element; 64 bits take sixteen) and is summed again in 64 bits where they leave
+// it open; only rows too few to fill the GPU, which wait for their loads and not for arithmetic, begin with 64 bits.
+// Weights in 64 bits come from a polynomial that is right to 4e-11 (this GPU does them at the rate of 32 bits), and where u Z
+// lies within 1e-10 Z of an end (a row in 10^5) the row is summed once more with the library's exponential.  Exponents of
+// 64 bits reach far enough that no maximum has to be known first.
 #include "mc_logits.h"
 
 #include <algorithm>
@@ -216,144 +217,92 @@ __global__ __launch_bounds__(BLOCK, 6) void k_logits_draw_sub(Rows a, DrawArgs d
 // ---- rows of many tokens ---------------------------------------------------------------------------------------------------
 constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 4;
 
-// The token by the definition's weights (every thread of the workgroup calls).
+// The token by the definition's weights, by one wave.  (Seldom: where sums that are right to 1e-10 leave it open.)
 template <int DT>
-__device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token) {
-    double mine = 0., total;
-    for (u32 v = threadIdx.x; v < a.nvec; v += WIDE) {
+__device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token, float &x) {
+    const u32 lane = threadIdx.x & 63;
+    double z = 0.;
 #pragma unroll 1
-        for (u32 i = v * VEC<DT>; i < min((v + 1) * VEC<DT>, a.vocab); ++i) mine += weight(element<DT>(p, i));
-    }
-    block_scan<WIDE>(mine, total);
-    const double target = u * total;
+    for (u32 i = lane; i < a.vocab; i += 64) z += weight(element<DT>(p, i));
+    z = group_all<64>(z, Add());
+    const double target = u * z;
     double before = 0.;
-    u32 last = 0;
-    __shared__ u32 hit;
-    for (u32 base = 0; base < a.nvec; base += WIDE) {
-        const u32 from = (base + threadIdx.x) * VEC<DT>, to = min(from + VEC<DT>, a.vocab);
-        double s = 0., step;
+    token = 0;
 #pragma unroll 1
-        for (u32 i = from; i < to; ++i) {
-            const double w = weight(element<DT>(p, i));
-            if (w > 0.) last = i;
-            s += w;
+    for (u32 base = 0; base < a.vocab; base += 64) {
+        const float e = base + lane < a.vocab ? element<DT>(p, base + lane) : -INFINITY;
+        const double w = weight(e), inc = before + group_scan<64>(w);
+        const u64 over = __ballot(w > 0. && inc > target), some = __ballot(w > 0.);
+        // (none yet: the last token with any weight stands in for a target at or behind the last running sum)
+        if (some) {
+            const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u - (u32)__clzll((long long)some);
+            token = base + who;
+            x = __shfl(e, who);
         }
-        const double lo = before + block_scan<WIDE>(s, step);
-        const u32 first = block_min<WIDE>(lo + s > target ? threadIdx.x : 0xFFFFFFFFu);
-        if (first != 0xFFFFFFFFu) {
-            if (threadIdx.x == first) {
-                double run = lo;
-                u32 got = 0xFFFFFFFFu;
-#pragma unroll 1
-                for (u32 i = from; i < to; ++i) {
-                    const double w = weight(element<DT>(p, i));
-                    run += w;
-                    if (got == 0xFFFFFFFFu && w > 0. && run > target) got = i;
-                }
-                hit = got != 0xFFFFFFFFu ? got : last;  // (the vector's sum exceeds the target, its running sum by a rounding not)
-            }
-            __syncthreads();
-            token = hit;
-            return total;
-        }
-        before += step;
+        if (over) break;
+        before = __shfl(inc, 63);
     }
-    // u Z at or behind the last running sum: the last token with any weight
-    token = 0xFFFFFFFFu - block_min<WIDE>(0xFFFFFFFFu - last);
-    return total;
+    return z;
 }
 
-struct LocateShared {
-    double sums[STEPS * WIDE_WAVES];
-    u32 token;
-    float x;
-    int sure;
-};
-
-// The token among vectors v0 .. v1, whose running sums begin at `before`: rounds of STEPS vectors a thread, of which every
-// wave's sum of every step is compared.
+// The token among vectors v0 .. v1, whose running sums begin at `before`, by one wave: the sums of rounds of STEPS steps of
+// 64 vectors.  False when the target lies within `margin` of an end of the token's interval.
 template <int DT, typename W>
-__device__ __forceinline__ bool locate(LocateShared &sh, const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, double before,
-                                       double target, double margin, u32 &token, float &x) {
-    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (u32 base = v0; base < v1; base += WIDE * STEPS) {
+__device__ __forceinline__ bool locate(const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, double before, double target, double margin,
+                                       u32 &token, float &x) {
+    typedef typename W::Sum Sum;
+    const u32 lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (u32 base = v0; base < v1; base += 64 * STEPS) {
         raw4 q[STEPS];
-        double s[STEPS];
+        Sum s[STEPS];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(p, a, base + i * WIDE + threadIdx.x, v1);
-        if (threadIdx.x == 0) sh.sure = 0;
+        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(p, a, base + i * 64 + lane, v1);
+        raw4 mq = q[0];
+        Sum ms = 0;
+        double start = before, run = before;
+        u32 step = 0;
+        bool found = false;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            s[i] = 0.;
-            if (base + i * WIDE < v1) {
+            s[i] = 0;
 #pragma unroll
-                for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(q[i], j));
-            }
-            const double all = group_all<64>(s[i], Add());
-            if (lane == 0) sh.sums[i * WIDE_WAVES + wave] = all;
+            for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(q[i], j));
+            const double all = (double)group_all<64>(s[i], Add());
+            const bool here = !found && run + all > target;
+            choose(mq, q[i], here);
+            ms = here ? s[i] : ms;
+            start = here ? run : start;
+            step = here ? i : step;
+            found = found || here;
+            run += all;
         }
-        __syncthreads();
-        static_assert(STEPS * WIDE_WAVES <= 64, "one lane for each sum");
-        const double mine = lane < STEPS * WIDE_WAVES ? sh.sums[lane] : 0., inc = group_scan<64>(mine);
-        const u64 passes = __ballot(before + inc > target);
-        if (passes) {
-            const u32 which = (u32)__ffsll((unsigned long long)passes) - 1;
-            const double start = before + __shfl(inc - mine, which);
-            if (which % WIDE_WAVES == wave) {
-                const u32 step = which / WIDE_WAVES;
-                raw4 mq = q[0];
-                double ms = s[0];
+        if (found) {
+            const Sum minc = group_scan<64>(ms);
+            const u64 over = __ballot(start + (double)minc > target);
+            const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u;
+            double at_lo = start + (double)(minc - ms);
+            u32 got = 0;
+            float got_x = 0.f;
+            bool sure = false;
 #pragma unroll
-                for (int i = 1; i < STEPS; ++i) {
-                    choose(mq, q[i], i == (int)step);
-                    ms = i == (int)step ? s[i] : ms;
+            for (int j = 0; j < VEC<DT>; ++j) {
+                const float e = unpack<DT>(mq, j);
+                const double next = at_lo + (double)weight(e);
+                if (!sure && target - at_lo >= margin && next - target >= margin) {
+                    sure = true;
+                    got = (base + step * 64 + lane) * VEC<DT> + j;
+                    got_x = e;
                 }
-                const double minc = group_scan<64>(ms);
-                const u64 over = __ballot(start + minc > target);
-                const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u;
-                if (lane == who) {
-                    double run = start + (minc - ms);
-                    int sure = 0;
-                    u32 got = 0;
-                    float got_x = 0.f;
-#pragma unroll
-                    for (int j = 0; j < VEC<DT>; ++j) {
-                        const float e = unpack<DT>(mq, j);
-                        const double next = run + weight(e);
-                        if (!sure && over && target - run >= margin && next - target >= margin) {
-                            sure = 1;
-                            got = (base + step * WIDE + threadIdx.x) * VEC<DT> + j;
-                            got_x = e;
-                        }
-                        run = next;
-                    }
-                    sh.token = got;
-                    sh.x = got_x;
-                    sh.sure = sure;
-                }
+                at_lo = next;
             }
-            __syncthreads();
-            token = sh.token;
-            x = sh.x;
-            return sh.sure;
+            token = __shfl(got, who);
+            x = __shfl(got_x, who);
+            return over && __shfl((int)sure, who);
         }
-        before += __shfl(inc, 63);
-        __syncthreads();
+        before = run;
     }
     return false;
-}
-
-// The token, from the sums of a row's parts of `share` vectors (lane i holds part i's).
-template <int DT, typename W>
-__device__ __forceinline__ bool find(LocateShared &sh, const char *p, const Rows &a, const W &weight, double mine, u32 share, double u,
-                                     u32 &token, float &x, double &z) {
-    const double inc = group_scan<64>(mine);
-    z = __shfl(inc, 63);
-    const double target = u * z;
-    const u64 passes = __ballot(inc > target);
-    if (!passes) return false;
-    const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
-    return locate<DT>(sh, p, a, weight, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
 }
 
 // How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose sums another launch joins.
@@ -410,12 +359,38 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
     }
 }
 
-// One workgroup a row: its waves' (or the parts') sums say in which of them the token lies; that part is looked at again.
-template <int DT, bool PART>
-__global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d, Split sp) {
-    __shared__ LocateShared sh;
+// A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave.  (Sums of Power are those of
+// PowerBelow for m = 0 but for roundings far below the margin.)
+template <int DT>
+__device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 row, const char *p, const PowerBelow &weight, float m, double mine,
+                                          u32 share, double u) {
+    const double inc = group_scan<64>(mine);
+    double z = __shfl(inc, 63), ref = weight.m;
+    const double target = u * z;
+    const u64 passes = __ballot(inc > target);
+    u32 token = 0;
+    float x = 0.f;
+    bool sure = false;
+    if (passes) {
+        const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
+        sure = locate<DT>(p, a, weight, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
+    }
+    if (!sure) {
+        ref = (double)m;
+        z = draw_exact<DT>(p, a, Definition{d.t, ref}, u, token, x);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        d.token[row] = (int)token;
+        d.ml2p[row] = ml2p_under(z, ((double)x - ref) * d.power.c);
+    }
+}
+
+// One workgroup a row.  Its waves sum a share of it each, and the wave whose share holds the token looks at it again.
+template <int DT>
+__global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
+    __shared__ float pm[WIDE_WAVES], pf[WIDE_WAVES];
     __shared__ double ps[WIDE_WAVES];
-    __shared__ float pm[WIDE_WAVES];
+    __shared__ int done;
     const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (row >= a.rows) return;
     if (d.live && !d.live[row]) {
@@ -427,31 +402,25 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d, Spl
     }
     const char *p = at(a.logits, a.inner, row);
     const double u = uniform_of(d, row);
-    u32 share;
-    double mine = 0.;
-    float m = -INFINITY;
-    if constexpr (PART) {
-        share = sp.vecs;
-        if (lane < (1u << sp.shift)) {
-            const double2 f = sp.stats[((u64)row << sp.shift) + lane];
-            mine = f.x;
-            m = (float)f.y;
-        }
-    } else {
-        share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES;
-        const u32 v0 = min(wave * share, a.nvec), v1 = min(a.nvec, v0 + share);
-        double s;
-        sum_vecs<DT, 64>(p, a, d.power, v0, v1, lane, s, m);
-        if (lane == 0) {
-            ps[wave] = s;
-            pm[wave] = m;
-        }
-        __syncthreads();
-        if (lane < WIDE_WAVES) mine = ps[lane];
-        m = lane < WIDE_WAVES ? pm[lane] : -INFINITY;
+    const u32 share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, a.nvec), v1 = min(a.nvec, v0 + share);
+    Stat st{-INFINITY, 0.f, 0.f, false};
+    for (u32 v = v0; v < v1; v += 64 * UNROLL) {
+        raw4 q[UNROLL];
+        load_chunk<DT, 64>(q, p, a, v, lane, v1);
+        take<DT, false>(st, q, a.c);
     }
-    // lane i holds part i
-    m = group_all<64>(m, Max());
+    st = group_stat<64, false>(st, a.c);
+    if (lane == 0) {
+        pm[wave] = st.m;
+        pf[wave] = st.s;
+    }
+    if (threadIdx.x == 0) done = 0;
+    __syncthreads();
+    // lane i holds wave i's sums, under its own largest logit
+    Stat mine{-INFINITY, 0.f, 0.f, false};
+    if (lane < WIDE_WAVES) mine.m = pm[lane], mine.s = pf[lane];
+    st.m = group_all<64>(mine.m, Max());
+    const float m = st.m;
     if (!drawable(m)) {
         if (threadIdx.x == 0) {
             d.token[row] = MC_TOKEN_OUTSIDE;
@@ -459,31 +428,75 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d, Spl
         }
         return;
     }
-    u32 token = 0;
-    float x = 0.f;
-    double z = 0., ref = 0.;
-    bool sure = false;
-    if (good(m, d.power.c)) {
-        sure = find<DT>(sh, p, a, d.power, mine, share, u, token, x, z);
-    } else {
-        const PowerBelow weight{d.power.c, ref = (double)m};
-        share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES;
-        double s;
-        sum_vecs<DT, 64>(p, a, weight, min(wave * share, a.nvec), min(a.nvec, (wave + 1) * share), lane, s, m);
+    if (!doubtful(m, a.c)) {
+        const Fast weight{Expo(st, a.c)};
+        const double w = (double)(mine.s * exp2_(scaled(mine.m, a.c) - weight.y_of.M)), inc = group_scan<64>(w);
+        const double z = __shfl(inc, 63), target = u * z;
+        const u64 passes = __ballot(inc > target);
+        const u32 part = passes ? (u32)__ffsll((unsigned long long)passes) - 1 : WIDE_WAVES;
+        if (wave == part) {
+            u32 token = 0;
+            float x = 0.f;
+            if (locate<DT>(p, a, weight, v0, v1, __shfl(inc - w, part), target, d.margin * z, token, x) && lane == 0) {
+                d.token[row] = (int)token;
+                d.ml2p[row] = ml2p_under(z, (double)weight.y_of.fast(x));
+                done = 1;
+            }
+        }
         __syncthreads();
-        if (lane == 0) ps[wave] = s;
-        __syncthreads();
-        sure = find<DT>(sh, p, a, weight, lane < WIDE_WAVES ? ps[lane] : 0., share, u, token, x, z);
+        if (done) return;
     }
-    if (!sure) {
-        ref = (double)block_max<WIDE>(m);
-        z = draw_exact<DT>(p, a, Definition{d.t, ref}, u, token);
-        x = element<DT>(p, token);
+    // in 64 bits
+    const bool suits = good(m, d.power.c);
+    double s;
+    float unused;
+    if (suits) sum_vecs<DT, 64>(p, a, d.power, v0, v1, lane, s, unused);
+    else sum_vecs<DT, 64>(p, a, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
+    if (lane == 0) ps[wave] = s;
+    __syncthreads();
+    const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), target = u * __shfl(inc, 63);
+    const u64 passes = __ballot(inc > target);
+    if (wave != (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) return;
+    put_token<DT>(a, d, row, p, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u);
+}
+
+// The parts of a row joined, one wave a row.
+template <int DT>
+__global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Split sp) {
+    const u32 row = block_id(), lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
+    if (d.live && !d.live[row]) {
+        if (lane == 0) {
+            d.token[row] = MC_TOKEN_SKIP;
+            d.ml2p[row] = 0.f;
+        }
+        return;
     }
-    if (threadIdx.x == 0) {
-        d.token[row] = (int)token;
-        d.ml2p[row] = ml2p_under(z, ((double)x - ref) * d.power.c);
+    const char *p = at(a.logits, a.inner, row);
+    const double u = uniform_of(d, row);
+    double mine = 0.;
+    float m = -INFINITY;
+    if (lane < (1u << sp.shift)) {
+        const double2 f = sp.stats[((u64)row << sp.shift) + lane];
+        mine = f.x;
+        m = (float)f.y;
     }
+    m = group_all<64>(m, Max());
+    if (!drawable(m)) {
+        if (lane == 0) {
+            d.token[row] = MC_TOKEN_OUTSIDE;
+            d.ml2p[row] = no_draw(m);
+        }
+        return;
+    }
+    const bool suits = good(m, d.power.c);
+    const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
+    if (!suits) {
+        float unused;
+        sum_vecs<DT, 64>(p, a, weight, 0, a.nvec, lane, mine, unused);
+        if (lane) mine = 0.;
+    }
+    put_token<DT>(a, d, row, p, weight, m, mine, suits ? sp.vecs : a.nvec, u);
 }
 
 // Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
@@ -496,10 +509,14 @@ u32 split_shift(u32 rows, u32 nvec) {
 
 size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * 16 : 0; }
 
-// How far off running sums of Fast over a row of few tokens may be, as a share of Z, in half steps of 32 bits: the weights (2
-// for the power; the exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions
-// in a vector, 8 over vectors, 6 over lanes, 2 where parts are joined; twice, since u Z is such a sum too.
-double margin_of(uint64_t vocab) { return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)vocab) + 24); }
+// How far off running sums of Fast may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
+// exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions in a vector, those
+// over a lane's vectors, each chunk's scaling, 6 additions over lanes, and 16 where parts are joined; twice, since u Z is such
+// a sum too.
+double margin_of(const Rows &a) {
+    const double vecs = a.nvec <= SUB_VECS ? 8 : (double)(a.nvec / WIDE + 1), chunks = a.nvec <= SUB_VECS ? 0 : vecs / UNROLL + 1;
+    return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)a.vocab) + 8 + vecs + 4 * chunks + 6 + 16);
+}
 
 // ---- keys ----------------------------------------------------------------------------------------------------------
 struct KeyArgs {
@@ -591,7 +608,7 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (!out_token || !out_ml2p) return bad(who, "no output");
     hipStream_t s = (hipStream_t)stream;
     const double c = LOG2E / temperature;
-    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(vocab), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
     if (a.nvec <= SUB_VECS) {
         BY_TYPE(dtype, BY_GROUP(a, hipLaunchKernelGGL((k_logits_draw_sub<DT, G, NV>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
     } else {
@@ -606,10 +623,10 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
             sp.stats = (double2 *)workspace;
                 BY_TYPE(dtype, {
                 hipLaunchKernelGGL((k_logits_draw_sums<DT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, d, sp);
-                hipLaunchKernelGGL((k_logits_draw<DT, true>), grid_of(a.rows), dim3(WIDE), 0, s, a, d, sp);
+                hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(64), 0, s, a, d, sp);
             });
         } else {
-                BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT, false>), grid_of(a.rows), dim3(WIDE), 0, s, a, d, sp));
+                BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(WIDE), 0, s, a, d));
         }
     }
     HIP_TRY(hipGetLastError());
