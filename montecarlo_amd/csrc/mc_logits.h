@@ -122,21 +122,41 @@ __device__ __forceinline__ raw4 nothing() {
     return raw4{Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF, Elt<DT>::NEG_INF};
 }
 
+// A row as vectors: `nvec` of them from p on, the first `full` whole, `vocab` elements in all.  head: 1 where the row's
+// first element stays before them, so that vectors of 2-byte elements begin at a multiple of 4 (rows of 50001 tokens, every
+// other one odd: score 61 -> 51 us, gradient 125 -> 103 us for 2684 rows).
+struct Span {
+    const char *p;
+    u32 head, vocab, nvec, full;
+    float first;  // the head's logit, or -inf
+};
+
+template <int DT>
+__device__ __forceinline__ Span span_of(const Rows &a, const char *row) {
+    if constexpr (Elt<DT>::BYTES == 2) {
+        if ((uintptr_t)row & 2) {
+            const u32 n = a.vocab - 1;
+            return Span{row + 2, 1, n, (n + VEC<DT> - 1) / VEC<DT>, n / VEC<DT>, element<DT>(row, 0)};
+        }
+    }
+    return Span{row, 0, a.vocab, a.nvec, a.full, -INFINITY};
+}
+
 // vector v of a row; what lies behind the row's end, or in vectors from `end` on, is -inf
 template <int DT>
-__device__ __forceinline__ raw4 load_vec(const char *row, const Rows &a, u32 v, u32 end) {
+__device__ __forceinline__ raw4 load_vec(const Span &r, u32 v, u32 end) {
     constexpr u32 N = VEC<DT>;
     raw4 q = nothing<DT>();
-    if (v < min(end, a.full)) {
-        q = *(const raw4_at2 *)(row + (u64)v * 16);
+    if (v < min(end, r.full)) {
+        q = *(const raw4_at2 *)(r.p + (u64)v * 16);
     } else if (v < end) {
 #pragma unroll
         for (u32 j = 0; j < N; ++j) {
-            if (v * N + j < a.vocab) {
+            if (v * N + j < r.vocab) {
                 if constexpr (Elt<DT>::BYTES == 4) {
-                    q[j] = *(const u32 *)(row + ((u64)v * N + j) * 4);
+                    q[j] = *(const u32 *)(r.p + ((u64)v * N + j) * 4);
                 } else {
-                    const u32 h = *(const unsigned short *)(row + ((u64)v * N + j) * 2);
+                    const u32 h = *(const unsigned short *)(r.p + ((u64)v * N + j) * 2);
                     q[j >> 1] = (j & 1) ? (q[j >> 1] & 0xFFFFu) | (h << 16) : (q[j >> 1] & 0xFFFF0000u) | h;
                 }
             }
@@ -154,8 +174,10 @@ __device__ __forceinline__ u32 pack2(float lo, float hi) {
         return (u32)__builtin_bit_cast(unsigned short, (_Float16)lo) | ((u32)__builtin_bit_cast(unsigned short, (_Float16)hi) << 16);
 }
 
-// the elements from `from` on that the row has room for
-template <int DT, bool MAY_END = true>
+// The elements from `from` on that the row has room for.  STREAM: past the caches (a row of many tokens fills whole lines by
+// itself, and what the gradient does not displace there is read again from there: 200000 tokens 173 -> 137 us; rows of 97
+// tokens leave parts of lines to each other and took twice as long that way).
+template <int DT, bool STREAM, bool MAY_END = true>
 __device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const float *g) {
     constexpr u32 N = VEC<DT>;
     if (!MAY_END || (u64)from + N <= vocab) {
@@ -165,7 +187,9 @@ __device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const f
             if constexpr (Elt<DT>::BYTES == 4) q[j] = __float_as_uint(g[j]);
             else q[j] = pack2<DT>(g[2 * j], g[2 * j + 1]);
         }
-        *(raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES) = q;
+        raw4_at2 *p = (raw4_at2 *)(row + (u64)from * Elt<DT>::BYTES);
+        if (STREAM) __builtin_nontemporal_store(q, p);
+        else *p = q;
     } else {
 #pragma unroll
         for (u32 j = 0; j < N; ++j) {
@@ -394,7 +418,7 @@ __device__ __forceinline__ void load_row(SubRow<DT, NV> &r, const char *p, const
 #pragma unroll
         for (int i = 0; i + 1 < N; ++i) r.q[i] = *(const raw4_at2 *)(p + (u64)(i * G + lane) * 16);
         if (NV == 0) {
-            r.q[0] = load_vec<DT>(p, a, lane, a.nvec);
+            r.q[0] = load_vec<DT>(Span{p, 0, a.vocab, a.nvec, a.full, 0.f}, lane, a.nvec);
         } else if (v < a.nvec) {
             r.from = min(v * E, a.vocab - E);
             r.q[N - 1] = *(const raw4_at2 *)(p + (u64)r.from * Elt<DT>::BYTES);
@@ -517,29 +541,40 @@ __device__ __forceinline__ float take(Stat &st, const raw4 (&q)[UNROLL], float c
 
 // the vectors base + u * STRIDE + lane of a row, as far as they are below `end`
 template <int DT, int STRIDE>
-__device__ __forceinline__ void load_chunk(raw4 (&q)[UNROLL], const char *p, const Rows &a, u32 base, u32 lane, u32 end) {
-    if (base + UNROLL * STRIDE <= min(end, a.full)) {
+__device__ __forceinline__ void load_chunk(raw4 (&q)[UNROLL], const Span &r, u32 base, u32 lane, u32 end) {
+    if (base + UNROLL * STRIDE <= min(end, r.full)) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = *(const raw4_at2 *)(p + (u64)(base + u * STRIDE + lane) * 16);
+        for (int u = 0; u < UNROLL; ++u) q[u] = *(const raw4_at2 *)(r.p + (u64)(base + u * STRIDE + lane) * 16);
     } else {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = load_vec<DT>(p, a, base + u * STRIDE + lane, end);
+        for (int u = 0; u < UNROLL; ++u) q[u] = load_vec<DT>(r, base + u * STRIDE + lane, end);
     }
+}
+
+// one logit joins a thread's running statistics (-inf changes nothing)
+template <bool ENT>
+__device__ __forceinline__ void take_one(Stat &st, float x, float c) {
+    const float old = scaled(st.m, c);
+    st.m = maximum(st.m, x);
+    const float M = scaled(st.m, c), d = old - M, f = exp2_(d), y = __builtin_fmaf(x, c, -M), w = exp2_(y);
+    if (ENT) st.e = __builtin_fmaf(d, st.s, st.e) * f + w * fmaxf(y, -FAR);
+    st.s = st.s * f + w;
 }
 
 // A doubtful row's statistics (every thread of the workgroup calls): m is its largest logit.
 template <int DT, int T, bool ENT>
-__device__ __forceinline__ Stat exact_stat(const char *p, const Rows &a, float m) {
+__device__ __forceinline__ Stat exact_stat(const Span &r, float c, float m) {
     Stat st{m, 0.f, 0.f, true};
-    m = fmaxf(m, LOWEST);
-    for (u32 v = threadIdx.x; v < a.nvec; v += T) {
-        const raw4 q = load_vec<DT>(p, a, v, a.nvec);
+    const auto add = [&](float x) {
+        const float y = (x - m) * c, w = exp2_(y);
+        st.s += w;
+        st.e += w * fmaxf(y, -FAR);
+    };
+    if (threadIdx.x == 0) add(r.first);
+    for (u32 v = threadIdx.x; v < r.nvec; v += T) {
+        const raw4 q = load_vec<DT>(r, v, r.nvec);
 #pragma unroll
-        for (int j = 0; j < VEC<DT>; ++j) {
-            const float y = (unpack<DT>(q, j) - m) * a.c, w = exp2_(y);
-            st.s += w;
-            st.e += w * fmaxf(y, -FAR);
-        }
+        for (int j = 0; j < VEC<DT>; ++j) add(unpack<DT>(q, j));
     }
     __shared__ float ps[T / 64], pe[T / 64];
     st.s = group_all<64>(st.s, Add());
@@ -616,20 +651,19 @@ inline u32 rows_to_blocks(u32 rows, u32 group) { return (u32)(((u64)rows * group
         default: { constexpr int DT = MC_LOGITS_BF16; __VA_ARGS__; break; }            \
     }
 
-// How many lanes share a row (G) and how many vectors each of them holds (NV).  Many rows: the fewest places for vectors, G
-// * NV, and the fewest lanes, since what is done once a row and lane costs as much as eight elements.  Few rows (less than
-// a wave for each of the 1024 SIMDs): the most lanes, since such a launch waits for its loads and its instructions (12 rows of
-// 97 tokens took 15.7 us with 4 lanes, 4.4 with 32).
+// How many lanes share a row (G) and how many vectors each of them holds (NV, at most 8).  Many rows: the fewest lanes, since
+// what is done once a row and lane costs as much as eight elements; but four at least, since two lanes ask for 32 bytes of a
+// row at a time and the loads then take as long as the arithmetic saved (1e6 rows of 97 tokens: 46 us with 4 lanes of 4
+// vectors, 48 with 2 of 7).  Few rows (less than a wave for each of the 1024 SIMDs): a lane for each vector, since such a launch waits for its loads and its instructions (12 rows of 97 tokens took
+// 15.7 us with 4 lanes, 4.4 with 32).
 inline void group_of(u32 rows, u32 vocab, u32 nvec, u32 vec, int &g, int &nv) {
     g = 4, nv = 0;
     if (vocab < vec) return;
-    u32 best = 0xFFFFFFFFu;
-    for (int G = 4; G <= 64; G *= 2) {
-        const u32 n = (nvec + G - 1) / G;
-        if (n > (G == 64 ? 8u : 4u)) continue;
-        const bool few = (u64)rows * G <= 65536;
-        if (best == 0xFFFFFFFFu || n * G < best || (few && nv > 1)) best = n * G, g = G, nv = (int)n;
+    while (nvec > 8u * g) g *= 2;
+    if ((u64)rows * g <= 32768) {
+        while (g < 64 && nvec > (u32)g) g *= 2;
     }
+    nv = (int)((nvec + g - 1) / g);
 }
 
 #define BY_LANES(...)                                              \
@@ -640,6 +674,10 @@ inline void group_of(u32 rows, u32 vocab, u32 nvec, u32 vec, int &g, int &nv) {
         case 32: { constexpr int G = 32; __VA_ARGS__; break; }     \
         default: { constexpr int G = 64; __VA_ARGS__; break; }     \
     }
+// (2 to 4 vectors a lane: the shortest rows and, of few rows, the longest)
+#define BY_ENDS(...)                                               \
+    if (g_ == 4) { constexpr int G = 4; __VA_ARGS__; }             \
+    else { constexpr int G = 64; __VA_ARGS__; }
 
 #define BY_GROUP(a, ...)                                                            \
     {                                                                               \
@@ -648,12 +686,12 @@ inline void group_of(u32 rows, u32 vocab, u32 nvec, u32 vec, int &g, int &nv) {
         switch (nv_) {                                                              \
             case 0: { constexpr int NV = 0, G = 4; __VA_ARGS__; break; }            \
             case 1: { constexpr int NV = 1; BY_LANES(__VA_ARGS__) break; }          \
-            case 2: { constexpr int NV = 2; BY_LANES(__VA_ARGS__) break; }          \
-            case 3: { constexpr int NV = 3; BY_LANES(__VA_ARGS__) break; }          \
-            case 4: { constexpr int NV = 4; BY_LANES(__VA_ARGS__) break; }          \
-            case 5: { constexpr int NV = 5, G = 64; __VA_ARGS__; break; }           \
-            case 6: { constexpr int NV = 6, G = 64; __VA_ARGS__; break; }           \
-            case 7: { constexpr int NV = 7, G = 64; __VA_ARGS__; break; }           \
-            default: { constexpr int NV = 8, G = 64; __VA_ARGS__; break; }          \
+            case 2: { constexpr int NV = 2; BY_ENDS(__VA_ARGS__) break; }           \
+            case 3: { constexpr int NV = 3; BY_ENDS(__VA_ARGS__) break; }           \
+            case 4: { constexpr int NV = 4; BY_ENDS(__VA_ARGS__) break; }           \
+            case 5: { constexpr int NV = 5; BY_LANES(__VA_ARGS__) break; }          \
+            case 6: { constexpr int NV = 6; BY_LANES(__VA_ARGS__) break; }          \
+            case 7: { constexpr int NV = 7; BY_LANES(__VA_ARGS__) break; }          \
+            default: { constexpr int NV = 8; BY_LANES(__VA_ARGS__) break; }         \
         }                                                                           \
     }

@@ -173,7 +173,7 @@ __device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weigh
 }
 
 template <int DT, int G, int NV>
-__global__ __launch_bounds__(BLOCK, 6) void k_logits_draw_sub(Rows a, DrawArgs d) {
+__global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows a, DrawArgs d) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows, live = there && (!d.live || d.live[row]);
     const char *p = there ? at(a.logits, a.inner, row) : nullptr;
@@ -248,16 +248,26 @@ __device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const
 // The token among vectors v0 .. v1, whose running sums begin at `before`, by one wave: the sums of rounds of STEPS steps of
 // 64 vectors.  False when the target lies within `margin` of an end of the token's interval.
 template <int DT, typename W>
-__device__ __forceinline__ bool locate(const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, double before, double target, double margin,
+__device__ __forceinline__ bool locate(const Span &r, const W &weight, u32 v0, u32 v1, double before, double target, double margin,
                                        u32 &token, float &x) {
     typedef typename W::Sum Sum;
     const u32 lane = threadIdx.x & 63;
+    if (v0 == 0 && r.head) {
+        const double next = before + (double)weight(r.first);
+        if (next > target) {
+            token = 0;
+            x = r.first;
+            return next - target >= margin;
+        }
+        if (target - next < margin) return false;
+        before = next;
+    }
 #pragma unroll 1
     for (u32 base = v0; base < v1; base += 64 * STEPS) {
         raw4 q[STEPS];
         Sum s[STEPS];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(p, a, base + i * 64 + lane, v1);
+        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(r, base + i * 64 + lane, v1);
         raw4 mq = q[0];
         Sum ms = 0;
         double start = before, run = before;
@@ -291,7 +301,7 @@ __device__ __forceinline__ bool locate(const char *p, const Rows &a, const W &we
                 const double next = at_lo + (double)weight(e);
                 if (!sure && target - at_lo >= margin && next - target >= margin) {
                     sure = true;
-                    got = (base + step * 64 + lane) * VEC<DT> + j;
+                    got = r.head + (base + step * 64 + lane) * VEC<DT> + j;
                     got_x = e;
                 }
                 at_lo = next;
@@ -313,12 +323,16 @@ struct Split {
 
 // the wave's sum and largest logit over its share of vectors v0 .. v1
 template <int DT, int STRIDE, typename W>
-__device__ __forceinline__ void sum_vecs(const char *p, const Rows &a, const W &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
+__device__ __forceinline__ void sum_vecs(const Span &r, const W &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
     s = 0.;
     m = -INFINITY;
+    if (v0 == 0 && lane == 0 && r.head) {
+        s = weight(r.first);
+        m = r.first;
+    }
     for (u32 v = v0; v < v1; v += STRIDE * UNROLL) {
         raw4 q[UNROLL];
-        load_chunk<DT, STRIDE>(q, p, a, v, lane, v1);
+        load_chunk<DT, STRIDE>(q, r, v, lane, v1);
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i)
 #pragma unroll
@@ -339,11 +353,11 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
     __shared__ float pm[BLOCK / 64];
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
     if (row >= a.rows || (d.live && !d.live[row])) return;
-    const char *p = at(a.logits, a.inner, row);
-    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
+    const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
     double s;
     float m;
-    sum_vecs<DT, BLOCK>(p, a, d.power, v0, v1, threadIdx.x, s, m);
+    sum_vecs<DT, BLOCK>(r, d.power, v0, v1, threadIdx.x, s, m);
     if ((threadIdx.x & 63) == 0) {
         ps[threadIdx.x >> 6] = s;
         pm[threadIdx.x >> 6] = m;
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
 // A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave.  (Sums of Power are those of
 // PowerBelow for m = 0 but for roundings far below the margin.)
 template <int DT>
-__device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 row, const char *p, const PowerBelow &weight, float m, double mine,
+__device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 row, const char *p, const Span &r, const PowerBelow &weight, float m, double mine,
                                           u32 share, double u) {
     const double inc = group_scan<64>(mine);
     double z = __shfl(inc, 63), ref = weight.m;
@@ -373,7 +387,7 @@ __device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 
     bool sure = false;
     if (passes) {
         const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
-        sure = locate<DT>(p, a, weight, part * share, min(a.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
+        sure = locate<DT>(r, weight, part * share, min(r.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
     }
     if (!sure) {
         ref = (double)m;
@@ -401,14 +415,16 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
         return;
     }
     const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
     const double u = uniform_of(d, row);
-    const u32 share = (a.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, a.nvec), v1 = min(a.nvec, v0 + share);
+    const u32 share = (r.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     Stat st{-INFINITY, 0.f, 0.f, false};
     for (u32 v = v0; v < v1; v += 64 * UNROLL) {
         raw4 q[UNROLL];
-        load_chunk<DT, 64>(q, p, a, v, lane, v1);
+        load_chunk<DT, 64>(q, r, v, lane, v1);
         take<DT, false>(st, q, a.c);
     }
+    if (threadIdx.x == 0) take_one<false>(st, r.first, a.c);
     st = group_stat<64, false>(st, a.c);
     if (lane == 0) {
         pm[wave] = st.m;
@@ -437,7 +453,7 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
         if (wave == part) {
             u32 token = 0;
             float x = 0.f;
-            if (locate<DT>(p, a, weight, v0, v1, __shfl(inc - w, part), target, d.margin * z, token, x) && lane == 0) {
+            if (locate<DT>(r, weight, v0, v1, __shfl(inc - w, part), target, d.margin * z, token, x) && lane == 0) {
                 d.token[row] = (int)token;
                 d.ml2p[row] = ml2p_under(z, (double)weight.y_of.fast(x));
                 done = 1;
@@ -450,14 +466,14 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     const bool suits = good(m, d.power.c);
     double s;
     float unused;
-    if (suits) sum_vecs<DT, 64>(p, a, d.power, v0, v1, lane, s, unused);
-    else sum_vecs<DT, 64>(p, a, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
+    if (suits) sum_vecs<DT, 64>(r, d.power, v0, v1, lane, s, unused);
+    else sum_vecs<DT, 64>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
     if (lane == 0) ps[wave] = s;
     __syncthreads();
     const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), target = u * __shfl(inc, 63);
     const u64 passes = __ballot(inc > target);
     if (wave != (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) return;
-    put_token<DT>(a, d, row, p, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u);
+    put_token<DT>(a, d, row, p, r, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u);
 }
 
 // The parts of a row joined, one wave a row.
@@ -473,6 +489,7 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
         return;
     }
     const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
     const double u = uniform_of(d, row);
     double mine = 0.;
     float m = -INFINITY;
@@ -493,10 +510,10 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
     const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
     if (!suits) {
         float unused;
-        sum_vecs<DT, 64>(p, a, weight, 0, a.nvec, lane, mine, unused);
+        sum_vecs<DT, 64>(r, weight, 0, r.nvec, lane, mine, unused);
         if (lane) mine = 0.;
     }
-    put_token<DT>(a, d, row, p, weight, m, mine, suits ? sp.vecs : a.nvec, u);
+    put_token<DT>(a, d, row, p, r, weight, m, mine, suits ? sp.vecs : r.nvec, u);
 }
 
 // Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.

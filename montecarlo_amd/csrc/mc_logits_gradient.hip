@@ -46,12 +46,29 @@ __device__ __forceinline__ void slope_vec(const raw4 &q, u32 from, const Slope &
     }
 }
 
-template <int DT>
-__device__ __forceinline__ void put_zeros(char *gp, u32 from, u32 vocab) {
+// vector v of a row's gradient, which begins at gp
+template <int DT, bool ENT>
+__device__ __forceinline__ void put_slope(char *gp, const Span &r, u32 v, const raw4 &q, const Slope &s, const Expo &y_of, bool exact) {
     float g[VEC<DT>];
+    if (s.none) {
 #pragma unroll
-    for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
-    store_at<DT>(gp, from, vocab, g);
+        for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
+    } else if (exact) {
+        slope_vec<DT, ENT, true>(q, r.head + v * VEC<DT>, s, y_of, g);
+    } else {
+        slope_vec<DT, ENT, false>(q, r.head + v * VEC<DT>, s, y_of, g);
+    }
+    store_at<DT, true>(gp + r.head * Elt<DT>::BYTES, v * VEC<DT>, r.vocab, g);
+}
+
+// the first element of a row whose vectors begin behind it
+template <int DT, bool ENT>
+__device__ __forceinline__ void put_head(char *gp, const Span &r, const Slope &s, const Expo &y_of) {
+    if (!r.head) return;
+    const float y = y_of(r.first), p = exp2_(y) * s.inv;
+    float g = ENT ? p * (s.A - s.B * (fmaxf(y, -FAR) + s.off)) : p * s.A;
+    if (s.tok == 0) g -= s.A;
+    *(unsigned short *)gp = (unsigned short)pack2<DT>(s.none ? 0.f : g, 0.f);
 }
 
 template <int DT, int G, int NV, bool ENT>
@@ -85,45 +102,36 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOu
 #pragma unroll
                 for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
             }
-            store_at<DT, NV == 0>(gp, from, a.vocab, g);
+            store_at<DT, false, NV == 0>(gp, from, a.vocab, g);
         }
     }
 }
 
-// one workgroup a row, the row in its registers
-constexpr int HELD = 8;  // vectors a lane holds
-
-template <int DT, int T, bool ENT>
-__global__ __launch_bounds__(T, 8) void k_logits_gradient_held(Rows a, GradOut out) {
+// one workgroup a row, the row in its registers: HELD vectors a lane at most
+template <int DT, int T, int HELD, bool ENT>
+__global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_gradient_held(Rows a, GradOut out) {
     const u32 row = block_id();
     if (row >= a.rows) return;
     const int tok = token_of(a, row);
     const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
     char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
-    const u32 nv = (a.nvec + T - 1) / T;
-    if (tok == MC_TOKEN_SKIP) {
-        if (threadIdx.x == 0) {
-            out.ml2p[row] = 0.f;
-            if (ENT) out.entropy[row] = 0.f;
-        }
-        for (u32 v = threadIdx.x; v < a.nvec; v += T) put_zeros<DT>(gp, v * VEC<DT>, a.vocab);
-        return;
-    }
+    const u32 nv = (r.nvec + T - 1) / T;
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
-    raw4 q[HELD];
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i < (int)nv) q[i] = load_vec<DT>(p, a, i * T + threadIdx.x, a.nvec);
-    }
     Stat st{-INFINITY, 0.f, 0.f, false};
+    raw4 q[HELD];
+    if (tok != MC_TOKEN_SKIP) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i < (int)nv) {
-#pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) st.m = maximum(st.m, unpack<DT>(q[i], j));
+        for (int i = 0; i < HELD; ++i) {
+            if (i < (int)nv) q[i] = load_vec<DT>(r, i * T + threadIdx.x, r.nvec);
         }
-    }
-    {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (i < (int)nv) {
+#pragma unroll
+                for (int j = 0; j < VEC<DT>; ++j) st.m = maximum(st.m, unpack<DT>(q[i], j));
+            }
+        }
         const Expo y_of(st, a.c);
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
@@ -137,30 +145,23 @@ __global__ __launch_bounds__(T, 8) void k_logits_gradient_held(Rows a, GradOut o
                 }
             }
         }
-    }
-    st = block_stat<T, ENT>(st, a.c);
+        if (threadIdx.x == 0) take_one<ENT>(st, r.first, a.c);
+        st = block_stat<T, ENT>(st, a.c);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) asm("" : "+v"(q[i]));
-    if (doubtful(st.m, a.c)) st = exact_stat<DT, T, ENT>(p, a, st.m);
-    if (threadIdx.x == 0) {
-        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
-        if (ENT) out.entropy[row] = entropy_of(tok, st);
+        for (int i = 0; i < HELD; ++i) asm("" : "+v"(q[i]));
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, T, ENT>(r, a.c, st.m);
     }
     const Slope s = slope_of<ENT>(a, out, row, tok, st);
     const Expo y_of(st, a.c);
+    if (threadIdx.x == 0) {
+        out.ml2p[row] = ml2p_of(tok, st, x, a.c);
+        if (ENT) out.entropy[row] = entropy_of(tok, st);
+        put_head<DT, ENT>(gp, r, s, y_of);
+    }
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const u32 v = i * T + threadIdx.x;
-        if (i < (int)nv && v < a.nvec) {
-            float g[VEC<DT>];
-            if (s.none) {
-                put_zeros<DT>(gp, v * VEC<DT>, a.vocab);
-                continue;
-            }
-            if (st.exact) slope_vec<DT, ENT, true>(q[i], v * VEC<DT>, s, y_of, g);
-            else slope_vec<DT, ENT, false>(q[i], v * VEC<DT>, s, y_of, g);
-            store_at<DT>(gp, v * VEC<DT>, a.vocab, g);
-        }
+        if (i < (int)nv && v < r.nvec) put_slope<DT, ENT>(gp, r, v, q[i], s, y_of, st.exact);
     }
 }
 
@@ -174,14 +175,15 @@ template <int DT, bool ENT>
 __global__ __launch_bounds__(BLOCK) void k_logits_gradient_sums(Rows a, Split sp) {
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
     if (row >= a.rows || token_of(a, row) == MC_TOKEN_SKIP) return;
-    const char *p = at(a.logits, a.inner, row);
-    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
+    const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
     Stat st{-INFINITY, 0.f, 0.f, false};
     for (u32 v = v0; v < v1; v += BLOCK * UNROLL) {
         raw4 q[UNROLL];
-        load_chunk<DT, BLOCK>(q, p, a, v, threadIdx.x, v1);
+        load_chunk<DT, BLOCK>(q, r, v, threadIdx.x, v1);
         take<DT, ENT>(st, q, a.c);
     }
+    if (threadIdx.x == 0 && part == 0) take_one<ENT>(st, r.first, a.c);
     st = block_stat<BLOCK, ENT>(st, a.c);
     if (threadIdx.x == 0) sp.stats[id] = make_float4(st.m, st.s, st.e, 0.f);
 }
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_join(Rows a, GradOut 
             st = Stat{f.x, f.y, f.z, false};
         }
         st = group_stat<64, ENT>(st, a.c);
-        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(span_of<DT>(a, p), a.c, st.m);
     }
     __syncthreads();  // (every wave has read the parts)
     if (threadIdx.x == 0) {
@@ -216,38 +218,33 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_parts(Rows a, GradOut
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
     if (row >= a.rows) return;
     const int tok = token_of(a, row);
-    const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
     char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
-    const u32 v0 = min(part * sp.vecs, a.nvec), v1 = min(a.nvec, v0 + sp.vecs);
+    const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
     const float4 f = sp.stats[(u64)row << sp.shift];
     const Stat st{f.x, f.y, f.z, f.w != 0.f};
     const Slope s = slope_of<ENT>(a, out, row, tok, st);
     const Expo y_of(st, a.c);
+    if (threadIdx.x == 0 && part == 0) put_head<DT, ENT>(gp, r, s, y_of);
     for (u32 v = v0; v < v1; v += BLOCK * UNROLL) {
         raw4 q[UNROLL];
-        if (!s.none) load_chunk<DT, BLOCK>(q, p, a, v, threadIdx.x, v1);
+        if (!s.none) load_chunk<DT, BLOCK>(q, r, v, threadIdx.x, v1);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const u32 mine = v + u * BLOCK + threadIdx.x;
-            if (mine >= v1) continue;
-            float g[VEC<DT>];
-            if (s.none) {
-                put_zeros<DT>(gp, mine * VEC<DT>, a.vocab);
-                continue;
-            }
-            if (st.exact) slope_vec<DT, ENT, true>(q[u], mine * VEC<DT>, s, y_of, g);
-            else slope_vec<DT, ENT, false>(q[u], mine * VEC<DT>, s, y_of, g);
-            store_at<DT>(gp, mine * VEC<DT>, a.vocab, g);
+            if (mine < v1) put_slope<DT, ENT>(gp, r, mine, q[u], s, y_of, st.exact);
         }
     }
 }
+
+constexpr u32 HELD_VECS = 1024 * 16;  // vectors of a row that one workgroup holds
 
 // Parts while there are too few rows to fill the GPU with one workgroup each, or a row is longer than one holds.
 u32 split_shift(u32 rows, u32 nvec) {
     if (nvec <= SUB_VECS) return 0;
     u32 shift = 0;
     while (shift < 6 && ((u64)rows << shift) < 256 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
-    while (shift < 6 && nvec > 1024 * HELD && (nvec >> shift) > 1024 * HELD / 2) ++shift;
+    while (shift < 6 && nvec > HELD_VECS && (nvec >> shift) > HELD_VECS / 4) ++shift;
     return shift;
 }
 
@@ -261,12 +258,14 @@ void launch(const Rows &a, const GradOut &out, const Split &sp, hipStream_t s) {
         hipLaunchKernelGGL((k_logits_gradient_sums<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, sp);
         hipLaunchKernelGGL((k_logits_gradient_join<DT, ENT>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
         hipLaunchKernelGGL((k_logits_gradient_parts<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, out, sp);
-    } else if (a.nvec <= 256 * HELD) {
-        hipLaunchKernelGGL((k_logits_gradient_held<DT, 256, ENT>), grid_of(a.rows), dim3(256), 0, s, a, out);
-    } else if (a.nvec <= 512 * HELD) {
-        hipLaunchKernelGGL((k_logits_gradient_held<DT, 512, ENT>), grid_of(a.rows), dim3(512), 0, s, a, out);
+    } else if (a.nvec <= 256 * 8) {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 256, 8, ENT>), grid_of(a.rows), dim3(256), 0, s, a, out);
+    } else if (a.nvec <= 512 * 8) {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 512, 8, ENT>), grid_of(a.rows), dim3(512), 0, s, a, out);
+    } else if (a.nvec <= 1024 * 8) {
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 1024, 8, ENT>), grid_of(a.rows), dim3(1024), 0, s, a, out);
     } else {
-        hipLaunchKernelGGL((k_logits_gradient_held<DT, 1024, ENT>), grid_of(a.rows), dim3(1024), 0, s, a, out);
+        hipLaunchKernelGGL((k_logits_gradient_held<DT, 1024, 16, ENT>), grid_of(a.rows), dim3(1024), 0, s, a, out);
     }
 }
 

@@ -81,7 +81,7 @@ __device__ __forceinline__ void sub_top(SubRow<DT, NV> &r, const Rows &a, const 
 }
 
 template <int DT, int G, int NV, bool ENT, bool TOP>
-__global__ __launch_bounds__(BLOCK, TOP ? 6 : 8) void k_logits_score_sub(Rows a, ScoreOut out) {
+__global__ __launch_bounds__(BLOCK, !TOP ? 8 : NV > 5 ? 4 : 6) void k_logits_score_sub(Rows a, ScoreOut out) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows;
     const int tok = there ? token_of(a, row) : MC_TOKEN_SKIP;
@@ -104,9 +104,10 @@ constexpr u32 LIST_CAP = 256, CAND_CAP = 512;
 // A pass over the row keeps, beside its sums, the largest logit of every cell (one thread's vectors of some chunks) and,
 // by lane, of all threads of that lane.  The k-th largest of these 64 is a lower bound of the k-th largest of all (about 64
 // ln(64 / (64 - k)) logits of a random row reach it): only the cells that do are looked at again.
+template <int T>
 struct TopShared {
-    float lanes[BLOCK];
-    u64 cand[CAND_CAP];
+    float lanes[T];
+    u64 cand[CAND_CAP + 1];  // (and the row's first element)
     u32 list[LIST_CAP];
     u32 n_list, n_cand;
 };
@@ -125,52 +126,52 @@ __device__ __forceinline__ u32 bound_of(u32 o, u32 k) {
     return least;
 }
 
-template <int DT>
-__device__ __forceinline__ u32 count_from(const char *row, const Rows &a, u32 v0, u32 v1, u32 order) {
+template <int DT, int T>
+__device__ __forceinline__ u32 count_from(const Span &row, u32 v0, u32 v1, u32 order) {
     u32 n = 0;
-    for (u32 v = v0 + threadIdx.x; v < v1; v += BLOCK) {
-        const raw4 q = load_vec<DT>(row, a, v, v1);
+    for (u32 v = v0 + threadIdx.x; v < v1; v += T) {
+        const raw4 q = load_vec<DT>(row, v, v1);
 #pragma unroll
         for (int j = 0; j < VEC<DT>; ++j) n += order_of(unpack<DT>(q, j)) >= order;
     }
-    return block_sum<BLOCK>(n);
+    return block_sum<T>(n);
 }
 
 // The k largest when the candidates do not fit (rows of equal logits, orders made to defeat the cells): the k-th largest
 // value by bits, unless `bound` is it already; then one pass in order of the index.
-template <int DT>
-__device__ __forceinline__ u32 select_by_bits(TopShared &sh, const char *row, const Rows &a, u32 v0, u32 v1, u32 k, u32 bound) {
+template <int DT, int T>
+__device__ __forceinline__ u32 select_by_bits(TopShared<T> &sh, const Span &row, u32 v0, u32 v1, u32 k, u32 bound) {
     u32 kth = bound, above;
     if (bound <= ORDER_NEG_INF) {  // fewer than k lanes hold anything: there may be fewer than k candidates
-        k = min(k, count_from<DT>(row, a, v0, v1, ORDER_NEG_INF + 1));
+        k = min(k, count_from<DT, T>(row, v0, v1, ORDER_NEG_INF + 1));
         if (k == 0) return 0;
         above = 0xFFFFFFFFu;
     } else {
-        above = count_from<DT>(row, a, v0, v1, bound + 1);
+        above = count_from<DT, T>(row, v0, v1, bound + 1);
     }
     if (above >= k) {
         kth = 0;
         for (int b = 31; b >= 0; --b) {
             const u32 t = kth | (1u << b);
-            if (count_from<DT>(row, a, v0, v1, t) >= k) kth = t;
+            if (count_from<DT, T>(row, v0, v1, t) >= k) kth = t;
         }
-        above = count_from<DT>(row, a, v0, v1, kth + 1);
+        above = count_from<DT, T>(row, v0, v1, kth + 1);
     }
     const u32 equal = k - above;
     __syncthreads();
     if (threadIdx.x == 0) sh.n_cand = equal;  // (those above come behind the equal ones, in any order)
     __syncthreads();
     u32 found = 0, base = v0;
-    for (; base < v1 && found < equal; base += BLOCK) {
+    for (; base < v1 && found < equal; base += T) {
         const u32 v = base + threadIdx.x;
-        const raw4 q = load_vec<DT>(row, a, v, v1);
+        const raw4 q = load_vec<DT>(row, v, v1);
         u32 n = 0;
 #pragma unroll
         for (int j = 0; j < VEC<DT>; ++j) n += order_of(unpack<DT>(q, j)) == kth;
-        u32 total, place = found + block_scan<BLOCK>(n, total);
+        u32 total, place = found + block_scan<T>(n, total);
 #pragma unroll
         for (int j = 0; j < VEC<DT>; ++j) {
-            const u32 o = order_of(unpack<DT>(q, j)), i = v * VEC<DT> + j;
+            const u32 o = order_of(unpack<DT>(q, j)), i = row.head + v * VEC<DT> + j;
             if (o == kth && place < equal) sh.cand[place] = key_of(o, i);
             place += o == kth;
             if (o > kth) sh.cand[atomicAdd(&sh.n_cand, 1u)] = key_of(o, i);
@@ -178,12 +179,12 @@ __device__ __forceinline__ u32 select_by_bits(TopShared &sh, const char *row, co
         found += total;
     }
     if (above) {
-        for (u32 v = base + threadIdx.x; v < v1; v += BLOCK) {
-            const raw4 q = load_vec<DT>(row, a, v, v1);
+        for (u32 v = base + threadIdx.x; v < v1; v += T) {
+            const raw4 q = load_vec<DT>(row, v, v1);
 #pragma unroll
             for (int j = 0; j < VEC<DT>; ++j) {
                 const u32 o = order_of(unpack<DT>(q, j));
-                if (o > kth) sh.cand[atomicAdd(&sh.n_cand, 1u)] = key_of(o, v * VEC<DT> + j);
+                if (o > kth) sh.cand[atomicAdd(&sh.n_cand, 1u)] = key_of(o, row.head + v * VEC<DT> + j);
             }
         }
     }
@@ -191,44 +192,55 @@ __device__ __forceinline__ u32 select_by_bits(TopShared &sh, const char *row, co
     return k;
 }
 
+// the row's first element is a candidate of its first part
+template <int T>
+__device__ __forceinline__ u32 add_head(TopShared<T> &sh, const Span &row, u32 v0, u32 n) {
+    if (v0 == 0 && row.first > -INFINITY) {
+        if (threadIdx.x == 0) sh.cand[n] = key_of(order_of(row.first), 0);
+        ++n;
+        __syncthreads();
+    }
+    return n;
+}
+
 // candidates for the k largest of vectors v0 .. v1 into sh.cand: their number (sh.lanes holds the threads' largest)
-template <int DT>
-__device__ __forceinline__ u32 select(TopShared &sh, const float *cells, const char *row, const Rows &a, u32 v0, u32 v1, u32 k, u32 per_cell) {
+template <int DT, int T>
+__device__ __forceinline__ u32 select(TopShared<T> &sh, const float *cells, const Span &row, u32 v0, u32 v1, u32 k, u32 per_cell) {
     if (threadIdx.x == 0) sh.n_list = sh.n_cand = 0;
     __syncthreads();
     float lm = sh.lanes[threadIdx.x & 63];
 #pragma unroll
-    for (int w = 1; w < BLOCK / 64; ++w) lm = fmaxf(lm, sh.lanes[w * 64 + (threadIdx.x & 63)]);
+    for (int w = 1; w < T / 64; ++w) lm = fmaxf(lm, sh.lanes[w * 64 + (threadIdx.x & 63)]);
     const u32 bound = bound_of(order_of(lm), k);
     const u32 cell_vecs = per_cell * UNROLL;
-    for (u32 r = 0; v0 + r * cell_vecs * BLOCK < v1; ++r) {
-        const float m = cells[r * BLOCK + threadIdx.x];
+    for (u32 r = 0; v0 + r * cell_vecs * T < v1; ++r) {
+        const float m = cells[r * T + threadIdx.x];
         if (m > -INFINITY && order_of(m) >= bound) {
             const u32 n = atomicAdd(&sh.n_list, 1u);
-            if (n < LIST_CAP) sh.list[n] = r * BLOCK + threadIdx.x;
+            if (n < LIST_CAP) sh.list[n] = r * T + threadIdx.x;
         }
     }
     __syncthreads();
     const u32 n_list = sh.n_list;
     if (n_list <= LIST_CAP) {
-        for (u32 i = threadIdx.x; i < n_list * cell_vecs; i += BLOCK) {
+        for (u32 i = threadIdx.x; i < n_list * cell_vecs; i += T) {
             const u32 cell = sh.list[i / cell_vecs], u = i % cell_vecs;
-            const u32 v = v0 + ((cell / BLOCK) * cell_vecs + u) * BLOCK + cell % BLOCK;
-            const raw4 q = load_vec<DT>(row, a, v, v1);
+            const u32 v = v0 + ((cell / T) * cell_vecs + u) * T + cell % T;
+            const raw4 q = load_vec<DT>(row, v, v1);
 #pragma unroll
             for (int j = 0; j < VEC<DT>; ++j) {
                 const float x = unpack<DT>(q, j);
                 if (x > -INFINITY && order_of(x) >= bound) {
                     const u32 n = atomicAdd(&sh.n_cand, 1u);
-                    if (n < CAND_CAP) sh.cand[n] = key_of(order_of(x), v * VEC<DT> + j);
+                    if (n < CAND_CAP) sh.cand[n] = key_of(order_of(x), row.head + v * VEC<DT> + j);
                 }
             }
         }
     }
     __syncthreads();
-    const u32 n = sh.n_cand;
-    if (n_list <= LIST_CAP && n <= CAND_CAP) return n;
-    return select_by_bits<DT>(sh, row, a, v0, v1, k, bound);
+    u32 n = sh.n_cand;
+    if (n_list > LIST_CAP || n > CAND_CAP) n = select_by_bits<DT, T>(sh, row, v0, v1, k, bound);
+    return add_head<T>(sh, row, v0, n);
 }
 
 // How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose statistics (and candidates, by place and part)
@@ -251,6 +263,7 @@ __device__ __forceinline__ void put_skipped(const ScoreOut &out, u32 row) {
 }
 
 // a row's statistics are known (to all threads): its outputs, with n candidates for the alternatives
+template <int T>
 __device__ __forceinline__ void put_row(const ScoreOut &out, u32 row, int tok, float x, const Stat &st, float c, const u64 *cand, u32 n) {
     if (threadIdx.x == 0) {
         out.ml2p[row] = ml2p_of(tok, st, x, c);
@@ -259,21 +272,21 @@ __device__ __forceinline__ void put_row(const ScoreOut &out, u32 row, int tok, f
     if (!out.k) return;
     if (!(st.s > 0.f)) n = 0;
     const float lz = log2f(st.s);
-    for (u32 i = threadIdx.x; i < n; i += BLOCK) {
+    for (u32 i = threadIdx.x; i < n; i += T) {
         const u64 key = cand[i];
         u32 rank = 0;
         for (u32 j = 0; j < n; ++j) rank += cand[j] > key;
         if (rank < out.k) put_top(out, row, rank, key, st, lz, c);
     }
-    for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) {
+    for (u32 i = n + threadIdx.x; i < out.k; i += T) {
         out.top[(u64)row * out.k + i] = MC_TOKEN_OUTSIDE;
         out.top_ml2p[(u64)row * out.k + i] = st.s == st.s ? INFINITY : st.s;
     }
 }
 
-template <int DT, bool ENT, bool TOP, bool PART>
-__global__ __launch_bounds__(BLOCK, 8) void k_logits_score(Rows a, ScoreOut out, Split sp) {
-    __shared__ typename std::conditional<TOP, TopShared, int>::type sh;
+template <int DT, int T, bool ENT, bool TOP, bool PART>
+__global__ __launch_bounds__(T, 8) void k_logits_score(Rows a, ScoreOut out, Split sp) {
+    __shared__ typename std::conditional<TOP, TopShared<T>, int>::type sh;
     extern __shared__ float cells[];
     const u32 id = block_id(), row = PART ? id >> sp.shift : id, part = PART ? id & ((1u << sp.shift) - 1) : 0;
     if (row >= a.rows) return;
@@ -283,55 +296,58 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_score(Rows a, ScoreOut out,
         return;
     }
     const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
     const float x = !PART && tok >= 0 ? element<DT>(p, tok) : 0.f;
-    const u32 v0 = PART ? min(part * sp.vecs, a.nvec) : 0, v1 = PART ? min(a.nvec, v0 + sp.vecs) : a.nvec;
-    const u32 chunks = (v1 - v0 + BLOCK * UNROLL - 1) / (BLOCK * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
+    const u32 v0 = PART ? min(part * sp.vecs, r.nvec) : 0, v1 = PART ? min(r.nvec, v0 + sp.vecs) : r.nvec;
+    const u32 chunks = (v1 - v0 + T * UNROLL - 1) / (T * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
     Stat st{-INFINITY, 0.f, 0.f, false};
     float cell = -INFINITY;
-    for (u32 ch = 0, in = 0, r = 0; ch < chunks; ++ch) {
+    for (u32 ch = 0, in = 0, cr = 0; ch < chunks; ++ch) {
         raw4 q[UNROLL];
-        load_chunk<DT, BLOCK>(q, p, a, v0 + ch * BLOCK * UNROLL, threadIdx.x, v1);
+        load_chunk<DT, T>(q, r, v0 + ch * T * UNROLL, threadIdx.x, v1);
         const float m = take<DT, ENT>(st, q, a.c);
         if constexpr (TOP) {
             cell = maximum(cell, m);
             if (++in == per_cell || ch + 1 == chunks) {
-                cells[r++ * BLOCK + threadIdx.x] = cell;
+                cells[cr++ * T + threadIdx.x] = cell;
                 cell = -INFINITY;
                 in = 0;
             }
         }
     }
     if constexpr (TOP) sh.lanes[threadIdx.x] = st.m;
-    st = block_stat<BLOCK, ENT>(st, a.c);
+    if (threadIdx.x == 0 && v0 == 0) take_one<ENT>(st, r.first, a.c);
+    st = block_stat<T, ENT>(st, a.c);
     if constexpr (PART) {
         if (threadIdx.x == 0) sp.stats[id] = make_float4(st.m, st.s, st.e, 0.f);
         if constexpr (TOP) {
-            const u32 n = select<DT>(sh, cells, p, a, v0, v1, out.k, per_cell);
+            const u32 n = select<DT, T>(sh, cells, r, v0, v1, out.k, per_cell);
             u64 *keys = sp.keys + ((u64)row * out.k << sp.shift) + part;
-            for (u32 i = threadIdx.x; i < n; i += BLOCK) {
+            for (u32 i = threadIdx.x; i < n; i += T) {
                 const u64 key = sh.cand[i];
                 u32 rank = 0;
                 for (u32 j = 0; j < n; ++j) rank += sh.cand[j] > key;
                 if (rank < out.k) keys[rank << sp.shift] = key;
             }
-            for (u32 i = n + threadIdx.x; i < out.k; i += BLOCK) keys[i << sp.shift] = 0;
+            for (u32 i = n + threadIdx.x; i < out.k; i += T) keys[i << sp.shift] = 0;
         }
     } else {
-        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, T, ENT>(r, a.c, st.m);
         u32 n = 0;
         const u64 *cand = nullptr;
         if constexpr (TOP) {
-            if (st.s > 0.f) n = select<DT>(sh, cells, p, a, v0, v1, out.k, per_cell);
+            if (st.s > 0.f) n = select<DT, T>(sh, cells, r, v0, v1, out.k, per_cell);
             cand = sh.cand;
         }
-        put_row(out, row, tok, x, st, a.c, cand, n);
+        put_row<T>(out, row, tok, x, st, a.c, cand, n);
     }
 }
 
 // the parts of a row joined
 template <int DT, bool ENT, bool TOP>
 __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut out, Split sp) {
-    __shared__ typename std::conditional<TOP, TopShared, int>::type sh;
+    constexpr int T = BLOCK;
+    __shared__ typename std::conditional<TOP, TopShared<T>, int>::type sh;
     const u32 row = block_id();
     if (row >= a.rows) return;
     const int tok = token_of(a, row);
@@ -340,6 +356,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
         return;
     }
     const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
     const u32 parts = 1u << sp.shift, lane = threadIdx.x & 63;
     Stat st{-INFINITY, 0.f, 0.f, false};
@@ -348,21 +365,21 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
         st = Stat{f.x, f.y, f.z, false};
     }
     st = group_stat<64, ENT>(st, a.c);
-    if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(p, a, st.m);
+    if (doubtful(st.m, a.c)) st = exact_stat<DT, T, ENT>(r, a.c, st.m);
     u32 n = 0;
     const u64 *cand = nullptr;
     if constexpr (TOP) {
         const u32 total = out.k << sp.shift;
         const u64 *keys = sp.keys + (u64)row * total;
         u32 lm = 0;
-        for (u32 i = threadIdx.x; i < total; i += BLOCK) lm = max(lm, (u32)(keys[i] >> 32));
+        for (u32 i = threadIdx.x; i < total; i += T) lm = max(lm, (u32)(keys[i] >> 32));
         if (threadIdx.x == 0) sh.n_cand = 0;
         sh.lanes[threadIdx.x] = __uint_as_float(lm);
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < BLOCK / 64; ++w) lm = max(lm, __float_as_uint(sh.lanes[w * 64 + lane]));
+        for (int w = 0; w < T / 64; ++w) lm = max(lm, __float_as_uint(sh.lanes[w * 64 + lane]));
         const u32 bound = bound_of(lm, out.k);
-        for (u32 i = threadIdx.x; i < total; i += BLOCK) {
+        for (u32 i = threadIdx.x; i < total; i += T) {
             const u64 key = keys[i];
             if (key && (u32)(key >> 32) >= bound) {
                 const u32 at = atomicAdd(&sh.n_cand, 1u);
@@ -371,10 +388,10 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
         }
         __syncthreads();
         n = sh.n_cand;
-        if (n > CAND_CAP) n = select_by_bits<DT>(sh, p, a, 0, a.nvec, out.k, bound);
+        if (n > CAND_CAP) n = add_head<T>(sh, r, 0, select_by_bits<DT, T>(sh, r, 0, r.nvec, out.k, bound));
         cand = sh.cand;
     }
-    put_row(out, row, tok, x, st, a.c, cand, n);
+    put_row<T>(out, row, tok, x, st, a.c, cand, n);
 }
 
 // Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
@@ -385,6 +402,9 @@ u32 split_shift(u32 rows, u32 nvec) {
     return shift;
 }
 
+constexpr int WIDE = 1024;
+constexpr u32 WIDE_VECS = 16384;
+
 u32 split_vecs(u32 nvec, u32 shift) {
     const u32 each = (nvec + (1u << shift) - 1) >> shift;
     return (each + BLOCK * UNROLL - 1) / (BLOCK * UNROLL) * (BLOCK * UNROLL);
@@ -392,16 +412,22 @@ u32 split_vecs(u32 nvec, u32 shift) {
 
 size_t split_bytes(u32 rows, u32 shift, u32 top) { return shift ? ((size_t)rows << shift) * (16 + 8 * (size_t)top) : 0; }
 
+// bytes of the cells of workgroups of `threads` lanes over `vecs` vectors
+size_t cell_bytes(u32 vecs, u32 threads) {
+    const u32 chunks = (vecs + threads * UNROLL - 1) / (threads * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
+    return (chunks + per_cell - 1) / per_cell * threads * sizeof(float);
+}
+
 template <int DT, bool ENT, bool TOP>
 void launch(const Rows &a, const ScoreOut &out, Split sp, hipStream_t s) {
-    const u32 chunks = ((sp.shift ? sp.vecs : a.nvec) + BLOCK * UNROLL - 1) / (BLOCK * UNROLL);
-    const u32 per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
-    const size_t lds = TOP ? (chunks + per_cell - 1) / per_cell * BLOCK * sizeof(float) : 0;
     if (sp.shift) {
-        hipLaunchKernelGGL((k_logits_score<DT, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK), lds, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK),
+                           TOP ? cell_bytes(sp.vecs, BLOCK) : 0, s, a, out, sp);
         hipLaunchKernelGGL((k_logits_score_join<DT, ENT, TOP>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
+    } else if (a.nvec < WIDE_VECS) {
+        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), TOP ? cell_bytes(a.nvec, BLOCK) : 0, s, a, out, sp);
     } else {
-        hipLaunchKernelGGL((k_logits_score<DT, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), lds, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_score<DT, WIDE, ENT, TOP, false>), grid_of(a.rows), dim3(WIDE), TOP ? cell_bytes(a.nvec, WIDE) : 0, s, a, out, sp);
     }
 }
 

@@ -8,7 +8,7 @@ import torch
 from montecarlo_amd import logits as lg
 from montecarlo_amd.lib4mc.MonteCarloLib import MonteCarloLib
 from oracle.philox import uniform53
-from tests.logits_ref import OUTSIDE, SKIP, Row
+from tests.logits_ref import OUTSIDE, SKIP, Row, steps_of
 
 pytestmark = pytest.mark.gpu
 
@@ -345,6 +345,51 @@ def test_keys_of_bad_offsets_and_nan():
     got = lg.logits_keys(m, offsets=off).tolist()
     assert got[:2] == [3.0, 0.0] and got[2] == 6.0 and got[3:7] == [0.0, 0.0, 0.0, 0.0] and math.isnan(got[7])
     assert lg.logits_keys(torch.empty(0).cuda(), offsets=torch.zeros(4, dtype=torch.int64).cuda()).tolist() == [0.0] * 3
+
+
+# ---- many rows of many tokens: a launch that gives each row a workgroup (or several, one batch of rows after another) ---
+@pytest.mark.parametrize("vocab,rows,dtype", [(2305, 1500, "fp32"), (5003, 1100, "bf16"), (20001, 1100, "fp16"), (33001, 1030, "fp32"),
+                                              (40001, 1030, "bf16"), (66001, 1030, "fp32"), (100003, 600, "bf16"), (131071, 300, "fp16"),
+                                              (140001, 500, "bf16")])
+def test_many_wide_rows(vocab, rows, dtype):
+    dt = DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g, device="cuda").mul_(2.5).to(dt)
+    some = list(range(26)) + [rows // 2, rows - 2, rows - 1]
+    x[:26] = make(26, vocab, dt, vocab).cuda()
+    cg = torch.Generator().manual_seed(vocab)
+    toks = torch.randint(0, vocab, (rows,), generator=cg)
+    toks[:26] = tokens_for(x[:26].cpu(), 3)
+    w, v = torch.rand(rows, generator=cg), torch.rand(rows, generator=cg) - 0.5
+    u = torch.rand(rows, generator=cg, dtype=torch.float64)
+    r = lg.logits_score(x, toks.cuda(), entropy=True, top=6)
+    sub = lg.LogitScores(*(t[some] for t in r))
+    check_score(x[some].cpu(), toks[some], sub, 1.0, 6)
+    d = lg.logits_draw(x, u.cuda(), temperature=0.9)
+    check_draw(x[some].cpu(), u[some], None, lg.LogitDraws(d.tokens[some], d.ml2p[some]), 0.9)
+    # every row, against each other: the drawn token's score, and gradients that sum to 0 (their roundings apart)
+    again = lg.logits_score(x, d.tokens, temperature=0.9).ml2p
+    fine = torch.isfinite(again)
+    assert (again - d.ml2p)[fine].abs().max().item() <= 2.0 ** -24 * (4 * steps_of(vocab) + 400)
+    for kw in ({}, {"entropy_weights": v.cuda()}):
+        gr = lg.logits_gradient(x, toks.cuda(), w.cuda(), **kw)
+        sub = lg.LogitGradient(gr.ml2p[some], gr.entropy[some] if kw else None, gr.grad[some])
+        check_gradient(x[some].cpu(), toks[some], w[some], v[some] if kw else None, sub, 1.0, dtype)
+        mine = x.clone()
+        lg.logits_gradient(mine, toks.cuda(), w.cuda(), out=mine, **kw)
+        assert torch.equal(mine.nan_to_num(nan=7.0), gr.grad.nan_to_num(nan=7.0))
+        # rows that begin at an odd element, in and out of step with their gradient
+        base = torch.empty(rows, vocab + 1, dtype=dt, device="cuda")
+        base[:, 1:] = x
+        odd = lg.logits_gradient(base[:, 1:], toks.cuda(), w.cuda(), **kw)
+        for a, b in ((odd.grad, gr.grad),):
+            near_enough = (a.float() - b.float()).nan_to_num().abs() <= 2 * torch.finfo(dt).eps * b.float().nan_to_num().abs() + 1e-5 * b.float().nan_to_num().abs().amax(-1, keepdim=True) + 2.0 ** -24
+            assert bool(near_enough.all())
+    base = torch.empty(rows, vocab + 1, dtype=dt, device="cuda")
+    base[:, 1:] = x
+    odd = lg.logits_score(base[:, 1:], toks.cuda(), entropy=True, top=6)
+    assert torch.equal(odd.top_tokens, r.top_tokens)
+    assert torch.equal(lg.logits_draw(base[:, 1:], u.cuda(), temperature=0.9).tokens, d.tokens)
 
 
 # ---- as they are used ----------------------------------------------------------------------------------------------
