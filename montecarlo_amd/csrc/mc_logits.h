@@ -291,6 +291,15 @@ __device__ __forceinline__ double group_all(double x, Op op) {
     return x;
 }
 
+struct AddWords {
+    __device__ __forceinline__ float operator()(float a, float b) const { return __uint_as_float(__float_as_uint(a) + __float_as_uint(b)); }
+};
+
+template <int G>
+__device__ __forceinline__ u32 group_sum(u32 x) {
+    return __float_as_uint(group_all<G>(__uint_as_float(x), AddWords()));
+}
+
 template <int G>
 __device__ __forceinline__ u32 group_min(u32 x) {
     return __float_as_uint(group_all<G>(__uint_as_float(x), Min()));
