@@ -549,14 +549,14 @@ __device__ __forceinline__ float take(Stat &st, const raw4 (&q)[UNROLL], float c
 }
 
 // the vectors base + u * STRIDE + lane of a row, as far as they are below `end`
-template <int DT, int STRIDE>
-__device__ __forceinline__ void load_chunk(raw4 (&q)[UNROLL], const Span &r, u32 base, u32 lane, u32 end) {
-    if (base + UNROLL * STRIDE <= min(end, r.full)) {
+template <int DT, int STRIDE, int U>
+__device__ __forceinline__ void load_chunk(raw4 (&q)[U], const Span &r, u32 base, u32 lane, u32 end) {
+    if (base + U * STRIDE <= min(end, r.full)) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = *(const raw4_at2 *)(r.p + (u64)(base + u * STRIDE + lane) * 16);
+        for (int u = 0; u < U; ++u) q[u] = *(const raw4_at2 *)(r.p + (u64)(base + u * STRIDE + lane) * 16);
     } else {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = load_vec<DT>(r, base + u * STRIDE + lane, end);
+        for (int u = 0; u < U; ++u) q[u] = load_vec<DT>(r, base + u * STRIDE + lane, end);
     }
 }
 

@@ -318,11 +318,13 @@ __device__ __forceinline__ bool locate(const Span &r, const W &weight, u32 v0, u
 // How the work on a row is cut: 2^shift workgroups of `vecs` vectors, whose sums another launch joins.
 struct Split {
     u32 shift, vecs;
-    double2 *stats;  // [row][part]: the sum, the largest logit
+    float *most;   // [row][part]: the largest logit
+    double *sums;  // [row][part][wave]: the waves' shares of the part lie behind each other
 };
+constexpr int PART_WAVES = BLOCK / 64;
 
 // the wave's sum and largest logit over its share of vectors v0 .. v1
-template <int DT, int STRIDE, typename W>
+template <int DT, int U, typename W>
 __device__ __forceinline__ void sum_vecs(const Span &r, const W &weight, u32 v0, u32 v1, u32 lane, double &s, float &m) {
     s = 0.;
     m = -INFINITY;
@@ -330,11 +332,11 @@ __device__ __forceinline__ void sum_vecs(const Span &r, const W &weight, u32 v0,
         s = weight(r.first);
         m = r.first;
     }
-    for (u32 v = v0; v < v1; v += STRIDE * UNROLL) {
-        raw4 q[UNROLL];
-        load_chunk<DT, STRIDE>(q, r, v, lane, v1);
+    for (u32 v = v0; v < v1; v += 64 * U) {
+        raw4 q[U];
+        load_chunk<DT, 64>(q, r, v, lane, v1);
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i)
+        for (int i = 0; i < U; ++i)
 #pragma unroll
             for (int j = 0; j < VEC<DT>; ++j) {
                 const float e = unpack<DT>(q[i], j);
@@ -349,35 +351,32 @@ __device__ __forceinline__ void sum_vecs(const Span &r, const W &weight, u32 v0,
 // the sums of the parts of a row
 template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, Split sp) {
-    __shared__ double ps[BLOCK / 64];
-    __shared__ float pm[BLOCK / 64];
-    const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
+    __shared__ float pm[PART_WAVES];
+    const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (row >= a.rows || (d.live && !d.live[row])) return;
     const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
-    const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
+    const u32 share = sp.vecs / PART_WAVES, v0 = min(part * sp.vecs + wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     double s;
     float m;
-    sum_vecs<DT, BLOCK>(r, d.power, v0, v1, threadIdx.x, s, m);
-    if ((threadIdx.x & 63) == 0) {
-        ps[threadIdx.x >> 6] = s;
-        pm[threadIdx.x >> 6] = m;
+    sum_vecs<DT, 2>(r, d.power, v0, v1, lane, s, m);
+    if (lane == 0) {
+        sp.sums[(u64)id * PART_WAVES + wave] = s;
+        pm[wave] = m;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int w = 1; w < BLOCK / 64; ++w) {
-            s += ps[w];
-            m = maximum(m, pm[w]);
-        }
-        sp.stats[id] = make_double2(s, (double)m);
+        for (int w = 1; w < PART_WAVES; ++w) m = maximum(m, pm[w]);
+        sp.most[id] = m;
     }
 }
 
-// A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave.  (Sums of Power are those of
-// PowerBelow for m = 0 but for roundings far below the margin.)
+// A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave.  `within` (if by_shares): the same
+// for the PART_WAVES shares of the lane's part.  (Sums of Power are those of PowerBelow for m = 0 but for roundings far
+// below the margin.)
 template <int DT>
 __device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 row, const char *p, const Span &r, const PowerBelow &weight, float m, double mine,
-                                          u32 share, double u) {
+                                          u32 share, double u, bool by_shares, const double (&within)[PART_WAVES]) {
     const double inc = group_scan<64>(mine);
     double z = __shfl(inc, 63), ref = weight.m;
     const double target = u * z;
@@ -387,7 +386,20 @@ __device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 
     bool sure = false;
     if (passes) {
         const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
-        sure = locate<DT>(r, weight, part * share, min(r.nvec, (part + 1) * share), __shfl(inc - mine, part), target, MARGIN * z, token, x);
+        double before = __shfl(inc - mine, part);
+        u32 v0 = part * share, v1 = v0 + share;
+        if (by_shares) {
+            v1 = v0;
+            bool found = false;
+#pragma unroll
+            for (int w = 0; w < PART_WAVES; ++w) {
+                const double next = before + __shfl(within[w], part);
+                if (!found) v1 = v0 + share / PART_WAVES;
+                found = found || next > target;
+                if (!found && w + 1 < PART_WAVES) before = next, v0 = v1;
+            }
+        }
+        sure = locate<DT>(r, weight, min(v0, r.nvec), min(r.nvec, v1), before, target, MARGIN * z, token, x);
     }
     if (!sure) {
         ref = (double)m;
@@ -466,14 +478,15 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     const bool suits = good(m, d.power.c);
     double s;
     float unused;
-    if (suits) sum_vecs<DT, 64>(r, d.power, v0, v1, lane, s, unused);
-    else sum_vecs<DT, 64>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
+    if (suits) sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, unused);
+    else sum_vecs<DT, UNROLL>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
     if (lane == 0) ps[wave] = s;
     __syncthreads();
     const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), target = u * __shfl(inc, 63);
     const u64 passes = __ballot(inc > target);
     if (wave != (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) return;
-    put_token<DT>(a, d, row, p, r, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u);
+    const double none[PART_WAVES] = {};
+    put_token<DT>(a, d, row, p, r, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u, false, none);
 }
 
 // The parts of a row joined, one wave a row.
@@ -491,12 +504,13 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
     const char *p = at(a.logits, a.inner, row);
     const Span r = span_of<DT>(a, p);
     const double u = uniform_of(d, row);
-    double mine = 0.;
+    double mine = 0., within[PART_WAVES] = {};
     float m = -INFINITY;
     if (lane < (1u << sp.shift)) {
-        const double2 f = sp.stats[((u64)row << sp.shift) + lane];
-        mine = f.x;
-        m = (float)f.y;
+        const u64 id = ((u64)row << sp.shift) + lane;
+        m = sp.most[id];
+#pragma unroll
+        for (int w = 0; w < PART_WAVES; ++w) mine += within[w] = sp.sums[id * PART_WAVES + w];
     }
     m = group_all<64>(m, Max());
     if (!drawable(m)) {
@@ -510,10 +524,10 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
     const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
     if (!suits) {
         float unused;
-        sum_vecs<DT, 64>(r, weight, 0, r.nvec, lane, mine, unused);
+        sum_vecs<DT, UNROLL>(r, weight, 0, r.nvec, lane, mine, unused);
         if (lane) mine = 0.;
     }
-    put_token<DT>(a, d, row, p, r, weight, m, mine, suits ? sp.vecs : r.nvec, u);
+    put_token<DT>(a, d, row, p, r, weight, m, mine, suits ? sp.vecs : r.nvec, u, suits, within);
 }
 
 // Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
@@ -524,7 +538,7 @@ u32 split_shift(u32 rows, u32 nvec) {
     return shift;
 }
 
-size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * 16 : 0; }
+size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * (8 * PART_WAVES + 4) : 0; }
 
 // How far off running sums of Fast may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
 // exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions in a vector, those
@@ -583,20 +597,30 @@ __global__ __launch_bounds__(BLOCK) void k_logits_keys(KeyArgs k) {
 // lane that reads its own password's from memory touches a line of its own with every load: 71 us for 2e6 passwords of 12
 // symbols).  What does not fit the window is read from memory.
 constexpr u32 WINDOW = 4096;
+typedef float float4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 __global__ __launch_bounds__(BLOCK) void k_logits_keys_packed(KeyArgs k) {
-    __shared__ float win[WINDOW];
+    __shared__ __attribute__((aligned(16))) float win[WINDOW];
     for (u64 first = (u64)blockIdx.x * BLOCK; first < k.count; first += (u64)gridDim.x * BLOCK) {
         const u64 last = min(first + BLOCK, k.count), i = first + threadIdx.x;
         const i64 lo = k.offsets[first], hi = k.offsets[last];
-        const u64 base = lo >= 0 && (u64)lo <= k.longest ? (u64)lo : 0;
-        const u32 n = hi > (i64)base && (u64)hi <= k.longest ? (u32)min((u64)hi - base, (u64)WINDOW) : 0u;
-        for (u32 j = threadIdx.x; j < n; j += BLOCK) win[j] = k.ml2p[base + j];
         u64 from = 0;
         const u64 m = i < k.count ? values_of(k, i, from) : 0;
+        const u64 base = lo >= 0 && (u64)lo <= k.longest ? (u64)lo : 0;
+        const u32 n = hi > (i64)base && (u64)hi <= k.longest ? (u32)min((u64)hi - base, (u64)WINDOW) : 0u;
+#pragma unroll
+        for (u32 u = 0; u < WINDOW / (4 * BLOCK); ++u) {
+            const u32 j = (u * BLOCK + threadIdx.x) * 4;
+            if (j + 4 <= n) {
+                *(float4_at4 *)(win + j) = *(const float4_at4 *)(k.ml2p + base + j);
+            } else {
+                for (u32 t = j; t < n; ++t) win[t] = k.ml2p[base + t];
+            }
+        }
         __syncthreads();
         double s = 0.;
         if (from >= base && from + m <= base + n) {
             const float *p = win + (u32)(from - base);
+#pragma unroll 4
             for (u32 j = 0; j < (u32)m; ++j) s += (double)p[j];
         } else {
             for (u64 j = 0; j < m; ++j) s += (double)k.ml2p[from + j];
@@ -629,7 +653,7 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (a.nvec <= SUB_VECS) {
         BY_TYPE(dtype, BY_GROUP(a, hipLaunchKernelGGL((k_logits_draw_sub<DT, G, NV>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
     } else {
-        Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
+        Split sp{split_shift(a.rows, a.nvec), 0, nullptr, nullptr};
         if (sp.shift) {
             if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);
@@ -637,7 +661,8 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
             }
             const u32 each = (a.nvec + (1u << sp.shift) - 1) >> sp.shift;
             sp.vecs = (each + BLOCK - 1) / BLOCK * BLOCK;
-            sp.stats = (double2 *)workspace;
+            sp.sums = (double *)workspace;
+            sp.most = (float *)(sp.sums + ((size_t)a.rows << sp.shift) * PART_WAVES);
                 BY_TYPE(dtype, {
                 hipLaunchKernelGGL((k_logits_draw_sums<DT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, d, sp);
                 hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(64), 0, s, a, d, sp);

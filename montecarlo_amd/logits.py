@@ -77,12 +77,15 @@ def _temperature(t) -> float:
 
 
 def _call(device: torch.device, fn, *args):
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
-        nv.check(fn(*args, stream))
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            nv.check(fn(*args, stream))
+            rc = fn(*args, stream)
+    if rc:
+        nv.check(rc)
 
 
 def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -117,7 +120,7 @@ def logits_score(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: flo
     ent = logits.new_empty(rows, dtype=torch.float32) if entropy else None
     ids = logits.new_empty((*rows, top), dtype=torch.int32) if top else None
     vals = logits.new_empty((*rows, top), dtype=torch.float32) if top else None
-    need = nv.lib.mc_logits_score_workspace_bytes(code, outer * inner, vocab, top)
+    need = nv.lib.mc_logits_score_workspace_bytes(code, outer * inner, vocab, top) if vocab > 2048 else 0
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_score, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
           tokens.element_size(), tos, tis, temperature, ml2p.data_ptr(), _ptr(ent), top, _ptr(ids), _ptr(vals),
@@ -155,7 +158,7 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
                 raise ValueError(f"out overlaps {name}")
     ml2p = logits.new_empty(rows, dtype=torch.float32)
     ent = logits.new_empty(rows, dtype=torch.float32) if entropy_weights is not None else None
-    need = nv.lib.mc_logits_gradient_workspace_bytes(code, outer * inner, vocab)
+    need = nv.lib.mc_logits_gradient_workspace_bytes(code, outer * inner, vocab) if vocab > 2048 else 0
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_gradient, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
           tokens.element_size(), tos, tis, temperature, weights.data_ptr(), wos, wis, _ptr(entropy_weights), eos, eis,
@@ -186,7 +189,7 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
         live = live.contiguous()
     tokens = logits.new_empty(shape, dtype=torch.int32)
     ml2p = logits.new_empty(shape, dtype=torch.float32)
-    need = nv.lib.mc_logits_draw_workspace_bytes(code, rows, vocab)
+    need = nv.lib.mc_logits_draw_workspace_bytes(code, rows, vocab) if vocab > 2048 else 0
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_draw, logits.data_ptr(), code, rows, vocab, stride, temperature, _ptr(uniforms),
           (seed or 0) & 0xFFFFFFFFFFFFFFFF, first_id & 0xFFFFFFFFFFFFFFFF, draw & 0xFFFFFFFF, _ptr(live), tokens.data_ptr(),
