@@ -116,3 +116,20 @@ def test_tensors_off_the_gpu_are_refused():
                  lambda: lg.logits_draw(x, seed=1), lambda: lg.logits_keys(x)):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_the_plugin_form_is_abstract_and_checks_its_arguments():
+    from montecarlo_amd.logits_simulator import LogitsMonteCarlo
+
+    class Model(LogitsMonteCarlo):
+        def logits(self, tokens):
+            raise NotImplementedError
+
+    with pytest.raises(TypeError):
+        LogitsMonteCarlo(["a", "<end>"], 1, device="cpu")
+    for end, max_len, batch in ((2, 4, 1), (-1, 4, 1), (1, 0, 1), (1, 4, 0)):
+        with pytest.raises(ValueError):
+            Model(["a", "<end>"], end, max_len=max_len, batch=batch, device="cpu")
+    m = Model(["a", "b", "<end>"], 2, device="cpu")
+    assert m.encode("abz") == [0, 1, OUTSIDE]
+    assert m._sampled_strings(torch.tensor([[0, 1, 2, SKIP], [2, SKIP, SKIP, SKIP]])) == ["ab", ""]
