@@ -87,6 +87,7 @@ struct DrawArgs {
     u32 draw;
     double t, margin;        // margin: how far off the running sums of Fast may be, as a share of Z
     Power power;
+    bool begin64;
     const unsigned char *live;
     int *token;
     float *ml2p;
@@ -431,16 +432,22 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     const double u = uniform_of(d, row);
     const u32 share = (r.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     Stat st{-INFINITY, 0.f, 0.f, false};
-    for (u32 v = v0; v < v1; v += 64 * UNROLL) {
-        raw4 q[UNROLL];
-        load_chunk<DT, 64>(q, r, v, lane, v1);
-        take<DT, false>(st, q, a.c);
+    double s = 0.;
+    if (d.begin64) {
+        sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, st.m);
+    } else {
+        for (u32 v = v0; v < v1; v += 64 * UNROLL) {
+            raw4 q[UNROLL];
+            load_chunk<DT, 64>(q, r, v, lane, v1);
+            take<DT, false>(st, q, a.c);
+        }
+        if (threadIdx.x == 0) take_one<false>(st, r.first, a.c);
+        st = group_stat<64, false>(st, a.c);
     }
-    if (threadIdx.x == 0) take_one<false>(st, r.first, a.c);
-    st = group_stat<64, false>(st, a.c);
     if (lane == 0) {
         pm[wave] = st.m;
         pf[wave] = st.s;
+        ps[wave] = s;
     }
     if (threadIdx.x == 0) done = 0;
     __syncthreads();
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
         }
         return;
     }
-    if (!doubtful(m, a.c)) {
+    if (!d.begin64 && !doubtful(m, a.c)) {
         const Fast weight{Expo(st, a.c)};
         const double w = (double)(mine.s * exp2_(scaled(mine.m, a.c) - weight.y_of.M)), inc = group_scan<64>(w);
         const double z = __shfl(inc, 63), target = u * z;
@@ -476,12 +483,14 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     }
     // in 64 bits
     const bool suits = good(m, d.power.c);
-    double s;
-    float unused;
-    if (suits) sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, unused);
-    else sum_vecs<DT, UNROLL>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
-    if (lane == 0) ps[wave] = s;
-    __syncthreads();
+    if (!suits || !d.begin64) {
+        float unused;
+        if (suits) sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, unused);
+        else sum_vecs<DT, UNROLL>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
+        __syncthreads();  // (no wave still reads the first ones)
+        if (lane == 0) ps[wave] = s;
+        __syncthreads();
+    }
     const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), target = u * __shfl(inc, 63);
     const u64 passes = __ballot(inc > target);
     if (wave != (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) return;
@@ -530,11 +539,13 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
     put_token<DT>(a, d, row, p, r, weight, m, mine, suits ? sp.vecs : r.nvec, u, suits, within);
 }
 
-// Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
-u32 split_shift(u32 rows, u32 nvec) {
-    if (nvec <= SUB_VECS) return 0;
+// Few rows begin with 64 bits: they wait for their loads, not for arithmetic, and a row that 32 bits leave open is read again
+// (64 rows of 20000 tokens: 17 us).  Of more than 40000 tokens they are cut into parts that still hold a chunk of 16 KB; a second
+// launch costs 4 us, which shorter rows take less than.
+bool few(u32 rows) { return rows < 512; }
+u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
     u32 shift = 0;
-    while (shift < 6 && ((u64)rows << shift) < 512 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+    while (few(rows) && vocab > 40000 && shift < 6 && ((u64)rows << shift) < 512 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
     return shift;
 }
 
@@ -635,7 +646,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_keys_packed(KeyArgs k) {
 extern "C" size_t mc_logits_draw_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab) {
     if (dtype > MC_LOGITS_BF16 || rows >= (1ull << 31) || vocab >= (1ull << 31)) return 0;
     const u64 per = dtype == MC_LOGITS_F32 ? 4 : 8;
-    return split_bytes((u32)rows, split_shift((u32)rows, (u32)((vocab + per - 1) / per)));
+    return split_bytes((u32)rows, split_shift((u32)rows, (u32)vocab, (u32)((vocab + per - 1) / per)));
 }
 
 extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows, uint64_t vocab, int64_t row_stride,
@@ -649,11 +660,11 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (!out_token || !out_ml2p) return bad(who, "no output");
     hipStream_t s = (hipStream_t)stream;
     const double c = LOG2E / temperature;
-    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, few(a.rows), live, out_token, out_ml2p};
     if (a.nvec <= SUB_VECS) {
         BY_TYPE(dtype, BY_GROUP(a, hipLaunchKernelGGL((k_logits_draw_sub<DT, G, NV>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
     } else {
-        Split sp{split_shift(a.rows, a.nvec), 0, nullptr, nullptr};
+        Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr};
         if (sp.shift) {
             if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);

@@ -239,12 +239,14 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_parts(Rows a, GradOut
 
 constexpr u32 HELD_VECS = 1024 * 16;  // vectors of a row that one workgroup holds
 
-// Parts while there are too few rows to fill the GPU with one workgroup each, or a row is longer than one holds.
+// Parts where a row is longer than one workgroup holds, and where it is half as long and there are few (one row of 131072
+// tokens of two bytes: 18 us either way for a caller who waits for the launches, 18 and 8 us of the GPU).
 u32 split_shift(u32 rows, u32 nvec) {
-    if (nvec <= SUB_VECS) return 0;
     u32 shift = 0;
-    while (shift < 6 && ((u64)rows << shift) < 256 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
-    while (shift < 6 && nvec > HELD_VECS && (nvec >> shift) > HELD_VECS / 4) ++shift;
+    if (nvec > HELD_VECS || (nvec > HELD_VECS / 2 && rows <= 64)) {
+        while (shift < 6 && ((u64)rows << shift) < 256 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+        while (shift < 6 && nvec > HELD_VECS && (nvec >> shift) > HELD_VECS / 4) ++shift;
+    }
     return shift;
 }
 
@@ -252,15 +254,16 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 
 template <int DT, bool ENT>
 void launch(const Rows &a, const GradOut &out, const Split &sp, hipStream_t s) {
+    const bool few = a.rows <= 256 && a.nvec >= 1024;  // (all the lanes there are for each)
     if (a.nvec <= SUB_VECS) {
         BY_GROUP(a, hipLaunchKernelGGL((k_logits_gradient_sub<DT, G, NV, ENT>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out));
     } else if (sp.shift) {
         hipLaunchKernelGGL((k_logits_gradient_sums<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, sp);
         hipLaunchKernelGGL((k_logits_gradient_join<DT, ENT>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
         hipLaunchKernelGGL((k_logits_gradient_parts<DT, ENT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, out, sp);
-    } else if (a.nvec <= 256 * 8) {
+    } else if (a.nvec <= 256 * 8 && !few) {
         hipLaunchKernelGGL((k_logits_gradient_held<DT, 256, 8, ENT>), grid_of(a.rows), dim3(256), 0, s, a, out);
-    } else if (a.nvec <= 512 * 8) {
+    } else if (a.nvec <= 512 * 8 && !few) {
         hipLaunchKernelGGL((k_logits_gradient_held<DT, 512, 8, ENT>), grid_of(a.rows), dim3(512), 0, s, a, out);
     } else if (a.nvec <= 1024 * 8) {
         hipLaunchKernelGGL((k_logits_gradient_held<DT, 1024, 8, ENT>), grid_of(a.rows), dim3(1024), 0, s, a, out);

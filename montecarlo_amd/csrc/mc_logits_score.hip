@@ -487,16 +487,21 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
     put_row<T>(out, row, tok, x, st, a.c, cand, n);
 }
 
-// Rows are cut into parts while there are too few to fill the GPU and the parts still hold a chunk of 16 KB.
-u32 split_shift(u32 rows, u32 nvec) {
-    if (nvec <= SUB_VECS) return 0;
+// Rows of more than 160000 tokens are cut into parts while there are too few to fill the GPU and the parts still hold a chunk
+// of 16 KB.  Shorter ones are not: a second launch costs the caller 4 us, what a workgroup of 1024 lanes takes for 10^5 tokens
+// (one row of 131072: 11 us a call whole, 15 in parts; of 262144: 17 and 15).
+u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
     u32 shift = 0;
-    while (shift < 6 && ((u64)rows << shift) < 1024 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
+    while (vocab > 160000 && shift < 6 && ((u64)rows << shift) < 1024 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
     return shift;
 }
 
+// Lanes of a workgroup that has a row to itself: 1024 for the longest rows (2049 rows of 131073 tokens, a third of them
+// skipped: 197 us with 256 lanes, 137 with 1024: fewer rows at a time share the load evenly) and where there are few rows;
+// else 256, since eight workgroups a compute unit hide each other's phases (8192 rows of 32768 with 10 alternatives: 113 and
+// 178 us).
 constexpr int WIDE = 1024;
-constexpr u32 WIDE_VECS = 16384;
+bool wide(u32 rows, u32 nvec) { return nvec >= 16384 || (rows <= 256 && nvec >= 2048); }
 
 u32 split_vecs(u32 nvec, u32 shift) {
     const u32 each = (nvec + (1u << shift) - 1) >> shift;
@@ -517,7 +522,7 @@ void launch(const Rows &a, const ScoreOut &out, Split sp, hipStream_t s) {
         hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK),
                            TOP ? cell_bytes(sp.vecs, BLOCK) : 0, s, a, out, sp);
         hipLaunchKernelGGL((k_logits_score_join<DT, ENT, TOP>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
-    } else if (a.nvec < WIDE_VECS) {
+    } else if (!wide(a.rows, a.nvec)) {
         hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), TOP ? cell_bytes(a.nvec, BLOCK) : 0, s, a, out, sp);
     } else {
         hipLaunchKernelGGL((k_logits_score<DT, WIDE, ENT, TOP, false>), grid_of(a.rows), dim3(WIDE), TOP ? cell_bytes(a.nvec, WIDE) : 0, s, a, out, sp);
@@ -529,7 +534,7 @@ void launch(const Rows &a, const ScoreOut &out, Split sp, hipStream_t s) {
 extern "C" size_t mc_logits_score_workspace_bytes(uint32_t dtype, uint64_t rows, uint64_t vocab, uint32_t top) {
     if (dtype > MC_LOGITS_BF16 || rows >= (1ull << 31) || vocab >= (1ull << 31) || top > MC_LOGITS_MAX_TOP) return 0;
     const u64 per = dtype == MC_LOGITS_F32 ? 4 : 8;
-    return split_bytes((u32)rows, split_shift((u32)rows, (u32)((vocab + per - 1) / per)), top);
+    return split_bytes((u32)rows, split_shift((u32)rows, (u32)vocab, (u32)((vocab + per - 1) / per)), top);
 }
 
 extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
@@ -557,7 +562,7 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
                     else hipLaunchKernelGGL((k_logits_score_sub<DT, G, NV, false, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out, 0u);
                 }));
     } else {
-        Split sp{split_shift(a.rows, a.nvec), 0, nullptr, nullptr};
+        Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr};
         if (sp.shift) {
             if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift, top) || (uintptr_t)workspace % 16) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift, top), workspace_bytes);

@@ -37,36 +37,38 @@ class LogitDraws(NamedTuple):
 
 
 def _rows(logits: torch.Tensor, most: int = 3):
-    """(dtype code, outer, inner, vocab, outer stride, inner stride) of logits [V], [N, V] or [B, L, V]."""
+    """(dtype code, outer, inner, vocab, outer stride, inner stride, shape of the rows) of logits [V], [N, V] or [B, L, V]."""
     if not logits.is_cuda:
         raise ValueError("logits: a tensor on the GPU is needed (there is no CPU fallback)")
     code = _DTYPES.get(logits.dtype)
     if code is None:
         raise TypeError(f"logits: float32, float16 or bfloat16, not {logits.dtype}")
-    shape, strides = logits.shape, logits.stride()
-    if not 1 <= len(shape) <= most:
-        raise ValueError(f"logits: 1 to {most} dimensions, the last one over the tokens; got {tuple(shape)}")
-    if shape[-1] == 0:
+    shape, strides = tuple(logits.shape), logits.stride()
+    dims = len(shape)
+    if not 1 <= dims <= most:
+        raise ValueError(f"logits: 1 to {most} dimensions, the last one over the tokens; got {shape}")
+    vocab = shape[-1]
+    if vocab == 0:
         raise ValueError("logits: no tokens")
-    if strides[-1] != 1 and shape[-1] > 1:
+    if strides[-1] != 1 and vocab > 1:
         raise ValueError("logits: the tokens of a row must be adjacent (stride 1 in the last dimension)")
-    if len(shape) == 3:
-        return code, shape[0], shape[1], shape[2], strides[0], strides[1]
-    if len(shape) == 2:
-        return code, 1, shape[0], shape[1], 0, strides[0]
-    return code, 1, 1, shape[0], 0, 0
+    if dims == 3:
+        return code, shape[0], shape[1], vocab, strides[0], strides[1], shape[:2]
+    if dims == 2:
+        return code, 1, shape[0], vocab, 0, strides[0], shape[:1]
+    return code, 1, 1, vocab, 0, 0, ()
 
 
-def _beside(name: str, t: torch.Tensor, logits: torch.Tensor, dtypes):
-    """Strides (outer, inner) of a tensor with one value for every row of ``logits``."""
-    if t.device != logits.device:
-        raise ValueError(f"{name}: on {t.device}, the logits are on {logits.device}")
+def _beside(name: str, t: torch.Tensor, dev: torch.device, rows: tuple, dtypes):
+    """Strides (outer, inner) of a tensor with one value for every row."""
+    if t.device != dev:
+        raise ValueError(f"{name}: on {t.device}, the logits are on {dev}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if t.shape != logits.shape[:-1]:
-        raise ValueError(f"{name}: shape {tuple(t.shape)} for rows {tuple(logits.shape[:-1])}")
+    if t.shape != rows:
+        raise ValueError(f"{name}: shape {tuple(t.shape)} for rows {rows}")
     s = t.stride()
-    return (s[0], s[1]) if len(s) == 2 else (0, s[0]) if s else (0, 0)
+    return s if len(s) == 2 else (0, s[0]) if s else (0, 0)
 
 
 def _temperature(t) -> float:
@@ -97,7 +99,7 @@ def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
-_INTS = (torch.int64, torch.int32)
+_INTS, _F32, _F64, _BOOL = (torch.int64, torch.int32), (torch.float32,), (torch.float64,), (torch.bool,)
 
 
 def logits_score(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, entropy: bool = False,
@@ -109,17 +111,17 @@ def logits_score(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: flo
     rows that are not to be read; any other id outside the vocabulary scores +inf, as does a token whose logit is -inf.
     Alternatives are in the order of the logits, equal ones by the lower id; where fewer than ``top`` have any
     probability the rest is ``OUTSIDE`` with +inf."""
-    code, outer, inner, vocab, os, is_ = _rows(logits)
-    tos, tis = _beside("tokens", tokens, logits, _INTS)
+    code, outer, inner, vocab, os, is_, rows = _rows(logits)
+    dev = logits.device
+    tos, tis = _beside("tokens", tokens, dev, rows, _INTS)
     temperature = _temperature(temperature)
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top: 0 .. {min(MAX_TOP, vocab)} alternatives, not {top}")
-    rows, dev = logits.shape[:-1], logits.device
     ml2p = logits.new_empty(rows, dtype=torch.float32)
     ent = logits.new_empty(rows, dtype=torch.float32) if entropy else None
-    ids = logits.new_empty((*rows, top), dtype=torch.int32) if top else None
-    vals = logits.new_empty((*rows, top), dtype=torch.float32) if top else None
+    ids = logits.new_empty(rows + (top,), dtype=torch.int32) if top else None
+    vals = logits.new_empty(rows + (top,), dtype=torch.float32) if top else None
     need = nv.lib.mc_logits_score_workspace_bytes(code, outer * inner, vocab, top) if vocab > 2048 else 0
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_score, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
@@ -137,12 +139,12 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
     result to ``logits.backward(grad)``.  Skipped rows and rows with no token left have gradient 0; a token outside
     the model contributes none.  ``out``: where to put it -- contiguous, of the logits' shape and type, either the
     logits themselves (overwritten) or memory apart from everything that goes in."""
-    code, outer, inner, vocab, os, is_ = _rows(logits)
-    tos, tis = _beside("tokens", tokens, logits, _INTS)
-    wos, wis = _beside("weights", weights, logits, (torch.float32,))
-    eos, eis = _beside("entropy_weights", entropy_weights, logits, (torch.float32,)) if entropy_weights is not None else (0, 0)
+    code, outer, inner, vocab, os, is_, rows = _rows(logits)
+    dev = logits.device
+    tos, tis = _beside("tokens", tokens, dev, rows, _INTS)
+    wos, wis = _beside("weights", weights, dev, rows, _F32)
+    eos, eis = _beside("entropy_weights", entropy_weights, dev, rows, _F32) if entropy_weights is not None else (0, 0)
     temperature = _temperature(temperature)
-    rows, dev = logits.shape[:-1], logits.device
     if out is None:
         out = logits.new_empty(logits.shape)
     else:
@@ -176,16 +178,16 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
     (``seed``, ``first_id`` + r, ``draw``) of the stream that ``DeviceModel.sample`` draws from, so a batch may be cut
     anywhere.  ``live``: bool, rows that are False are not read (``SKIP``, 0).  A row with no token left gives
     ``OUTSIDE`` and +inf."""
-    code, _, rows, vocab, _, stride = _rows(logits, 2)
+    code, _, rows, vocab, _, stride, shape = _rows(logits, 2)
     temperature = _temperature(temperature)
-    dev, shape = logits.device, logits.shape[:-1]
+    dev = logits.device
     if (uniforms is None) == (seed is None):
         raise ValueError("either uniforms or a seed is needed")
     if uniforms is not None:
-        _beside("uniforms", uniforms, logits, (torch.float64,))
+        _beside("uniforms", uniforms, dev, shape, _F64)
         uniforms = uniforms.contiguous()
     if live is not None:
-        _beside("live", live, logits, (torch.bool,))
+        _beside("live", live, dev, shape, _BOOL)
         live = live.contiguous()
     tokens = logits.new_empty(shape, dtype=torch.int32)
     ml2p = logits.new_empty(shape, dtype=torch.float32)

@@ -86,6 +86,16 @@ def test_score(vocab, dtype):
         near(plain.ml2p[i].item(), *Row(x[i].double().numpy(), t).score(toks[i].item()), i)
 
 
+@pytest.mark.parametrize("vocab,dtype", [(200003, "bf16"), (170001, "fp32"), (300000, "fp16")])
+def test_score_of_few_very_wide_rows(vocab, dtype):
+    x = make(25, vocab, DTYPES[dtype], vocab)
+    toks = tokens_for(x, 5)
+    check_score(x, toks, lg.logits_score(x.cuda(), toks.cuda(), temperature=0.9, entropy=True, top=33), 0.9, 33)
+    base = torch.empty(25, vocab + 1, dtype=x.dtype).cuda()
+    base[:, 1:] = x.cuda()
+    check_score(x, toks, lg.logits_score(base[:, 1:], toks.cuda(), entropy=True, top=2), 1.0, 2)
+
+
 @pytest.mark.parametrize("vocab,rows", [(97, 5000), (64, 1023), (700, 777), (5000, 300), (40000, 3)])
 def test_score_many_rows_agree_with_the_same_rows_alone(vocab, rows):
     """Whatever way a launch takes with many rows and with few, each row's alternatives are the same and its score is within
@@ -106,7 +116,7 @@ def test_score_many_rows_agree_with_the_same_rows_alone(vocab, rows):
 
 
 @pytest.mark.parametrize("kind", ["ascending", "descending", "equal", "sawtooth", "two_values", "few_left", "one_left", "spikes"])
-@pytest.mark.parametrize("vocab,dtype", [(1000, "fp32"), (20000, "bf16"), (131073, "fp32"), (70000, "fp16")])
+@pytest.mark.parametrize("vocab,dtype", [(1000, "fp32"), (20000, "bf16"), (131073, "fp32"), (70000, "fp16"), (170001, "bf16")])
 def test_top_in_orders_that_are_hard(kind, vocab, dtype):
     i = torch.arange(vocab, dtype=torch.float32)
     x = {"ascending": i * (30.0 / vocab), "descending": -i * (30.0 / vocab), "equal": torch.zeros(vocab), "sawtooth": (i % 1024) / 64,

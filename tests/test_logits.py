@@ -88,14 +88,14 @@ def test_the_others_refuse(name, args):
 
 
 def test_a_workspace_that_is_too_small_is_refused():
-    need = nv.lib.mc_logits_score_workspace_bytes(0, 2, 100000, 5)
+    need = nv.lib.mc_logits_score_workspace_bytes(0, 2, 300000, 5)
     assert need > 0 and nv.lib.mc_logits_score_workspace_bytes(0, 2, 100, 5) == 0
-    big = dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, inner=2, vocab=100000, top=5, ids=ADDR, vals=ADDR)
+    big = dict(logits=ADDR, tokens=ADDR, ml2p=ADDR, inner=2, vocab=300000, top=5, ids=ADDR, vals=ADDR)
     for ws, size in ((None, need), (ADDR, need - 1), (ADDR + 8, need)):
         assert _score(**big, ws=ws, wsb=size) == -6
-    need = nv.lib.mc_logits_gradient_workspace_bytes(2, 2, 100000)
+    need = nv.lib.mc_logits_gradient_workspace_bytes(2, 2, 300000)
     assert need > 0
-    assert nv.lib.mc_logits_gradient(ADDR, 2, 1, 2, 100000, 0, 100000, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, ADDR,
+    assert nv.lib.mc_logits_gradient(ADDR, 2, 1, 2, 300000, 0, 300000, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, None, 0, 0, ADDR, None, ADDR, ADDR,
                                      need - 1, None) == -6
     need = nv.lib.mc_logits_draw_workspace_bytes(1, 2, 100000)
     assert need > 0
