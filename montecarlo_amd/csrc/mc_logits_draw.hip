@@ -87,7 +87,6 @@ struct DrawArgs {
     u32 draw;
     double t, margin;        // margin: how far off the running sums of Fast may be, as a share of Z
     Power power;
-    bool begin64;
     const unsigned char *live;
     int *token;
     float *ml2p;
@@ -413,8 +412,8 @@ __device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 
 }
 
 // One workgroup a row.  Its waves sum a share of it each, and the wave whose share holds the token looks at it again.
-template <int DT>
-__global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
+template <int DT, bool BEGIN64>
+__global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, DrawArgs d) {
     __shared__ float pm[WIDE_WAVES], pf[WIDE_WAVES];
     __shared__ double ps[WIDE_WAVES];
     __shared__ int done;
@@ -433,7 +432,7 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     const u32 share = (r.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     Stat st{-INFINITY, 0.f, 0.f, false};
     double s = 0.;
-    if (d.begin64) {
+    if constexpr (BEGIN64) {
         sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, st.m);
     } else {
         for (u32 v = v0; v < v1; v += 64 * UNROLL) {
@@ -463,7 +462,7 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
         }
         return;
     }
-    if (!d.begin64 && !doubtful(m, a.c)) {
+    if (!BEGIN64 && !doubtful(m, a.c)) {
         const Fast weight{Expo(st, a.c)};
         const double w = (double)(mine.s * exp2_(scaled(mine.m, a.c) - weight.y_of.M)), inc = group_scan<64>(w);
         const double z = __shfl(inc, 63), target = u * z;
@@ -483,7 +482,7 @@ __global__ __launch_bounds__(WIDE, 8) void k_logits_draw(Rows a, DrawArgs d) {
     }
     // in 64 bits
     const bool suits = good(m, d.power.c);
-    if (!suits || !d.begin64) {
+    if (!suits || !BEGIN64) {
         float unused;
         if (suits) sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, unused);
         else sum_vecs<DT, UNROLL>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
@@ -660,7 +659,7 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (!out_token || !out_ml2p) return bad(who, "no output");
     hipStream_t s = (hipStream_t)stream;
     const double c = LOG2E / temperature;
-    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, few(a.rows), live, out_token, out_ml2p};
+    DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
     if (a.nvec <= SUB_VECS) {
         BY_TYPE(dtype, BY_GROUP(a, hipLaunchKernelGGL((k_logits_draw_sub<DT, G, NV>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, d)));
     } else {
@@ -679,7 +678,10 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
                 hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(64), 0, s, a, d, sp);
             });
         } else {
-                BY_TYPE(dtype, hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(WIDE), 0, s, a, d));
+                BY_TYPE(dtype, {
+                if (few(a.rows)) hipLaunchKernelGGL((k_logits_draw<DT, true>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
+                else hipLaunchKernelGGL((k_logits_draw<DT, false>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
+            });
         }
     }
     HIP_TRY(hipGetLastError());
