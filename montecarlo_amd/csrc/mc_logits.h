@@ -43,6 +43,7 @@ struct Div {
 struct View {
     const char *p;
     i64 os, is;
+    u32 narrow;  // neither stride is negative or needs more than 32 bits
 };
 
 struct Rows {
@@ -53,8 +54,9 @@ struct Rows {
 };
 
 __device__ __forceinline__ const char *at(const View &v, const Div &inner, u32 row) {
-    const u32 o = __umulhi(row << 1, inner.mul) >> inner.shift;
-    return v.p + (i64)o * v.os + (i64)(row - o * inner.d) * v.is;
+    const u32 o = __umulhi(row << 1, inner.mul) >> inner.shift, i = row - o * inner.d;
+    if (v.narrow) return v.p + ((u64)o * (u32)v.os + (u64)i * (u32)v.is);
+    return v.p + (i64)o * v.os + (i64)i * v.is;
 }
 
 // A token id as the kernels use it: [0, V), MC_TOKEN_SKIP, or MC_TOKEN_OUTSIDE for everything else.
@@ -205,6 +207,13 @@ __device__ __forceinline__ void store_at(char *row, u32 from, u32 vocab, const f
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// of sums, which are 0, about 1 or more, or NaN: no scaling of the smallest numbers is needed
+__device__ __forceinline__ float log2_(float s) { return __builtin_amdgcn_logf(s); }
+// 1 / s for a sum other than 0, to about half a step: the instruction's value and one step of Newton's method
+__device__ __forceinline__ float inverse(float s) {
+    const float r = __builtin_amdgcn_rcpf(s);
+    return __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
+}
 
 // A row's (or a part's) largest logit m, the sum s of 2^y and the sum e of 2^y y; `exact` says how y is meant.
 struct Stat {
@@ -230,11 +239,11 @@ __device__ __forceinline__ bool doubtful(float m, float c) { return fabsf(m) < I
 __device__ __forceinline__ float ml2p_of(int tok, const Stat &st, float x, float c) {
     if (tok == MC_TOKEN_SKIP) return 0.f;
     if (!(st.s == st.s)) return st.s;
-    return tok >= 0 && st.s > 0.f ? log2f(st.s) - Expo(st, c)(x) : INFINITY;
+    return tok >= 0 && st.s > 0.f ? log2_(st.s) - Expo(st, c)(x) : INFINITY;
 }
 
 __device__ __forceinline__ float entropy_of(int tok, const Stat &st) {
-    return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : log2f(st.s) - st.e / st.s;
+    return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : log2_(st.s) - st.e * inverse(st.s);
 }
 
 // ---- reductions over groups of lanes and over workgroups ---------------------------------------------------------------
@@ -613,6 +622,11 @@ inline Div make_div(u64 d) {
     return r;
 }
 
+inline View view_of(const void *p, int64_t outer_stride, int64_t inner_stride, int64_t bytes) {
+    const i64 os = outer_stride * bytes, is = inner_stride * bytes;
+    return View{(const char *)p, os, is, os >= 0 && is >= 0 && os < (1ll << 32) && is < (1ll << 32)};
+}
+
 inline bool one_run(uint64_t inner, int64_t outer_stride, int64_t inner_stride) { return outer_stride == (int64_t)inner * inner_stride; }
 
 // the arguments that every entry point on logits shares (`flat`: everything else that a row has lies as one run too)
@@ -630,7 +644,7 @@ inline int rows_of(const char *who, Rows &a, const void *logits, uint32_t dtype,
         inner *= outer;
         outer = 1;
     }
-    a.logits = View{(const char *)logits, outer_stride * bytes, inner_stride * bytes};
+    a.logits = view_of(logits, outer_stride, inner_stride, bytes);
     a.inner = make_div(inner ? inner : 1);
     a.vocab = (u32)vocab;
     a.full = (u32)(vocab / (16 / bytes));
@@ -645,7 +659,7 @@ inline int tokens_of(const char *who, Rows &a, const void *tokens, uint32_t toke
     if (rows && !tokens) return bad(who, "no tokens");
     if ((uintptr_t)tokens % token_bytes) return bad(who, "tokens that are not aligned to their type");
     a.token_bytes = token_bytes;
-    a.tokens = View{(const char *)tokens, outer_stride * (i64)token_bytes, inner_stride * (i64)token_bytes};
+    a.tokens = view_of(tokens, outer_stride, inner_stride, token_bytes);
     return MC_OK;
 }
 

@@ -13,9 +13,9 @@ struct GradOut {
     char *grad;
 };
 
-// what the elements of a row's gradient need
+// What the elements of a row's gradient need: p (C - B y) - [i = t] A with C = A - B (H - log2 Z); all 0 where there is none.
 struct Slope {
-    float A, B, inv, off;
+    float A, B, C, inv;
     bool none;
     int tok;
 };
@@ -24,20 +24,26 @@ template <bool ENT>
 __device__ __forceinline__ Slope slope_of(const Rows &a, const GradOut &out, u32 row, int tok, const Stat &st) {
     Slope s;
     s.none = tok == MC_TOKEN_SKIP || st.s == 0.f;
-    s.A = tok >= 0 ? *(const float *)at(out.weights, a.inner, row) * a.c : 0.f;
-    s.B = ENT ? *(const float *)at(out.entropy_weights, a.inner, row) * out.inv_t : 0.f;
-    s.inv = s.none ? 0.f : 1.f / st.s;
-    s.off = ENT && !s.none ? entropy_of(tok, st) - log2f(st.s) : 0.f;  // log2 p + H = y + off
+    s.A = tok >= 0 && !s.none ? *(const float *)at(out.weights, a.inner, row) * a.c : 0.f;
+    s.B = ENT && !s.none ? *(const float *)at(out.entropy_weights, a.inner, row) * out.inv_t : 0.f;
+    s.inv = s.none ? 0.f : inverse(st.s);
+    s.C = ENT && !s.none ? __builtin_fmaf(st.e * s.inv, s.B, s.A) : s.A;  // (H - log2 Z = -e / Z)
     s.tok = tok;
     return s;
+}
+
+template <bool ENT>
+__device__ __forceinline__ float slope(float y, const Slope &s) {
+    const float p = exp2_(y) * s.inv;
+    return ENT ? p * __builtin_fmaf(-s.B, fmaxf(y, -FAR), s.C) : p * s.A;
 }
 
 template <int DT, bool ENT, bool EXACT>
 __device__ __forceinline__ void slope_vec(const raw4 &q, u32 from, const Slope &s, const Expo &y_of, float *g) {
 #pragma unroll
     for (int j = 0; j < VEC<DT>; ++j) {
-        const float x = unpack<DT>(q, j), y = EXACT ? y_of(x) : y_of.fast(x), p = exp2_(y) * s.inv;
-        g[j] = ENT ? p * (s.A - s.B * (fmaxf(y, -FAR) + s.off)) : p * s.A;
+        const float x = unpack<DT>(q, j);
+        g[j] = slope<ENT>(EXACT ? y_of(x) : y_of.fast(x), s);
     }
     const u32 t = (u32)s.tok - from;
     if (t < (u32)VEC<DT>) {
@@ -65,8 +71,7 @@ __device__ __forceinline__ void put_slope(char *gp, const Span &r, u32 v, const 
 template <int DT, bool ENT>
 __device__ __forceinline__ void put_head(char *gp, const Span &r, const Slope &s, const Expo &y_of) {
     if (!r.head) return;
-    const float y = y_of(r.first), p = exp2_(y) * s.inv;
-    float g = ENT ? p * (s.A - s.B * (fmaxf(y, -FAR) + s.off)) : p * s.A;
+    float g = slope<ENT>(y_of(r.first), s);
     if (s.tok == 0) g -= s.A;
     *(unsigned short *)gp = (unsigned short)pack2<DT>(s.none ? 0.f : g, 0.f);
 }
@@ -98,10 +103,6 @@ __global__ __launch_bounds__(BLOCK, 8) void k_logits_gradient_sub(Rows a, GradOu
             float g[VEC<DT>];
             if (st.exact) slope_vec<DT, ENT, true>(r.q[i], from, s, y_of, g);
             else slope_vec<DT, ENT, false>(r.q[i], from, s, y_of, g);
-            if (s.none) {
-#pragma unroll
-                for (int j = 0; j < VEC<DT>; ++j) g[j] = 0.f;
-            }
             store_at<DT, false, NV == 0>(gp, from, a.vocab, g);
         }
     }
@@ -297,8 +298,8 @@ extern "C" int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t o
     if (!weights) return bad(who, "no weights");
     if (!out_ml2p || !out_grad || (entropy_weights && !out_entropy)) return bad(who, "no output");
     if ((uintptr_t)out_grad % (dtype == MC_LOGITS_F32 ? 4 : 2)) return bad(who, "a gradient that is not aligned to its type");
-    GradOut out{View{(const char *)weights, weight_outer_stride * 4, weight_inner_stride * 4},
-                View{(const char *)entropy_weights, entropy_outer_stride * 4, entropy_inner_stride * 4},
+    GradOut out{view_of(weights, weight_outer_stride, weight_inner_stride, 4),
+                view_of(entropy_weights, entropy_outer_stride, entropy_inner_stride, 4),
                 (float)(1.0 / temperature), out_ml2p, out_entropy, (char *)out_grad};
     Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
     if (sp.shift) {

@@ -47,7 +47,7 @@ __device__ __forceinline__ void put_top(const ScoreOut &out, u32 row, u32 rank, 
 template <int DT, int G, int NV>
 __device__ __forceinline__ void top_by_turns(SubRow<DT, NV> &r, const Stat &st, const ScoreOut &out, u32 row, bool writes, float c) {
     const u32 lane = threadIdx.x & (G - 1);
-    const float lz = log2f(st.s);
+    const float lz = log2_(st.s);
     float last = INFINITY;
     u32 last_i = 0xFFFFFFFFu;
     for (u32 k = 0; k < out.k; ++k) {
@@ -147,7 +147,7 @@ __device__ __forceinline__ void sub_top(SubRow<DT, NV> &r, const Rows &a, const 
     }
     __syncthreads();
     if (fits && writes) {
-        const float lz = log2f(st.s);
+        const float lz = log2_(st.s);
         for (u32 i = lane; i < n; i += G) {
             const u64 key = cand[i];
             u32 rank = 0;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void put_row(const ScoreOut &out, u32 row, int tok, f
     }
     if (!out.k) return;
     if (!(st.s > 0.f)) n = 0;
-    const float lz = log2f(st.s);
+    const float lz = log2_(st.s);
     for (u32 i = threadIdx.x; i < n; i += T) {
         const u64 key = cand[i];
         u32 rank = 0;
