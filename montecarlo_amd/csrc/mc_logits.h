@@ -325,6 +325,19 @@ __device__ __forceinline__ A group_scan(A x) {
     return x;
 }
 
+template <int G>
+__device__ __forceinline__ float group_scan(float x) {
+    const u32 lane = threadIdx.x & (G - 1);
+    float o;
+    if constexpr (G >= 2) o = dpp<0x111>(x), x += lane >= 1 ? o : 0.f;  // rows shifted by 1, 2, 4, 8
+    if constexpr (G >= 4) o = dpp<0x112>(x), x += lane >= 2 ? o : 0.f;
+    if constexpr (G >= 8) o = dpp<0x114>(x), x += lane >= 4 ? o : 0.f;
+    if constexpr (G >= 16) o = dpp<0x118>(x), x += lane >= 8 ? o : 0.f;
+    if constexpr (G >= 32) o = __shfl(x, 15, 32), x += (lane & 31) >= 16 ? o : 0.f;  // (rows do not see each other: the sum of
+    if constexpr (G >= 64) o = __shfl(x, 31, 64), x += lane >= 32 ? o : 0.f;         // all before)
+    return x;
+}
+
 // the lanes of a group joined: the common maximum, the sums scaled to it
 template <int G, bool ENT>
 __device__ __forceinline__ Stat group_stat(Stat st, float c) {

@@ -172,6 +172,53 @@ __device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weigh
     return __shfl((int)ok, who, G) || margin == 0.;
 }
 
+// The same in 32 bits, for the lane that holds the token: true there, and only there, when u Z is at least `margin` Z from both
+// ends of the token's interval (nowhere otherwise).  Running sums ascend, so that a token's place is the number of them at or
+// below the target, and the nearest of them says how near an end is.
+template <int DT, int G, int NV>
+__device__ __forceinline__ bool draw_fast(const SubRow<DT, NV> &r, const Expo &y_of, double u, double margin, u32 &token, float &x, float &z) {
+    constexpr int N = SubRow<DT, NV>::N;
+    float s[N], upto[N], mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        s[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) s[i] += exp2_(y_of.fast(unpack<DT>(vec_of(r, i), j)));
+        upto[i] = group_all<G>(s[i], Add());
+        if (i) upto[i] += upto[i - 1];
+    }
+    z = upto[N - 1];
+    const float target = (float)(u * (double)z), near = (float)margin * z;
+    float before = 0.f;
+    raw4 q = vec_of(r, 0);
+    u32 from = from_of<DT, G>(r, 0);
+    mine = s[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        const bool past = upto[i - 1] <= target;
+        before = past ? upto[i - 1] : before;
+        mine = past ? s[i] : mine;
+        from = past ? from_of<DT, G>(r, i) : from;
+        choose(q, vec_of(r, i), past);
+    }
+    const float t = target - (before + (group_scan<G>(mine) - mine));
+    float run = 0.f, off = t;
+    u32 place = 0;
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) {
+        run += exp2_(y_of.fast(unpack<DT>(q, j)));
+        place += run <= t;
+        off = fminf(off, fabsf(run - t));
+    }
+    token = from + place;
+    u32 word = q[0];
+    constexpr u32 PER = VEC<DT> / 4;
+#pragma unroll
+    for (u32 w = 1; w < 4; ++w) word = place >= w * PER ? q[w] : word;
+    x = PER == 1 ? to_float<DT>(word, 0) : to_float<DT>(place & 1 ? word >> 16 : word & 0xFFFFu, 0);
+    return off >= near && place < (u32)VEC<DT>;
+}
+
 template <int DT, int G, int NV>
 __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows a, DrawArgs d) {
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
@@ -182,35 +229,38 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
     const double u = there ? uniform_of(d, row) : 0.;
     Stat st{sub_max<DT, G>(r), 0.f, 0.f, false};
     if (NV > 4) forget(r);
+    const Expo y_of(st, a.c);
+    const float m = st.m;
     u32 token;
     float x;
-    bool sure = draw_sub<DT, G>(r, Fast{Expo(st, a.c)}, u, d.margin, token, x, st.s) && !doubtful(st.m, a.c);
-    float ml2p = ml2p_of(0, st, x, a.c);
-    if (!drawable(st.m)) sure = true, token = (u32)MC_TOKEN_OUTSIDE, ml2p = no_draw(st.m);
-    if (!live) sure = true, token = (u32)MC_TOKEN_SKIP, ml2p = 0.f;
-    if (__ballot(!sure)) {  // the whole wave decides again, in 64 bits
-        forget(r);
-        const double m = (double)st.m;
-        u32 again;
-        double z;
-        bool now = draw_sub<DT, G>(r, PowerBelow{d.power.c, m}, u, MARGIN, again, x, z);
-        if (!sure) {
-            token = again;
-            ml2p = ml2p_under(z, ((double)x - m) * d.power.c);
+    if (drawable(m) && live) {  // (a group's lanes agree)
+        const bool mine = draw_fast<DT, G>(r, y_of, u, d.margin, token, x, st.s) && !doubtful(m, a.c);
+        if (mine) {
+            d.token[row] = (int)token;
+            d.ml2p[row] = log2_(st.s) - y_of.fast(x);
         }
-        now = now || sure;
-        if (__ballot(!now)) {  // and again, by the definition
-            forget(r);
-            draw_sub<DT, G>(r, Definition{d.t, m}, u, 0., again, x, z);
-            if (!now) {
-                token = again;
-                ml2p = ml2p_under(z, ((double)x - m) * d.power.c);
-            }
-        }
+        st.exact = group_sum<G>(mine) == 0;  // still open
+    } else if (there && lane == 0) {
+        d.token[row] = live ? MC_TOKEN_OUTSIDE : MC_TOKEN_SKIP;
+        d.ml2p[row] = live ? no_draw(m) : 0.f;
     }
-    if (there && lane == 0) {
-        d.token[row] = (int)token;
-        d.ml2p[row] = ml2p;
+    const bool open = st.exact;
+    if (__ballot(open)) {  // the whole wave decides again, in 64 bits
+        forget(r);
+        double z;
+        bool now = draw_sub<DT, G>(r, PowerBelow{d.power.c, (double)m}, u, MARGIN, token, x, z);
+        if (__ballot(open && !now)) {  // and again, by the definition
+            forget(r);
+            u32 again;
+            float x_again;
+            double z_again;
+            draw_sub<DT, G>(r, Definition{d.t, (double)m}, u, 0., again, x_again, z_again);
+            if (!now) token = again, x = x_again, z = z_again;
+        }
+        if (open && lane == 0) {
+            d.token[row] = (int)token;
+            d.ml2p[row] = ml2p_under(z, ((double)x - (double)m) * d.power.c);
+        }
     }
 }
 
@@ -552,11 +602,11 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 
 // How far off running sums of Fast may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
 // exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions in a vector, those
-// over a lane's vectors, each chunk's scaling, 6 additions over lanes, and 16 where parts are joined; twice, since u Z is such
-// a sum too.
+// over a lane's vectors, each chunk's scaling, 6 additions over lanes, and 18 where parts are joined and the target rounded;
+// twice, since u Z is such a sum too.
 double margin_of(const Rows &a) {
     const double vecs = a.nvec <= SUB_VECS ? 8 : (double)(a.nvec / WIDE + 1), chunks = a.nvec <= SUB_VECS ? 0 : vecs / UNROLL + 1;
-    return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)a.vocab) + 8 + vecs + 4 * chunks + 6 + 16);
+    return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)a.vocab) + 8 + vecs + 4 * chunks + 6 + 18);
 }
 
 // ---- keys ----------------------------------------------------------------------------------------------------------
