@@ -33,7 +33,6 @@ __device__ __forceinline__ double power_of(double n_word, double f) {
 // 2^(x c) for x c in [-1000, 900]; lower ones as 2^-1000: so far below any sum that `good` lets pass that it changes
 // nothing.
 struct Power {
-    typedef double Sum;
     double c;
     float lo;
     __device__ __forceinline__ double operator()(float x) const {
@@ -44,7 +43,6 @@ struct Power {
 
 // 2^((x - m) c): for rows whose logits are too far from 0 for Power
 struct PowerBelow {
-    typedef double Sum;
     double c, m;
     __device__ __forceinline__ double operator()(float x) const {
         const double y = fmax(((double)x - m) * c, -1000.), t = y + 0x1.8p52;
@@ -53,16 +51,8 @@ struct PowerBelow {
 };
 constexpr double MARGIN = 1e-10;
 
-// weights in 32 bits under the row's largest logit
-struct Fast {
-    typedef float Sum;
-    Expo y_of;
-    __device__ __forceinline__ float operator()(float x) const { return exp2_(y_of.fast(x)); }
-};
-
 // The draw's own weights: exp((x - m) / T) in 64 bits, m the row's largest logit.
 struct Definition {
-    typedef double Sum;
     double t, m;
     __device__ __forceinline__ double operator()(float x) const { return exp(((double)x - m) / t); }
 };
@@ -85,7 +75,7 @@ struct DrawArgs {
     const double *uniforms;  // or null: Philox
     u64 seed, first_id;
     u32 draw;
-    double t, margin;        // margin: how far off the running sums of Fast may be, as a share of Z
+    double t, margin;        // margin: how far off the running sums in 32 bits may be, as a share of Z
     Power power;
     const unsigned char *live;
     int *token;
@@ -108,29 +98,28 @@ __device__ __forceinline__ double uniform_of(const DrawArgs &d, u32 row) {
 // The token of a group's row in registers: running sums in the order of the index, vector step by vector step.  False when
 // u Z lies within `margin` Z of an end of the token's interval (0 takes any answer).
 template <int DT, int G, typename W, int NV>
-__device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weight, double u, double margin, u32 &token, float &x, typename W::Sum &z) {
-    typedef typename W::Sum Sum;
+__device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weight, double u, double margin, u32 &token, float &x, double &z) {
     constexpr int N = SubRow<DT, NV>::N;
-    Sum s[N];
-    z = 0;
+    double s[N];
+    z = 0.;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s[i] = 0;
+        s[i] = 0.;
 #pragma unroll
         for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(vec_of(r, i), j));
         z += s[i];
     }
     z = group_all<G>(z, Add());
-    const double target = u * (double)z, near = margin * (double)z;
+    const double target = u * z, near = margin * z;
     // the vector step whose running sum passes the target, or the last one with any weight
     double before = 0., run = 0.;
-    Sum mine = 0;
+    double mine = 0.;
     raw4 q = vec_of(r, 0);
     u32 from = from_of<DT, G>(r, 0);
     bool found = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const double step = (double)group_all<G>(s[i], Add());
+        const double step = group_all<G>(s[i], Add());
         const bool here = !found && step > 0.;
         before = here ? run : before;
         mine = here ? s[i] : mine;
@@ -139,23 +128,23 @@ __device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weigh
         found = found || (here && run + step > target);
         run += step;
     }
-    const Sum inc = group_scan<G>(mine);
+    const double inc = group_scan<G>(mine);
     const u32 shift = threadIdx.x & 63 & ~(G - 1);
     const u64 all = G == 64 ? ~0ull : (1ull << (G & 63)) - 1;
-    const u64 passes = (__ballot(before + (double)inc > target) >> shift) & all, some = (__ballot(mine > 0) >> shift) & all;
+    const u64 passes = (__ballot(before + inc > target) >> shift) & all, some = (__ballot(mine > 0.) >> shift) & all;
     // (a sum that passes by a rounding only, or none: the last lane with any weight)
     const bool hit = found && passes;
     const u32 who = hit ? (u32)__ffsll((unsigned long long)passes) - 1 : some ? 63u - (u32)__clzll((long long)some) : 0u;
-    double at_lo = before + (double)(inc - mine);
+    double at_lo = before + (inc - mine);
     u32 got = 0xFFFFFFFFu, last = 0;
     float got_x = 0.f, last_x = 0.f;
     bool ok = false;
 #pragma unroll
     for (int j = 0; j < VEC<DT>; ++j) {
         const float e = unpack<DT>(q, j);
-        const Sum w = weight(e);
-        const double next = at_lo + (double)w;
-        if (w > 0) {
+        const double w = weight(e);
+        const double next = at_lo + w;
+        if (w > 0.) {
             last = from + j;
             last_x = e;
             if (got == 0xFFFFFFFFu && next > target) {
@@ -172,9 +161,29 @@ __device__ __forceinline__ bool draw_sub(const SubRow<DT, NV> &r, const W &weigh
     return __shfl((int)ok, who, G) || margin == 0.;
 }
 
+// The token in a vector of which u Z lies `t` behind the beginning: running sums ascend, so that its place is the number of
+// them at or below t, and the nearest of them says how near an end is.  True if the token is here and none is nearer than `near`.
+template <int DT>
+__device__ __forceinline__ bool place_of(const raw4 &q, const Expo &y_of, float t, float near, u32 from, u32 &token, float &x) {
+    float run = 0.f, off = t;
+    u32 place = 0;
+#pragma unroll
+    for (int j = 0; j < VEC<DT>; ++j) {
+        run += exp2_(y_of.fast(unpack<DT>(q, j)));
+        place += run <= t;
+        off = fminf(off, fabsf(run - t));
+    }
+    token = from + place;
+    u32 word = q[0];
+    constexpr u32 PER = VEC<DT> / 4;
+#pragma unroll
+    for (u32 w = 1; w < 4; ++w) word = place >= w * PER ? q[w] : word;
+    x = PER == 1 ? to_float<DT>(word, 0) : to_float<DT>(place & 1 ? word >> 16 : word & 0xFFFFu, 0);
+    return off >= near && place < (u32)VEC<DT>;
+}
+
 // The same in 32 bits, for the lane that holds the token: true there, and only there, when u Z is at least `margin` Z from both
-// ends of the token's interval (nowhere otherwise).  Running sums ascend, so that a token's place is the number of them at or
-// below the target, and the nearest of them says how near an end is.
+// ends of the token's interval (nowhere otherwise).
 template <int DT, int G, int NV>
 __device__ __forceinline__ bool draw_fast(const SubRow<DT, NV> &r, const Expo &y_of, double u, double margin, u32 &token, float &x, float &z) {
     constexpr int N = SubRow<DT, NV>::N;
@@ -201,22 +210,7 @@ __device__ __forceinline__ bool draw_fast(const SubRow<DT, NV> &r, const Expo &y
         from = past ? from_of<DT, G>(r, i) : from;
         choose(q, vec_of(r, i), past);
     }
-    const float t = target - (before + (group_scan<G>(mine) - mine));
-    float run = 0.f, off = t;
-    u32 place = 0;
-#pragma unroll
-    for (int j = 0; j < VEC<DT>; ++j) {
-        run += exp2_(y_of.fast(unpack<DT>(q, j)));
-        place += run <= t;
-        off = fminf(off, fabsf(run - t));
-    }
-    token = from + place;
-    u32 word = q[0];
-    constexpr u32 PER = VEC<DT> / 4;
-#pragma unroll
-    for (u32 w = 1; w < 4; ++w) word = place >= w * PER ? q[w] : word;
-    x = PER == 1 ? to_float<DT>(word, 0) : to_float<DT>(place & 1 ? word >> 16 : word & 0xFFFFu, 0);
-    return off >= near && place < (u32)VEC<DT>;
+    return place_of<DT>(q, y_of, target - (before + (group_scan<G>(mine) - mine)), near, from, token, x);
 }
 
 template <int DT, int G, int NV>
@@ -295,15 +289,63 @@ __device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const
     return z;
 }
 
-// The token among vectors v0 .. v1, whose running sums begin at `before`, by one wave: the sums of rounds of STEPS steps of
-// 64 vectors.  False when the target lies within `margin` of an end of the token's interval.
-template <int DT, typename W>
-__device__ __forceinline__ bool locate(const Span &r, const W &weight, u32 v0, u32 v1, double before, double target, double margin,
-                                       u32 &token, float &x) {
-    typedef typename W::Sum Sum;
+// The token among vectors v0 .. v1, whose running sums in 32 bits begin at `before`, by one wave in rounds of STEPS steps of 64
+// vectors: true in the lane that holds it, and only there, when no end of its interval is nearer than `near`.
+template <int DT>
+__device__ __forceinline__ bool locate_fast(const Span &r, const Expo &y_of, u32 v0, u32 v1, float before, float target, float near, u32 &token,
+                                            float &x) {
     const u32 lane = threadIdx.x & 63;
     if (v0 == 0 && r.head) {
-        const double next = before + (double)weight(r.first);
+        const float next = before + exp2_(y_of.fast(r.first));
+        if (next > target) {
+            token = 0;
+            x = r.first;
+            return lane == 0 && next - target >= near;
+        }
+        if (target - next < near) return false;
+        before = next;
+    }
+#pragma unroll 1
+    for (u32 base = v0; base < v1; base += 64 * STEPS) {
+        raw4 q[STEPS];
+        float s[STEPS], upto[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(r, base + i * 64 + lane, v1);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            s[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) s[i] += exp2_(y_of.fast(unpack<DT>(q[i], j)));
+            upto[i] = (i ? upto[i ? i - 1 : 0] : before) + group_all<64>(s[i], Add());
+        }
+        if (upto[STEPS - 1] > target) {
+            raw4 mq = q[0];
+            float mine = s[0];
+            u32 step = 0;
+#pragma unroll
+            for (int i = 1; i < STEPS; ++i) {
+                const bool past = upto[i - 1] <= target;
+                before = past ? upto[i - 1] : before;
+                mine = past ? s[i] : mine;
+                step += past;
+                choose(mq, q[i], past);
+            }
+            const float t = target - (before + (group_scan<64>(mine) - mine));
+            return place_of<DT>(mq, y_of, t, near, r.head + (base + step * 64 + lane) * VEC<DT>, token, x);
+        }
+        before = upto[STEPS - 1];
+    }
+    return false;
+}
+
+// The token among vectors v0 .. v1, whose running sums begin at `before`, by one wave: the sums of rounds of STEPS steps of
+// 64 vectors.  False when the target lies within `margin` of an end of the token's interval.
+template <int DT>
+__device__ __forceinline__ bool locate(const Span &r, const PowerBelow &weight, u32 v0, u32 v1, double before, double target, double margin,
+                                       u32 &token, float &x) {
+    const u32 lane = threadIdx.x & 63;
+    if (v0 == 0 && r.head) {
+        const double next = before + weight(r.first);
         if (next > target) {
             token = 0;
             x = r.first;
@@ -315,20 +357,20 @@ __device__ __forceinline__ bool locate(const Span &r, const W &weight, u32 v0, u
 #pragma unroll 1
     for (u32 base = v0; base < v1; base += 64 * STEPS) {
         raw4 q[STEPS];
-        Sum s[STEPS];
+        double s[STEPS];
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(r, base + i * 64 + lane, v1);
         raw4 mq = q[0];
-        Sum ms = 0;
+        double ms = 0.;
         double start = before, run = before;
         u32 step = 0;
         bool found = false;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            s[i] = 0;
+            s[i] = 0.;
 #pragma unroll
             for (int j = 0; j < VEC<DT>; ++j) s[i] += weight(unpack<DT>(q[i], j));
-            const double all = (double)group_all<64>(s[i], Add());
+            const double all = group_all<64>(s[i], Add());
             const bool here = !found && run + all > target;
             choose(mq, q[i], here);
             ms = here ? s[i] : ms;
@@ -338,17 +380,17 @@ __device__ __forceinline__ bool locate(const Span &r, const W &weight, u32 v0, u
             run += all;
         }
         if (found) {
-            const Sum minc = group_scan<64>(ms);
-            const u64 over = __ballot(start + (double)minc > target);
+            const double minc = group_scan<64>(ms);
+            const u64 over = __ballot(start + minc > target);
             const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u;
-            double at_lo = start + (double)(minc - ms);
+            double at_lo = start + (minc - ms);
             u32 got = 0;
             float got_x = 0.f;
             bool sure = false;
 #pragma unroll
             for (int j = 0; j < VEC<DT>; ++j) {
                 const float e = unpack<DT>(mq, j);
-                const double next = at_lo + (double)weight(e);
+                const double next = at_lo + weight(e);
                 if (!sure && target - at_lo >= margin && next - target >= margin) {
                     sure = true;
                     got = r.head + (base + step * 64 + lane) * VEC<DT> + j;
@@ -500,11 +542,9 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
     }
     if (threadIdx.x == 0) done = 0;
     __syncthreads();
-    // lane i holds wave i's sums, under its own largest logit
-    Stat mine{-INFINITY, 0.f, 0.f, false};
-    if (lane < WIDE_WAVES) mine.m = pm[lane], mine.s = pf[lane];
-    st.m = group_all<64>(mine.m, Max());
-    const float m = st.m;
+    // eight lanes hold the eight waves' sums, each under its own largest logit
+    const u32 of = lane & (WIDE_WAVES - 1);
+    const float m = group_all<WIDE_WAVES>(pm[of], Max());
     if (!drawable(m)) {
         if (threadIdx.x == 0) {
             d.token[row] = MC_TOKEN_OUTSIDE;
@@ -513,17 +553,16 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
         return;
     }
     if (!BEGIN64 && !doubtful(m, a.c)) {
-        const Fast weight{Expo(st, a.c)};
-        const double w = (double)(mine.s * exp2_(scaled(mine.m, a.c) - weight.y_of.M)), inc = group_scan<64>(w);
-        const double z = __shfl(inc, 63), target = u * z;
-        const u64 passes = __ballot(inc > target);
-        const u32 part = passes ? (u32)__ffsll((unsigned long long)passes) - 1 : WIDE_WAVES;
+        const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
+        const float w = pf[of] * exp2_(scaled(pm[of], a.c) - y_of.M), inc = group_scan<WIDE_WAVES>(w), z = __shfl(inc, WIDE_WAVES - 1);
+        const float target = (float)(u * (double)z);
+        const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WIDE_WAVES) - 1));
         if (wave == part) {
-            u32 token = 0;
-            float x = 0.f;
-            if (locate<DT>(r, weight, v0, v1, __shfl(inc - w, part), target, d.margin * z, token, x) && lane == 0) {
+            u32 token;
+            float x;
+            if (locate_fast<DT>(r, y_of, v0, v1, __shfl(inc - w, part), target, (float)d.margin * z, token, x)) {
                 d.token[row] = (int)token;
-                d.ml2p[row] = ml2p_under(z, (double)weight.y_of.fast(x));
+                d.ml2p[row] = log2_(z) - y_of.fast(x);
                 done = 1;
             }
         }
@@ -600,7 +639,7 @@ u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
 
 size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * (8 * PART_WAVES + 4) : 0; }
 
-// How far off running sums of Fast may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
+// How far off running sums in 32 bits may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
 // exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions in a vector, those
 // over a lane's vectors, each chunk's scaling, 6 additions over lanes, and 18 where parts are joined and the target rounded;
 // twice, since u Z is such a sum too.
