@@ -1,11 +1,11 @@
 // What the kernels on logits share (device code; mc_logits_score.hip says what they compute).
 //
-// With c = log2(e) / T a token's exponent is y = x c - M, where M = m c is the largest logit's: one multiply-add, one power
-// and the sums an element.  M may be off by a rounding; every use of it subtracts the same number, so that cancels.  That
-// holds while |M| <= 2^15 (the largest weight is then 2^(2^-9) at most).  Parts of a row whose own maximum lies lower take
-// -2^15 for it; a ROW whose M is beyond is summed again with y = (x - m) c (`exact`): a row of the type's lowest value,
-// temperatures near 0.  m says the rest: it is -inf where nothing is left (s is 0 then), NaN where the row holds a NaN and
-// +inf where it holds one (s is NaN then).
+// With c = log2(e) / T a token's exponent is y = x c - M, where M is the largest logit's m c rounded up to a whole number:
+// one multiply-add, one power and the sums an element, and sums under different M are brought together without a rounding.
+// (m c itself may be off by a rounding; every use subtracts the same M, so that cancels.)  That holds while |M| <= 2^15.
+// Parts of a row whose own maximum lies lower take -2^15 for it; a ROW whose M is beyond is summed again with
+// y = (x - m) c (`exact`): a row of the type's lowest value, temperatures near 0.  m says the rest: it is -inf where nothing
+// is left (s is 0 then), NaN where the row holds a NaN and +inf where it holds one (s is NaN then).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -221,7 +221,10 @@ struct Stat {
     bool exact;
 };
 
-__device__ __forceinline__ float scaled(float m, float c) { return fmaxf(m * c, -FAR); }
+__device__ __forceinline__ float scaled(float m, float c) { return ceilf(fmaxf(m * c, -FAR)); }
+
+// s 2^d for a whole number d
+__device__ __forceinline__ float times2(float s, float d) { return __builtin_amdgcn_ldexpf(s, (int)d); }
 
 // the exponent of a logit under a row's statistics
 struct Expo {
@@ -343,9 +346,9 @@ template <int G, bool ENT>
 __device__ __forceinline__ Stat group_stat(Stat st, float c) {
     const float mine = scaled(st.m, c);
     st.m = group_all<G>(st.m, Max());
-    const float d = mine - scaled(st.m, c), f = exp2_(d);
-    if (ENT) st.e = group_all<G>(__builtin_fmaf(d, st.s, st.e) * f, Add());
-    st.s = group_all<G>(st.s * f, Add());
+    const float d = mine - scaled(st.m, c);
+    if (ENT) st.e = group_all<G>(times2(__builtin_fmaf(d, st.s, st.e), d), Add());
+    st.s = group_all<G>(times2(st.s, d), Add());
     return st;
 }
 
@@ -420,6 +423,12 @@ __device__ __forceinline__ u32 block_min(u32 v) {
 #pragma unroll
     for (int w = 0; w < T / 64; ++w) v = min(v, part[w]);
     return v;
+}
+
+template <int N>
+__device__ __forceinline__ float pairs(const float *w) {
+    if constexpr (N == 1) return w[0];
+    else return pairs<N / 2>(w) + pairs<N / 2>(w + N / 2);
 }
 
 // ---- rows of few tokens: a group of G lanes a row, several rows a wave, the row in registers ---------------------------------
@@ -552,21 +561,22 @@ __device__ __forceinline__ float take(Stat &st, const raw4 (&q)[UNROLL], float c
         for (int j = 0; j < N; ++j) m = maximum(m, unpack<DT>(q[u], j));
     const float old = scaled(st.m, c);
     st.m = maximum(st.m, m);
-    const float M = scaled(st.m, c), d = old - M, f = exp2_(d);
-    if (ENT) st.e = __builtin_fmaf(d, st.s, st.e) * f;
-    st.s *= f;
+    const float M = scaled(st.m, c), d = old - M;
+    if (ENT) st.e = times2(__builtin_fmaf(d, st.s, st.e), d);
+    float s[UNROLL];  // (in pairs, so that few additions follow each other)
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-        float s = 0.f, e = 0.f;  // (a vector's own, so that fewer additions follow each other)
+        float w[N], e = 0.f;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float y = __builtin_fmaf(unpack<DT>(q[u], j), c, -M), w = exp2_(y);
-            s += w;
-            if (ENT) e = __builtin_fmaf(w, fmaxf(y, -FAR), e);
+            const float y = __builtin_fmaf(unpack<DT>(q[u], j), c, -M);
+            w[j] = exp2_(y);
+            if (ENT) e = __builtin_fmaf(w[j], fmaxf(y, -FAR), e);
         }
-        st.s += s;
+        s[u] = pairs<N>(w);
         if (ENT) st.e += e;
     }
+    st.s = times2(st.s, d) + pairs<UNROLL>(s);
     return m;
 }
 
@@ -587,9 +597,9 @@ template <bool ENT>
 __device__ __forceinline__ void take_one(Stat &st, float x, float c) {
     const float old = scaled(st.m, c);
     st.m = maximum(st.m, x);
-    const float M = scaled(st.m, c), d = old - M, f = exp2_(d), y = __builtin_fmaf(x, c, -M), w = exp2_(y);
-    if (ENT) st.e = __builtin_fmaf(d, st.s, st.e) * f + w * fmaxf(y, -FAR);
-    st.s = st.s * f + w;
+    const float M = scaled(st.m, c), d = old - M, y = __builtin_fmaf(x, c, -M), w = exp2_(y);
+    if (ENT) st.e = times2(__builtin_fmaf(d, st.s, st.e), d) + w * fmaxf(y, -FAR);
+    st.s = times2(st.s, d) + w;
 }
 
 // A doubtful row's statistics (every thread of the workgroup calls): m is its largest logit.

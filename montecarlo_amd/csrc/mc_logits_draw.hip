@@ -190,9 +190,10 @@ __device__ __forceinline__ bool draw_fast(const SubRow<DT, NV> &r, const Expo &y
     float s[N], upto[N], mine = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s[i] = 0.f;
+        float w[VEC<DT>];
 #pragma unroll
-        for (int j = 0; j < VEC<DT>; ++j) s[i] += exp2_(y_of.fast(unpack<DT>(vec_of(r, i), j)));
+        for (int j = 0; j < VEC<DT>; ++j) w[j] = exp2_(y_of.fast(unpack<DT>(vec_of(r, i), j)));
+        s[i] = pairs<VEC<DT>>(w);
         upto[i] = group_all<G>(s[i], Add());
         if (i) upto[i] += upto[i - 1];
     }
@@ -313,9 +314,10 @@ __device__ __forceinline__ bool locate_fast(const Span &r, const Expo &y_of, u32
         for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(r, base + i * 64 + lane, v1);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            s[i] = 0.f;
+            float w[VEC<DT>];
 #pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) s[i] += exp2_(y_of.fast(unpack<DT>(q[i], j)));
+            for (int j = 0; j < VEC<DT>; ++j) w[j] = exp2_(y_of.fast(unpack<DT>(q[i], j)));
+            s[i] = pairs<VEC<DT>>(w);
             upto[i] = (i ? upto[i ? i - 1 : 0] : before) + group_all<64>(s[i], Add());
         }
         if (upto[STEPS - 1] > target) {
@@ -554,7 +556,7 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
     }
     if (!BEGIN64 && !doubtful(m, a.c)) {
         const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
-        const float w = pf[of] * exp2_(scaled(pm[of], a.c) - y_of.M), inc = group_scan<WIDE_WAVES>(w), z = __shfl(inc, WIDE_WAVES - 1);
+        const float w = times2(pf[of], scaled(pm[of], a.c) - y_of.M), inc = group_scan<WIDE_WAVES>(w), z = __shfl(inc, WIDE_WAVES - 1);
         const float target = (float)(u * (double)z);
         const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WIDE_WAVES) - 1));
         if (wave == part) {
@@ -639,13 +641,14 @@ u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
 
 size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift) * (8 * PART_WAVES + 4) : 0; }
 
-// How far off running sums in 32 bits may be, as a share of Z, in half steps of 32 bits: the weights (2 for the power; the
-// exponent's roundings, 1.4 times the exponent of each weight, in the sum at most log2 V), 8 additions in a vector, those
-// over a lane's vectors, each chunk's scaling, 6 additions over lanes, and 18 where parts are joined and the target rounded;
-// twice, since u Z is such a sum too.
+// How near u Z may come to an end of a token's interval, as a share of Z, before sums in 32 bits leave the token open, in half
+// steps.  The weights: 2 for the power, 1.4 times its exponent for the exponent's two roundings, which the weights' mean
+// makes at most log2 V + 1 (they weigh once: what is off in the running sum is off in Z too).  Of the additions behind each
+// other, in Z: 3 in a vector and 2 in a chunk (in pairs), a lane's chunks or vectors, 6 over lanes, 3 over waves; in the running
+// sum as many and 8 in the last vector; 3 where its parts are joined, 2 for the target.
 double margin_of(const Rows &a) {
-    const double vecs = a.nvec <= SUB_VECS ? 8 : (double)(a.nvec / WIDE + 1), chunks = a.nvec <= SUB_VECS ? 0 : vecs / UNROLL + 1;
-    return 0x1p-24 * 2. * (2 + 1.4 * std::log2((double)a.vocab) + 8 + vecs + 4 * chunks + 6 + 18);
+    const double adds = a.nvec <= SUB_VECS ? 3 + 8 + 6 : 3 + 2 + (a.nvec / (WIDE * UNROLL) + 1) + 6 + 3;
+    return 0x1p-24 * (2 + 1.4 * (std::log2((double)a.vocab) + 1) + 2 * adds + 8 + 5);
 }
 
 // ---- keys ----------------------------------------------------------------------------------------------------------
