@@ -141,6 +141,50 @@ def test_score_takes_any_strides():
         check_score(x.contiguous(), t.contiguous(), r, 1.0, 4)
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 1e-5, 0.01, 300.0, 1e30])
+@pytest.mark.parametrize("vocab", [33, 700, 9001])
+def test_temperatures_far_from_one(vocab, temperature):
+    x = make(25, vocab, torch.float32, vocab + 9)
+    toks = tokens_for(x, 2)
+    g = torch.Generator().manual_seed(vocab)
+    u, w, v = torch.rand(25, generator=g, dtype=torch.float64), torch.rand(25, generator=g), torch.rand(25, generator=g)
+    check_score(x, toks, lg.logits_score(x.cuda(), toks.cuda(), temperature=temperature, entropy=True, top=3), temperature, 3)
+    check_draw(x, u, None, lg.logits_draw(x.cuda(), u.cuda(), temperature=temperature), temperature)
+    check_gradient(x, toks, w, v, lg.logits_gradient(x.cuda(), toks.cuda(), w.cuda(), entropy_weights=v.cuda(), temperature=temperature),
+                   temperature, "fp32")
+
+
+@pytest.mark.parametrize("vocab,rows,dtype,top", [(97, 20000, "bf16", 64), (200, 40000, "fp32", 33), (4096, 900, "fp16", 64), (3001, 3000, "bf16", 64),
+                                                  (262144, 1100, "fp32", 64)])
+def test_many_alternatives_of_many_rows(vocab, rows, dtype, top):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g, device="cuda").mul_(2.5).to(DTYPES[dtype])
+    some = list(range(26)) + [rows // 2, rows - 1]
+    x[:26] = make(26, vocab, DTYPES[dtype], vocab).cuda()
+    toks = torch.zeros(rows, dtype=torch.int64)
+    r = lg.logits_score(x, toks.cuda(), entropy=True, top=top)
+    check_score(x[some].cpu(), toks[some], lg.LogitScores(*(t[some] for t in r)), 1.0, top)
+
+
+def test_more_rows_than_a_grid_is_wide():
+    rows = (1 << 26) + 77                                   # 64 of them a workgroup, 2^20 workgroups a line of the grid
+    x = torch.zeros(rows, 3, dtype=torch.bfloat16, device="cuda")
+    x[-40:] = make(40, 3, torch.bfloat16, 1).cuda()
+    toks = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    r = lg.logits_score(x, toks)
+    check_score(x[-40:].cpu(), toks[-40:].cpu(), lg.logits_score(x[-40:], toks[-40:], entropy=True), 1.0, 0)
+    assert torch.equal(r.ml2p[-40:].view(torch.int32), lg.logits_score(x[-40:], toks[-40:]).ml2p.view(torch.int32))
+    assert bool((r.ml2p[:-40] == r.ml2p[0]).all()) and abs(r.ml2p[0].item() - math.log2(3)) < 1e-6
+    del x, r
+    rows = (1 << 20) + 5                                    # one a workgroup
+    x = torch.zeros(rows, 2052, dtype=torch.float32, device="cuda")
+    x[-1, 7] = 20.0
+    d = lg.logits_draw(x, torch.full((rows,), 0.5, dtype=torch.float64, device="cuda"))
+    assert d.tokens[-1].item() == 7 and bool((d.tokens[:-1] == 1026).all())
+    s = lg.logits_score(x, torch.full((rows,), 7, device="cuda"), top=1)
+    assert s.top_tokens[-1].item() == 7 and bool((s.top_tokens[:-1] == 0).all())
+
+
 def test_rows_beyond_32_bits_of_offset():
     base = torch.empty(2_200_000_400, dtype=torch.bfloat16, device="cuda")
     x = base.as_strided((2, 2, 100), (2_200_000_100, 150, 1))

@@ -133,3 +133,39 @@ def test_the_plugin_form_is_abstract_and_checks_its_arguments():
     m = Model(["a", "b", "<end>"], 2, device="cpu")
     assert m.encode("abz") == [0, 1, OUTSIDE]
     assert m._sampled_strings(torch.tensor([[0, 1, 2, SKIP], [2, SKIP, SKIP, SKIP]])) == ["ab", ""]
+
+
+def test_the_multiplication_that_stands_for_a_division():
+    """make_div / at of csrc/mc_logits.h in whole numbers: exact for every row number below 2^31."""
+    rng = np.random.default_rng(1)
+    for d in [1, 2, 3, 5, 7, 16, 31, 97, 1000, 65535, 65536, 65537, (1 << 30) - 1, 1 << 30, (1 << 31) - 1] + rng.integers(1, 1 << 31, 300).tolist():
+        shift = 0
+        while (1 << shift) < d:
+            shift += 1
+        mul = ((1 << (31 + shift)) + d - 1) // d
+        assert mul < 1 << 32
+        rows = {0, 1, d - 1, d, d + 1, 2 * d - 1, (1 << 31) - 1, ((1 << 31) - 1) // d * d, ((1 << 31) - 1) // d * d - 1}
+        for r in list(rows) + rng.integers(0, 1 << 31, 20).tolist():
+            if 0 <= r < 1 << 31:
+                assert (((r << 1) * mul) >> 32) >> shift == r // d, (r, d)
+
+
+def test_the_polynomial_of_the_draw():
+    """2^f on [-1/2, 1/2] as csrc/mc_logits_draw.hip has it: off by less than 4.1e-11 of its value, with room to the margin."""
+    import os
+    import re
+    from decimal import Decimal, getcontext
+    getcontext().prec = 40
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "montecarlo_amd", "csrc", "mc_logits_draw.hip")).read()
+    body = src[src.index("double power_of("):src.index("return __hiloint2double")]
+    c = [Decimal(float.fromhex(h)) for h in re.findall(r"(0x1\.[0-9a-f]+p[+-]\d+)", body)]
+    assert len(c) == 8                                      # from the highest power down
+    worst = Decimal(0)
+    for i in range(-500, 501):
+        f = Decimal(i) / 1000
+        p = Decimal(0)
+        for k in c:
+            p = p * f + k
+        worst = max(worst, abs(p / (f * Decimal(2).ln()).exp() - 1))
+    margin = float(re.search(r"MARGIN = ([0-9e.-]+);", src).group(1))
+    assert worst < Decimal("4.1e-11") and margin >= 2 * float(worst)
