@@ -416,7 +416,8 @@ __global__ __launch_bounds__(T, 8) void k_logits_score(Rows a, ScoreOut out, Spl
     if constexpr (PART) {
         if (threadIdx.x == 0) sp.stats[id] = make_float4(st.m, st.s, st.e, 0.f);
         if constexpr (TOP) {
-            const u32 n = select<DT, T>(sh, cells, r, v0, v1, out.k, per_cell);
+            // (a part with a NaN or +inf needs none, and NaNs have no place in the order that the selection counts by)
+            const u32 n = fabsf(st.m) < INFINITY ? select<DT, T>(sh, cells, r, v0, v1, out.k, per_cell) : 0u;
             u64 *keys = sp.keys + ((u64)row * out.k << sp.shift) + part;
             for (u32 i = threadIdx.x; i < n; i += T) {
                 const u64 key = sh.cand[i];
@@ -464,25 +465,27 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
     u32 n = 0;
     const u64 *cand = nullptr;
     if constexpr (TOP) {
-        const u32 total = out.k << sp.shift;
-        const u64 *keys = sp.keys + (u64)row * total;
-        u32 lm = 0;
-        for (u32 i = threadIdx.x; i < total; i += T) lm = max(lm, (u32)(keys[i] >> 32));
-        if (threadIdx.x == 0) sh.n_cand = 0;
-        sh.most[threadIdx.x] = lm;
-        __syncthreads();
-        const u32 bound = bound_among<T>(sh.most, out.k);
-        for (u32 i = threadIdx.x; i < total; i += T) {
-            const u64 key = keys[i];
-            if (key && (u32)(key >> 32) >= bound) {
-                const u32 at = atomicAdd(&sh.n_cand, 1u);
-                if (at < CAND_CAP) sh.cand[at] = key;
-            }
-        }
-        __syncthreads();
-        n = sh.n_cand;
-        if (n > CAND_CAP) n = add_head<T>(sh, r, 0, select_by_bits<DT, T>(sh, r, 0, r.nvec, out.k, bound));
         cand = sh.cand;
+        if (st.s > 0.f) {
+            const u32 total = out.k << sp.shift;
+            const u64 *keys = sp.keys + (u64)row * total;
+            u32 lm = 0;
+            for (u32 i = threadIdx.x; i < total; i += T) lm = max(lm, (u32)(keys[i] >> 32));
+            if (threadIdx.x == 0) sh.n_cand = 0;
+            sh.most[threadIdx.x] = lm;
+            __syncthreads();
+            const u32 bound = bound_among<T>(sh.most, out.k);
+            for (u32 i = threadIdx.x; i < total; i += T) {
+                const u64 key = keys[i];
+                if (key && (u32)(key >> 32) >= bound) {
+                    const u32 at = atomicAdd(&sh.n_cand, 1u);
+                    if (at < CAND_CAP) sh.cand[at] = key;
+                }
+            }
+            __syncthreads();
+            n = sh.n_cand;
+            if (n > CAND_CAP) n = add_head<T>(sh, r, 0, select_by_bits<DT, T>(sh, r, 0, r.nvec, out.k, bound));
+        }
     }
     put_row<T>(out, row, tok, x, st, a.c, cand, n);
 }

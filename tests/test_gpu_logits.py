@@ -130,6 +130,20 @@ def test_top_in_orders_that_are_hard(kind, vocab, dtype):
         check_score(xs, toks[:rows], r, 1.0, 40)
 
 
+@pytest.mark.parametrize("bits", [0x7FFFFFFF, 0x7F800001, -1])
+@pytest.mark.parametrize("vocab,rows", [(200000, 3), (200000, 1030), (40000, 4), (4000, 9)])
+def test_alternatives_beside_nan_of_any_bits(vocab, rows, bits):
+    """Equal logits and, where one thread has them, more NaNs than alternatives: no row's selection may count these."""
+    x = torch.ones(rows, vocab, device="cuda")
+    for u in range(16):                                     # vectors that lie 256 lanes apart
+        x[0, u * 1024:u * 1024 + 4].view(torch.int32).fill_(bits) if u * 1024 + 4 <= vocab else None
+    x[1].view(torch.int32).fill_(bits)
+    x[2, vocab - 1:].view(torch.int32).fill_(bits)
+    toks = torch.arange(rows)
+    r = lg.logits_score(x, toks.cuda(), entropy=True, top=min(64, vocab))
+    check_score(x[:4].cpu(), toks[:4], lg.LogitScores(*(t[:4] for t in r)), 1.0, 64)
+
+
 def test_score_takes_any_strides():
     g = torch.Generator().manual_seed(3)
     base = torch.randn(6, 5, 40, generator=g).to(torch.float16).cuda()
@@ -540,6 +554,84 @@ def test_captured_and_replayed(rows, vocab):
         torch.cuda.synchronize()
         for p, q in zip(held, want):
             assert torch.equal(p.nan_to_num(nan=3.0), q.nan_to_num(nan=3.0))
+
+
+def test_captured_wide_rows_with_workspaces():
+    """Two graphs of calls that are cut into parts, replayed in turn with eager work between them."""
+    x = make(9, 200003, torch.float32, 3).cuda()
+    t = tokens_for(x.cpu(), 1).cuda()
+    w = torch.rand(9).cuda()
+    u = torch.rand(9, dtype=torch.float64).cuda()
+
+    def all_of():
+        return [*lg.logits_score(x, t, entropy=True, top=20), *lg.logits_gradient(x, t, w, entropy_weights=w), *lg.logits_draw(x, u)]
+
+    all_of()
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(all_of())
+    for seed in range(3):
+        x.copy_(make(9, 200003, torch.float32, 30 + seed))
+        u.uniform_(generator=None)
+        graphs[0].replay()
+        want = all_of()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for mine in held:
+            for p, q in zip(mine, want):
+                assert torch.equal(p.nan_to_num(nan=3.0), q.nan_to_num(nan=3.0))
+
+
+def test_two_streams_and_two_threads_at_once():
+    import threading
+    xs = [make(9, 200003, torch.bfloat16, 5 + i).cuda() for i in range(2)] + [make(3000, 97, torch.float16, 9).cuda()]
+    ts = [tokens_for(x.cpu(), 1).cuda() for x in xs]
+    us = [torch.rand(x.shape[0], dtype=torch.float64).cuda() for x in xs]
+    ws = [torch.rand(x.shape[0]).cuda() for x in xs]
+
+    def all_of(i):
+        return [*lg.logits_score(xs[i], ts[i], entropy=True, top=8), *lg.logits_gradient(xs[i], ts[i], ws[i], entropy_weights=ws[i]),
+                *lg.logits_draw(xs[i], us[i])]
+
+    want = [all_of(i) for i in range(3)]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in xs], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i].append(all_of(i))
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for i in range(3):
+        for run in got[i]:
+            for p, q in zip(run, want[i]):
+                assert torch.equal(p.nan_to_num(nan=3.0), q.nan_to_num(nan=3.0))
+
+
+def test_a_gradient_in_the_logits_place_is_noticed():
+    """What autograd saved of the logits is overwritten: its backward refuses, and works where the logits were not needed."""
+    a = torch.randn(4, 50, device="cuda", requires_grad=True)
+    t, w = torch.arange(4).cuda(), torch.ones(4).cuda()
+    x = a.tanh()
+    g = lg.logits_gradient(x, t, w, out=x.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        x.backward(g.grad)
+    x = a * 2.0
+    want = lg.logits_gradient(x, t, w).grad
+    x.backward(lg.logits_gradient(x, t, w, out=x.detach()).grad)
+    assert torch.equal(a.grad, want * 2.0)
 
 
 def test_refusals():
