@@ -146,8 +146,9 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
     eos, eis = _beside("entropy_weights", entropy_weights, dev, rows, _F32) if entropy_weights is not None else (0, 0)
     temperature = _temperature(temperature)
     if out is None:
-        out = logits.new_empty(logits.shape)
+        grad = logits.new_empty(logits.shape)
     else:
+        grad = out
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError("out: a contiguous tensor of the logits' shape, type and device is needed")
         lo, hi = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
@@ -164,8 +165,10 @@ def logits_gradient(logits: torch.Tensor, tokens: torch.Tensor, weights: torch.T
     ws = _workspace(need, dev)
     _call(dev, nv.lib.mc_logits_gradient, logits.data_ptr(), code, outer, inner, vocab, os, is_, tokens.data_ptr(),
           tokens.element_size(), tos, tis, temperature, weights.data_ptr(), wos, wis, _ptr(entropy_weights), eos, eis,
-          ml2p.data_ptr(), _ptr(ent), out.data_ptr(), _ptr(ws), need)
-    return LogitGradient(ml2p, ent, out)
+          ml2p.data_ptr(), _ptr(ent), grad.data_ptr(), _ptr(ws), need)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)  # (what autograd saved of it is gone: its backward must notice)
+    return LogitGradient(ml2p, ent, grad)
 
 
 def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *, temperature: float = 1.0,
