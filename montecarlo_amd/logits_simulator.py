@@ -100,8 +100,8 @@ class LogitsMonteCarlo(MonteCarlo):
         parts: List[List[str]] = []
         for at in range(0, len(pwds), self.batch):
             ids = [self.encode(p) for p in pwds[at:at + self.batch]]
-            # (a password that is too long is impossible whatever its tokens are: it stands as one unknown token)
-            rows = [r + [self.end] if len(r) < self.max_len else r if len(r) == self.max_len else [OUTSIDE] for r in ids]
+            # (a password that is too long, or holds the end, is impossible whatever its tokens are: it stands as one unknown token)
+            rows = [[OUTSIDE] if len(r) > self.max_len or self.end in r else r + [self.end] if len(r) < self.max_len else r for r in ids]
             width = max(len(r) for r in rows)
             tokens = torch.tensor([r + [SKIP] * (width - len(r)) for r in rows], dtype=torch.int64, device=self.device)
             scores = logits_score(self.logits(tokens[:, :-1].clamp(min=0)), tokens, temperature=self.temperature)

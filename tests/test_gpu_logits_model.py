@@ -57,6 +57,17 @@ def test_probabilities_of_all_strings_add_up_to_one():
     assert m.calc_ml2p("abcab")[0] == 1022.0 and m.calc_ml2p("axe")[0] == 1022.0
 
 
+def test_a_password_that_holds_the_end_is_impossible():
+    class Careless(Bigram):
+        def encode(self, pwd):
+            return [len(self.vocabulary) - 1 if c == "$" else self.vocabulary.index(c) for c in pwd]
+
+    m = Careless("abc", 1, max_len=4)
+    ml2p, parts = m.score_batch(["a$c", "$", "ac", ""])
+    assert ml2p[:2] == [1022.0, 1022.0] and parts[:2] == [["a$c"], ["$"]]
+    assert ml2p[2] < 1022.0 and ml2p[3] < 1022.0
+
+
 def test_samples_are_the_streams_and_come_with_their_scores():
     m = Bigram("abcdefg", 2, max_len=9, batch=700, temperature=0.8)
     m.seed(11, first_id=5)
