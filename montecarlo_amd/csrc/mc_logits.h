@@ -382,18 +382,6 @@ __device__ __forceinline__ u32 block_sum(u32 v) {
     return v;
 }
 
-template <int T>
-__device__ __forceinline__ float block_max(float v) {
-    __shared__ float part[T / 64];
-    v = group_all<64>(v, Max());
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) v = maximum(v, part[w]);
-    return v;
-}
-
 // exclusive prefix sum over the workgroup and the total
 template <int T, typename A>
 __device__ __forceinline__ A block_scan(A v, A &total) {
@@ -410,19 +398,6 @@ __device__ __forceinline__ A block_scan(A v, A &total) {
         total += part[w];
     }
     return base + inc - v;
-}
-
-template <int T>
-__device__ __forceinline__ u32 block_min(u32 v) {
-    __shared__ u32 part[T / 64];
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = min(v, (u32)__shfl_xor(v, d));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) v = min(v, part[w]);
-    return v;
 }
 
 template <int N>
@@ -650,7 +625,7 @@ inline View view_of(const void *p, int64_t outer_stride, int64_t inner_stride, i
     return View{(const char *)p, os, is, os >= 0 && is >= 0 && os < (1ll << 32) && is < (1ll << 32)};
 }
 
-inline bool one_run(uint64_t inner, int64_t outer_stride, int64_t inner_stride) { return outer_stride == (int64_t)inner * inner_stride; }
+inline bool one_run(uint64_t inner, int64_t outer_stride, int64_t inner_stride) { return (u64)outer_stride == inner * (u64)inner_stride; }
 
 // the arguments that every entry point on logits shares (`flat`: everything else that a row has lies as one run too)
 inline int rows_of(const char *who, Rows &a, const void *logits, uint32_t dtype, uint64_t outer, uint64_t inner, uint64_t vocab,
@@ -700,8 +675,8 @@ inline u32 rows_to_blocks(u32 rows, u32 group) { return (u32)(((u64)rows * group
 // How many lanes share a row (G) and how many vectors each of them holds (NV, at most 8).  Many rows: the fewest lanes, since
 // what is done once a row and lane costs as much as eight elements; but four at least, since two lanes ask for 32 bytes of a
 // row at a time and the loads then take as long as the arithmetic saved (1e6 rows of 97 tokens: 46 us with 4 lanes of 4
-// vectors, 48 with 2 of 7).  Few rows (less than a wave for each of the 1024 SIMDs): a lane for each vector, since such a launch waits for its loads and its instructions (12 rows of 97 tokens took
-// 15.7 us with 4 lanes, 4.4 with 32).
+// vectors, 48 with 2 of 7).  Few rows (less than a wave for each of the 1024 SIMDs): a lane for each vector, since such a
+// launch waits for its loads and its instructions (12 rows of 97 tokens took 15.7 us with 4 lanes, 4.4 with 32).
 inline void group_of(u32 rows, u32 vocab, u32 nvec, u32 vec, int &g, int &nv) {
     g = 4, nv = 0;
     if (vocab < vec) return;

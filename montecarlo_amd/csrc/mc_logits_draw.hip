@@ -1,8 +1,8 @@
 // Draws from rows of logits by inversion, and the keys of whole passwords (formulas: mc_logits_score.hip).
 //
 // The draw is defined by running sums in 64 bits.  Sums in 32 bits are known to e = a few parts in 10^6 and leave the token
-// open where u Z lies nearer than that to an end of its interval: a share sum of min(p_i, 2 e) of the draws, one in a
-// thousand at V = 97, one in 20 at V = 32768, every third where 10^5 tokens are about equally likely.  Every row begins
+// open where u Z lies nearer than that to an end of its interval: a share sum of min(p_i, 2 e) of the draws, 0.07 % at V = 97,
+// a tenth at V = 32768 and a quarter at 131072 (logits of deviation 2.5; most where 10^5 are about equally likely).  Every row begins
 // with them (seven operations an element; 64 bits take sixteen) and is summed again in 64 bits where they leave
 // it open; only rows too few to fill the GPU, which wait for their loads and not for arithmetic, begin with 64 bits.
 // Weights in 64 bits come from a polynomial that is right to 4e-11 (this GPU does them at the rate of 32 bits), and where u Z
@@ -765,12 +765,12 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
             sp.vecs = (each + BLOCK - 1) / BLOCK * BLOCK;
             sp.sums = (double *)workspace;
             sp.most = (float *)(sp.sums + ((size_t)a.rows << sp.shift) * PART_WAVES);
-                BY_TYPE(dtype, {
+            BY_TYPE(dtype, {
                 hipLaunchKernelGGL((k_logits_draw_sums<DT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, d, sp);
                 hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(64), 0, s, a, d, sp);
             });
         } else {
-                BY_TYPE(dtype, {
+            BY_TYPE(dtype, {
                 if (few(a.rows)) hipLaunchKernelGGL((k_logits_draw<DT, true>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
                 else hipLaunchKernelGGL((k_logits_draw<DT, false>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
             });
