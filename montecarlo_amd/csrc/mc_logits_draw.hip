@@ -2,9 +2,9 @@
 //
 // The draw is defined by running sums in 64 bits.  Sums in 32 bits are known to e = a few parts in 10^6 and leave the token
 // open where u Z lies nearer than that to an end of its interval: a share sum of min(p_i, 2 e) of the draws, 0.07 % at V = 97,
-// a tenth at V = 32768 and a quarter at 131072 (logits of deviation 2.5; most where 10^5 are about equally likely).  Every row begins
-// with them (seven operations an element; 64 bits take sixteen) and is summed again in 64 bits where they leave
-// it open; only rows too few to fill the GPU, which wait for their loads and not for arithmetic, begin with 64 bits.
+// a tenth at V = 32768 and a quarter at 131072 (logits of deviation 2.5; most where 10^5 are about equally likely).  Rows begin
+// with them (seven operations an element; 64 bits take sixteen) and are summed again in 64 bits where they leave the token
+// open, but for those that begin with 64 bits (in_64_bits).
 // Weights in 64 bits come from a polynomial that is right to 4e-11 (this GPU does them at the rate of 32 bits), and where u Z
 // lies within 1e-10 Z of an end (a row in 10^5) the row is summed once more with the library's exponential.  Exponents of
 // 64 bits reach far enough that no maximum has to be known first.
@@ -262,82 +262,67 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
 // ---- rows of many tokens ---------------------------------------------------------------------------------------------------
 constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 4;
 
-// The token by the definition's weights, by one wave.  (Seldom: where sums that are right to 1e-10 leave it open.)
-template <int DT>
-__device__ __forceinline__ double draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token, float &x) {
-    const u32 lane = threadIdx.x & 63;
-    double z = 0.;
+// The token by the definition's weights, by the whole workgroup: every wave sums a share of the row, and the one whose share
+// holds the token (true there) looks for it, first by steps of 4 x 64 tokens.  Where sums that are right to 1e-10 leave it open:
+// one row of 131072 in 40000, which took a single wave 1.8 ms.
+template <int DT, int T>
+__device__ __forceinline__ bool draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token, float &x, double &z) {
+    constexpr int WAVES = T / 64;
+    constexpr u32 STEP = 4 * 64;
+    __shared__ double part[WAVES];
+    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const auto step_sum = [&](u32 from, u32 to) {
+        float e[4];
+#pragma unroll
+        for (u32 j = 0; j < 4; ++j) e[j] = from + j * 64 + lane < to ? element<DT>(p, from + j * 64 + lane) : -INFINITY;
+        double w = 0.;
 #pragma unroll 1
-    for (u32 i = lane; i < a.vocab; i += 64) z += weight(element<DT>(p, i));
-    z = group_all<64>(z, Add());
+        for (u32 j = 0; j < 4; ++j) {
+            w += weight(e[0]);
+            e[0] = e[1], e[1] = e[2], e[2] = e[3];
+        }
+        return w;
+    };
+    const u32 share = (a.vocab / STEP / WAVES + 1) * STEP, i0 = min(wave * share, a.vocab), i1 = min(a.vocab, i0 + share);
+    double s = 0.;
+#pragma unroll 1
+    for (u32 i = i0; i < i1; i += STEP) s += step_sum(i, i1);
+    s = group_all<64>(s, Add());
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    const double inc = group_scan<64>(lane < (u32)WAVES ? part[lane] : 0.);
+    z = __shfl(inc, 63);
     const double target = u * z;
-    double before = 0.;
-    token = 0;
+    const u64 passes = __ballot(inc > target);
+    const u32 who = passes ? (u32)__ffsll((unsigned long long)passes) - 1 : WAVES - 1;
+    if (wave != who) return false;
+    double before = who ? __shfl(inc, (int)who - 1) : 0.;
+    u32 from = i0;
 #pragma unroll 1
-    for (u32 base = 0; base < a.vocab; base += 64) {
-        const float e = base + lane < a.vocab ? element<DT>(p, base + lane) : -INFINITY;
-        const double w = weight(e), inc = before + group_scan<64>(w);
-        const u64 over = __ballot(w > 0. && inc > target), some = __ballot(w > 0.);
-        // (none yet: the last token with any weight stands in for a target at or behind the last running sum)
-        if (some) {
-            const u32 who = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u - (u32)__clzll((long long)some);
-            token = base + who;
-            x = __shfl(e, who);
-        }
-        if (over) break;
-        before = __shfl(inc, 63);
-    }
-    return z;
-}
-
-// The token among vectors v0 .. v1, whose running sums in 32 bits begin at `before`, by one wave in rounds of STEPS steps of 64
-// vectors: true in the lane that holds it, and only there, when no end of its interval is nearer than `near`.
-template <int DT>
-__device__ __forceinline__ bool locate_fast(const Span &r, const Expo &y_of, u32 v0, u32 v1, float before, float target, float near, u32 &token,
-                                            float &x) {
-    const u32 lane = threadIdx.x & 63;
-    if (v0 == 0 && r.head) {
-        const float next = before + exp2_(y_of.fast(r.first));
-        if (next > target) {
-            token = 0;
-            x = r.first;
-            return lane == 0 && next - target >= near;
-        }
-        if (target - next < near) return false;
+    for (; from + STEP < i1; from += STEP) {
+        const double next = before + group_all<64>(step_sum(from, i1), Add());
+        if (next > target) break;
         before = next;
     }
+    token = 0;
+    // (the last token with any weight stands in for a target at or behind the last running sum: found from 0 on, if not from here)
+    for (bool any = false, again = false; !any && !again; again = from == 0, from = 0, before = 0.) {
 #pragma unroll 1
-    for (u32 base = v0; base < v1; base += 64 * STEPS) {
-        raw4 q[STEPS];
-        float s[STEPS], upto[STEPS];
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) q[i] = load_vec<DT>(r, base + i * 64 + lane, v1);
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            float w[VEC<DT>];
-#pragma unroll
-            for (int j = 0; j < VEC<DT>; ++j) w[j] = exp2_(y_of.fast(unpack<DT>(q[i], j)));
-            s[i] = pairs<VEC<DT>>(w);
-            upto[i] = (i ? upto[i ? i - 1 : 0] : before) + group_all<64>(s[i], Add());
-        }
-        if (upto[STEPS - 1] > target) {
-            raw4 mq = q[0];
-            float mine = s[0];
-            u32 step = 0;
-#pragma unroll
-            for (int i = 1; i < STEPS; ++i) {
-                const bool past = upto[i - 1] <= target;
-                before = past ? upto[i - 1] : before;
-                mine = past ? s[i] : mine;
-                step += past;
-                choose(mq, q[i], past);
+        for (u32 base = from; base < a.vocab; base += 64) {
+            const float e = base + lane < a.vocab ? element<DT>(p, base + lane) : -INFINITY;
+            const double w = weight(e), upto = before + group_scan<64>(w);
+            const u64 over = __ballot(w > 0. && upto > target), some = __ballot(w > 0.);
+            if (some) {
+                const u32 at = over ? (u32)__ffsll((unsigned long long)over) - 1 : 63u - (u32)__clzll((long long)some);
+                token = base + at;
+                x = __shfl(e, at);
+                any = true;
             }
-            const float t = target - (before + (group_scan<64>(mine) - mine));
-            return place_of<DT>(mq, y_of, t, near, r.head + (base + step * 64 + lane) * VEC<DT>, token, x);
+            if (over) break;
+            before = __shfl(upto, 63);
         }
-        before = upto[STEPS - 1];
     }
-    return false;
+    return true;
 }
 
 // The token among vectors v0 .. v1, whose running sums begin at `before`, by one wave: the sums of rounds of STEPS steps of
@@ -465,50 +450,55 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
     }
 }
 
-// A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave.  `within` (if by_shares): the same
-// for the PART_WAVES shares of the lane's part.  (Sums of Power are those of PowerBelow for m = 0 but for roundings far
-// below the margin.)
+// A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave; false where its outputs are still to
+// be put.  `within` (if by_shares): the same for the PART_WAVES shares of the lane's part.  (Sums of Power are those of PowerBelow
+// for m = 0 but for roundings far below the margin.)
 template <int DT>
-__device__ __forceinline__ void put_token(const Rows &a, const DrawArgs &d, u32 row, const char *p, const Span &r, const PowerBelow &weight, float m, double mine,
-                                          u32 share, double u, bool by_shares, const double (&within)[PART_WAVES]) {
-    const double inc = group_scan<64>(mine);
-    double z = __shfl(inc, 63), ref = weight.m;
-    const double target = u * z;
+__device__ __forceinline__ bool put_token(const DrawArgs &d, u32 row, const Span &r, const PowerBelow &weight, double mine, u32 share, double u,
+                                          bool by_shares, const double (&within)[PART_WAVES]) {
+    const double inc = group_scan<64>(mine), z = __shfl(inc, 63), target = u * z;
     const u64 passes = __ballot(inc > target);
+    if (!passes) return false;
+    const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
+    double before = __shfl(inc - mine, part);
+    u32 v0 = part * share, v1 = v0 + share;
+    if (by_shares) {
+        v1 = v0;
+        bool found = false;
+#pragma unroll
+        for (int w = 0; w < PART_WAVES; ++w) {
+            const double next = before + __shfl(within[w], part);
+            if (!found) v1 = v0 + share / PART_WAVES;
+            found = found || next > target;
+            if (!found && w + 1 < PART_WAVES) before = next, v0 = v1;
+        }
+    }
     u32 token = 0;
     float x = 0.f;
-    bool sure = false;
-    if (passes) {
-        const u32 part = (u32)__ffsll((unsigned long long)passes) - 1;
-        double before = __shfl(inc - mine, part);
-        u32 v0 = part * share, v1 = v0 + share;
-        if (by_shares) {
-            v1 = v0;
-            bool found = false;
-#pragma unroll
-            for (int w = 0; w < PART_WAVES; ++w) {
-                const double next = before + __shfl(within[w], part);
-                if (!found) v1 = v0 + share / PART_WAVES;
-                found = found || next > target;
-                if (!found && w + 1 < PART_WAVES) before = next, v0 = v1;
-            }
-        }
-        sure = locate<DT>(r, weight, min(v0, r.nvec), min(r.nvec, v1), before, target, MARGIN * z, token, x);
-    }
-    if (!sure) {
-        ref = (double)m;
-        z = draw_exact<DT>(p, a, Definition{d.t, ref}, u, token, x);
-    }
+    if (!locate<DT>(r, weight, min(v0, r.nvec), min(r.nvec, v1), before, target, MARGIN * z, token, x)) return false;
     if ((threadIdx.x & 63) == 0) {
         d.token[row] = (int)token;
-        d.ml2p[row] = ml2p_under(z, ((double)x - ref) * d.power.c);
+        d.ml2p[row] = ml2p_under(z, ((double)x - weight.m) * d.power.c);
+    }
+    return true;
+}
+
+// the same by the definition, by the workgroup
+template <int DT, int T>
+__device__ __forceinline__ void put_exact(const Rows &a, const DrawArgs &d, u32 row, const char *p, float m, double u) {
+    u32 token;
+    float x = m;
+    double z;
+    if (draw_exact<DT, T>(p, a, Definition{d.t, (double)m}, u, token, x, z) && (threadIdx.x & 63) == 0) {
+        d.token[row] = (int)token;
+        d.ml2p[row] = ml2p_under(z, ((double)x - (double)m) * d.power.c);
     }
 }
 
-// One workgroup a row.  Its waves sum a share of it each, and the wave whose share holds the token looks at it again.
-template <int DT, bool BEGIN64>
-__global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, DrawArgs d) {
-    __shared__ float pm[WIDE_WAVES], pf[WIDE_WAVES];
+// One workgroup a row, in 64 bits.  Its waves sum a share of it each, and the wave whose share holds the token looks at it again.
+template <int DT>
+__global__ __launch_bounds__(WIDE, 4) void k_logits_draw(Rows a, DrawArgs d) {
+    __shared__ float pm[WIDE_WAVES];
     __shared__ double ps[WIDE_WAVES];
     __shared__ int done;
     const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -524,29 +514,16 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
     const Span r = span_of<DT>(a, p);
     const double u = uniform_of(d, row);
     const u32 share = (r.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
-    Stat st{-INFINITY, 0.f, 0.f, false};
-    double s = 0.;
-    if constexpr (BEGIN64) {
-        sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, st.m);
-    } else {
-        for (u32 v = v0; v < v1; v += 64 * UNROLL) {
-            raw4 q[UNROLL];
-            load_chunk<DT, 64>(q, r, v, lane, v1);
-            take<DT, false>(st, q, a.c);
-        }
-        if (threadIdx.x == 0) take_one<false>(st, r.first, a.c);
-        st = group_stat<64, false>(st, a.c);
-    }
+    double s;
+    float m;
+    sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, m);
     if (lane == 0) {
-        pm[wave] = st.m;
-        pf[wave] = st.s;
+        pm[wave] = m;
         ps[wave] = s;
     }
     if (threadIdx.x == 0) done = 0;
     __syncthreads();
-    // eight lanes hold the eight waves' sums, each under its own largest logit
-    const u32 of = lane & (WIDE_WAVES - 1);
-    const float m = group_all<WIDE_WAVES>(pm[of], Max());
+    m = group_all<WIDE_WAVES>(pm[lane & (WIDE_WAVES - 1)], Max());
     if (!drawable(m)) {
         if (threadIdx.x == 0) {
             d.token[row] = MC_TOKEN_OUTSIDE;
@@ -554,15 +531,131 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
         }
         return;
     }
-    if (!BEGIN64 && !doubtful(m, a.c)) {
+    const bool suits = good(m, d.power.c);
+    const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
+    if (!suits) {
+        float unused;
+        sum_vecs<DT, UNROLL>(r, weight, v0, v1, lane, s, unused);
+        if (lane == 0) ps[wave] = s;  // (nobody has read the first ones)
+        __syncthreads();
+    }
+    const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum);
+    const u64 passes = __ballot(inc > u * __shfl(inc, 63));
+    if (wave == (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) {
+        const double none[PART_WAVES] = {};
+        if (put_token<DT>(d, row, r, weight, part_sum, share, u, false, none)) done = 1;
+    }
+    __syncthreads();
+    if (!done) put_exact<DT, WIDE>(a, d, row, p, m, u);
+}
+
+// One workgroup a row, in 32 bits first, the row in the registers of T lanes, HELD vectors each at most: what decides it is not
+// loaded again (bf16, 30000 rows of 4099: 200 us when streamed, 96 held; 8000 of 16384: 73 and 62; 1024 of 131072: 128 and 107; 4096
+// of 32768: 74 and 73, where both wait for the loads in flight).  The waves' vectors lie behind each other.
+template <int DT, int T, int HELD>
+__global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a, DrawArgs d) {
+    constexpr int WAVES = T / 64;
+    __shared__ float pm[WAVES], pf[WAVES];
+    __shared__ double ps[WAVES];
+    __shared__ int done;
+    const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (row >= a.rows) return;
+    if (d.live && !d.live[row]) {
+        if (threadIdx.x == 0) {
+            d.token[row] = MC_TOKEN_SKIP;
+            d.ml2p[row] = 0.f;
+        }
+        return;
+    }
+    const char *p = at(a.logits, a.inner, row);
+    const Span r = span_of<DT>(a, p);
+    const u32 nv = (r.nvec + T - 1) / T, v0 = wave * nv * 64;
+    raw4 q[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        q[i] = nothing<DT>();
+        if (i < (int)nv) q[i] = load_vec<DT>(r, v0 + i * 64 + lane, r.nvec);
+    }
+    const double u = uniform_of(d, row);
+    float m = threadIdx.x == 0 ? r.first : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (i < (int)nv) {
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) m = maximum(m, unpack<DT>(q[i], j));
+        }
+    }
+    m = group_all<64>(m, Max());
+    const auto sum_of = [&](const raw4 &v, const Expo &y_of) {
+        float w[VEC<DT>];
+#pragma unroll
+        for (int j = 0; j < VEC<DT>; ++j) w[j] = exp2_(y_of.fast(unpack<DT>(v, j)));
+        return pairs<VEC<DT>>(w);
+    };
+    float s[HELD];
+    {
         const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
-        const float w = times2(pf[of], scaled(pm[of], a.c) - y_of.M), inc = group_scan<WIDE_WAVES>(w), z = __shfl(inc, WIDE_WAVES - 1);
-        const float target = (float)(u * (double)z);
-        const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WIDE_WAVES) - 1));
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            asm("" : "+v"(q[i]));  // (see forget)
+            s[i] = i < (int)nv ? sum_of(q[i], y_of) : 0.f;
+        }
+        const float sum = pairs<HELD>(s) + (threadIdx.x == 0 ? exp2_(y_of.fast(r.first)) : 0.f), all = group_all<64>(sum, Add());
+        if (lane == 0) {
+            pm[wave] = m;
+            pf[wave] = all;
+        }
+    }
+    if (threadIdx.x == 0) done = 0;
+    __syncthreads();
+    // as many lanes as there are waves hold the waves' sums, each under its own largest logit
+    const u32 of = lane & (WAVES - 1);
+    const float mine_m = m;
+    m = group_all<WAVES>(pm[of], Max());
+    if (!drawable(m)) {
+        if (threadIdx.x == 0) {
+            d.token[row] = MC_TOKEN_OUTSIDE;
+            d.ml2p[row] = no_draw(m);
+        }
+        return;
+    }
+    if (!doubtful(m, a.c)) {
+        const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
+        const float w = times2(pf[of], scaled(pm[of], a.c) - y_of.M), inc = group_scan<WAVES>(w), z = __shfl(inc, WAVES - 1);
+        const float target = (float)(u * (double)z), near = (float)d.margin * z;
+        const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WAVES) - 1));
         if (wave == part) {
-            u32 token;
-            float x;
-            if (locate_fast<DT>(r, y_of, v0, v1, __shfl(inc - w, part), target, (float)d.margin * z, token, x)) {
+            u32 token = 0;
+            float x = r.first, run = __shfl(inc - w, part);
+            bool here = false, sure = true;  // (here: the row's first element is it)
+            if (wave == 0 && r.head) {
+                run = exp2_(y_of.fast(r.first));
+                here = run > target;
+                sure = here ? lane == 0 && run - target >= near : target - run >= near;
+            }
+            if (!here && sure) {
+                const float d2 = scaled(mine_m, a.c) - y_of.M;
+                raw4 mq = q[0];
+                float mine = 0.f, start = run;
+                u32 step = 0;
+                bool found = false;
+#pragma unroll
+                for (int i = 0; i < HELD; ++i) {
+                    if (i < (int)nv) {
+                        const float t = times2(s[i], d2), upto = run + group_all<64>(t, Add());
+                        const bool now = !found && upto > target;
+                        mine = now ? t : mine;
+                        start = now ? run : start;
+                        step = now ? i : step;
+                        choose(mq, q[i], now);
+                        found = found || now;
+                        run = upto;
+                    }
+                }
+                const float t = target - (start + (group_scan<64>(mine) - mine));
+                sure = found && place_of<DT>(mq, y_of, t, near, r.head + (v0 + step * 64 + lane) * VEC<DT>, token, x);
+            }
+            if (sure) {
                 d.token[row] = (int)token;
                 d.ml2p[row] = log2_(z) - y_of.fast(x);
                 done = 1;
@@ -572,29 +665,37 @@ __global__ __launch_bounds__(WIDE, BEGIN64 ? 4 : 8) void k_logits_draw(Rows a, D
         if (done) return;
     }
     // in 64 bits
-    const bool suits = good(m, d.power.c);
-    if (!suits || !BEGIN64) {
-        float unused;
-        if (suits) sum_vecs<DT, UNROLL>(r, d.power, v0, v1, lane, s, unused);
-        else sum_vecs<DT, UNROLL>(r, PowerBelow{d.power.c, (double)m}, v0, v1, lane, s, unused);
-        __syncthreads();  // (no wave still reads the first ones)
-        if (lane == 0) ps[wave] = s;
-        __syncthreads();
+    const PowerBelow weight{d.power.c, (double)m};
+    double sum = threadIdx.x == 0 ? weight(r.first) : 0.;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        asm("" : "+v"(q[i]));
+        if (i < (int)nv) {
+#pragma unroll
+            for (int j = 0; j < VEC<DT>; ++j) sum += weight(unpack<DT>(q[i], j));
+        }
     }
-    const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), target = u * __shfl(inc, 63);
-    const u64 passes = __ballot(inc > target);
-    if (wave != (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) return;
-    const double none[PART_WAVES] = {};
-    put_token<DT>(a, d, row, p, r, PowerBelow{d.power.c, suits ? 0. : (double)m}, m, part_sum, share, u, false, none);
+    sum = group_all<64>(sum, Add());
+    if (lane == 0) ps[wave] = sum;
+    __syncthreads();
+    const double part_sum = lane < (u32)WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum);
+    const u64 passes = __ballot(inc > u * __shfl(inc, 63));
+    if (wave == (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) {
+        const double none[PART_WAVES] = {};
+        if (put_token<DT>(d, row, r, weight, part_sum, nv * 64, u, false, none)) done = 1;
+    }
+    __syncthreads();
+    if (!done) put_exact<DT, T>(a, d, row, p, m, u);
 }
 
-// The parts of a row joined, one wave a row.
+// The parts of a row joined, by the workgroup's first wave; the others help where it leaves the token open.
 template <int DT>
-__global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Split sp) {
+__global__ __launch_bounds__(BLOCK) void k_logits_draw_join(Rows a, DrawArgs d, Split sp) {
+    __shared__ int done;
     const u32 row = block_id(), lane = threadIdx.x & 63;
     if (row >= a.rows) return;
     if (d.live && !d.live[row]) {
-        if (lane == 0) {
+        if (threadIdx.x == 0) {
             d.token[row] = MC_TOKEN_SKIP;
             d.ml2p[row] = 0.f;
         }
@@ -613,26 +714,34 @@ __global__ __launch_bounds__(64) void k_logits_draw_join(Rows a, DrawArgs d, Spl
     }
     m = group_all<64>(m, Max());
     if (!drawable(m)) {
-        if (lane == 0) {
+        if (threadIdx.x == 0) {
             d.token[row] = MC_TOKEN_OUTSIDE;
             d.ml2p[row] = no_draw(m);
         }
         return;
     }
-    const bool suits = good(m, d.power.c);
-    const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
-    if (!suits) {
-        float unused;
-        sum_vecs<DT, UNROLL>(r, weight, 0, r.nvec, lane, mine, unused);
-        if (lane) mine = 0.;
+    if (threadIdx.x < 64) {
+        const bool suits = good(m, d.power.c);
+        const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
+        if (!suits) {
+            float unused;
+            sum_vecs<DT, UNROLL>(r, weight, 0, r.nvec, lane, mine, unused);
+            if (lane) mine = 0.;
+        }
+        const bool sure = put_token<DT>(d, row, r, weight, mine, suits ? sp.vecs : r.nvec, u, suits, within);
+        if (lane == 0) done = sure;
     }
-    put_token<DT>(a, d, row, p, r, weight, m, mine, suits ? sp.vecs : r.nvec, u, suits, within);
+    __syncthreads();
+    if (!done) put_exact<DT, BLOCK>(a, d, row, p, m, u);
 }
 
-// Few rows begin with 64 bits: they wait for their loads, not for arithmetic, and a row that 32 bits leave open is read again
-// (64 rows of 20000 tokens: 17 us).  Of more than 40000 tokens they are cut into parts that still hold a chunk of 16 KB; a second
-// launch costs 4 us, which shorter rows take less than.
+// Rows begin with 64 bits where 32 would leave too many open: from 128 KB on (of 4-byte logits, which 64 bits keep up with: 2048
+// rows of 41000 tokens 89 us, 120 from 32 bits on; 2048 of 20000 52 and 48) or 256 KB (1024 rows of 200000 tokens of two bytes 176 us,
+// 210 from 32 bits on; 1024 of 90000 83 and 78).  Few rows do too: they wait for their loads, not for arithmetic, and an open
+// row would be summed twice (511 rows of 30000 tokens 21 us, 512 from 32 bits on 26).  Few rows of more than 40000 tokens are cut
+// into parts that still hold a chunk of 16 KB; a second launch costs 4 us, which shorter rows take less than.
 bool few(u32 rows) { return rows < 512; }
+bool in_64_bits(u32 rows, u32 dtype, u32 nvec) { return few(rows) || nvec > (dtype == MC_LOGITS_F32 ? 512u * 16 : 1024u * 16); }
 u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
     u32 shift = 0;
     while (few(rows) && vocab > 40000 && shift < 6 && ((u64)rows << shift) < 512 && (nvec >> (shift + 1)) >= BLOCK * UNROLL) ++shift;
@@ -644,11 +753,26 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 // How near u Z may come to an end of a token's interval, as a share of Z, before sums in 32 bits leave the token open, in half
 // steps.  The weights: 2 for the power, 1.4 times its exponent for the exponent's two roundings, which the weights' mean
 // makes at most log2 V + 1 (they weigh once: what is off in the running sum is off in Z too).  Of the additions behind each
-// other, in Z: 3 in a vector and 2 in a chunk (in pairs), a lane's chunks or vectors, 6 over lanes, 3 over waves; in the running
-// sum as many and 8 in the last vector; 3 where its parts are joined, 2 for the target.
+// other, in Z: 3 in a vector and at most 8 (one after the other) or 4 + 1 (in pairs, and the row's first element) over a lane's,
+// 6 over lanes, 4 over waves.
+// The running sum up to a wave, or inside it up to a step of 64 vectors, has at most as many; then one for each step before,
+// 8 in the last vector, 3 where its parts are joined, 2 for the target.
 double margin_of(const Rows &a) {
-    const double adds = a.nvec <= SUB_VECS ? 3 + 8 + 6 : 3 + 2 + (a.nvec / (WIDE * UNROLL) + 1) + 6 + 3;
-    return 0x1p-24 * (2 + 1.4 * (std::log2((double)a.vocab) + 1) + 2 * adds + 8 + 5);
+    const double adds = a.nvec <= SUB_VECS ? 3 + 8 + 6 : 3 + 4 + 1 + 6 + 4, steps = a.nvec <= SUB_VECS ? 0 : a.nvec <= 512 * 8 ? 8 : 16;
+    return 0x1p-24 * (2 + 1.4 * (std::log2((double)a.vocab) + 1) + 2 * adds + steps + 8 + 3 + 2);
+}
+
+template <int DT>
+void launch_wide(const Rows &a, const DrawArgs &d, hipStream_t s) {
+    if (in_64_bits(a.rows, DT, a.nvec)) {
+        hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
+        return;
+    }
+    // the fewest lanes that hold the row with eight waves a SIMD, then with four
+    if (a.nvec <= 256 * 8) hipLaunchKernelGGL((k_logits_draw_held<DT, 256, 8>), grid_of(a.rows), dim3(256), 0, s, a, d);
+    else if (a.nvec <= 512 * 8) hipLaunchKernelGGL((k_logits_draw_held<DT, 512, 8>), grid_of(a.rows), dim3(512), 0, s, a, d);
+    else if (DT == MC_LOGITS_F32 || a.nvec <= 512 * 16) hipLaunchKernelGGL((k_logits_draw_held<DT, 512, 16>), grid_of(a.rows), dim3(512), 0, s, a, d);
+    else if constexpr (DT != MC_LOGITS_F32) hipLaunchKernelGGL((k_logits_draw_held<DT, 1024, 16>), grid_of(a.rows), dim3(1024), 0, s, a, d);
 }
 
 // ---- keys ----------------------------------------------------------------------------------------------------------
@@ -767,13 +891,10 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
             sp.most = (float *)(sp.sums + ((size_t)a.rows << sp.shift) * PART_WAVES);
             BY_TYPE(dtype, {
                 hipLaunchKernelGGL((k_logits_draw_sums<DT>), grid_of(a.rows << sp.shift), dim3(BLOCK), 0, s, a, d, sp);
-                hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(64), 0, s, a, d, sp);
+                hipLaunchKernelGGL((k_logits_draw_join<DT>), grid_of(a.rows), dim3(BLOCK), 0, s, a, d, sp);
             });
         } else {
-            BY_TYPE(dtype, {
-                if (few(a.rows)) hipLaunchKernelGGL((k_logits_draw<DT, true>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
-                else hipLaunchKernelGGL((k_logits_draw<DT, false>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
-            });
+            BY_TYPE(dtype, launch_wide<DT>(a, d, s));
         }
     }
     HIP_TRY(hipGetLastError());

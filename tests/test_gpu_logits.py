@@ -350,6 +350,40 @@ def test_draw_at_and_beside_the_borders(vocab):
     assert close <= 8, close
 
 
+@pytest.mark.parametrize("rows", [600, 40])
+@pytest.mark.parametrize("vocab,dtype", [(2305, "fp32"), (4099, "fp16"), (20001, "bf16"), (50001, "fp16"), (66001, "bf16"), (33001, "fp32"),
+                                         (140001, "fp16")])
+def test_draw_beside_the_borders_of_many_rows(vocab, dtype, rows):
+    """As above for every way that rows of many tokens are drawn, down to where 64 bits leave it to the definition: numpy's running
+    sums are right to 1e-12 here (vocab roundings of 2^-53), a tenth of the least distance."""
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.randn(vocab, generator=g) * 2).to(DTYPES[dtype])
+    x[torch.rand(vocab, generator=g) < 0.05] = -math.inf
+    x[0] = 1.0
+    w = np.exp(x.double().numpy() - x.double().max().item())
+    c = np.cumsum(w)
+    c /= c[-1]
+    at = np.unique(np.concatenate([[0], np.linspace(0, vocab - 1, rows // 8 + 1).astype(int)]))
+    at = at[w[at] > 1e-6][:rows // 8]
+    us = np.concatenate([c[at] + s * d for s in (-1, 1) for d in (1.5e-11, 8e-11, 2e-8, 1e-6)])
+    us = np.clip(np.concatenate([us, np.linspace(0, 1, rows, endpoint=False)])[:rows], 0, 1 - 2.0 ** -53)
+    r = lg.logits_draw(x.cuda().expand(rows, vocab), torch.from_numpy(us).cuda())
+    want = np.searchsorted(c, us, side="right")
+    assert r.tokens.tolist() == want.tolist()
+    ml2p = -np.log2(w[want] / w.sum())
+    assert np.all(np.abs(r.ml2p.cpu().numpy() - ml2p) <= 2.0 ** -24 * (steps_of(vocab) + np.abs(ml2p)))
+
+
+@pytest.mark.parametrize("vocab,dtype", [(4099, "fp16"), (20001, "bf16"), (66001, "bf16"), (140001, "fp32")])
+def test_draw_of_many_rows_outside_zero_to_one(vocab, dtype):
+    x = torch.full((600, vocab), 2.0, dtype=DTYPES[dtype], device="cuda")
+    x[:, 0] = -math.inf
+    x[:, vocab - 700:] = -math.inf
+    u = torch.tensor([-1.0, math.nan, 1.0, 5.0, math.inf, 1 - 2.0 ** -53] * 100, dtype=torch.float64)
+    last = vocab - 701
+    assert lg.logits_draw(x, u.cuda()).tokens.tolist() == [1, 1, last, last, last, last] * 100
+
+
 @pytest.mark.parametrize("vocab", [5, 97, 3000, 60000])
 def test_draw_outside_zero_to_one(vocab):
     x = torch.zeros(5, vocab)
