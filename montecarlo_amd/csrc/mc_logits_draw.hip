@@ -2,7 +2,7 @@
 //
 // The draw is defined by running sums in 64 bits.  Sums in 32 bits are known to e = a few parts in 10^6 and leave the token
 // open where u Z lies nearer than that to an end of its interval: a share sum of min(p_i, 2 e) of the draws, 0.07 % at V = 97,
-// a tenth at V = 32768 and a quarter at 131072 (logits of deviation 2.5; most where 10^5 are about equally likely).  Rows begin
+// a twelfth at V = 32768 and a fifth at 131072 (logits of deviation 2.5; most where 10^5 are about equally likely).  Rows begin
 // with them (seven operations an element; 64 bits take sixteen) and are summed again in 64 bits where they leave the token
 // open, but for those that begin with 64 bits (in_64_bits).
 // Weights in 64 bits come from a polynomial that is right to 4e-11 (this GPU does them at the rate of 32 bits), and where u Z
@@ -550,12 +550,12 @@ __global__ __launch_bounds__(WIDE, 4) void k_logits_draw(Rows a, DrawArgs d) {
 }
 
 // One workgroup a row, in 32 bits first, the row in the registers of T lanes, HELD vectors each at most: what decides it is not
-// loaded again (bf16, 30000 rows of 4099: 200 us when streamed, 96 held; 8000 of 16384: 73 and 62; 1024 of 131072: 128 and 107; 4096
-// of 32768: 74 and 73, where both wait for the loads in flight).  The waves' vectors lie behind each other.
+// loaded again (bf16, 16000 rows of 8192 tokens: 115 us when streamed, 70 held; 2600 of 50001: 95 and 84; 4096 of 32768: 80 and 75).  The
+// waves' vectors lie behind each other.  (Eight waves a SIMD spill: 83 us for the last of these.)
 template <int DT, int T, int HELD>
-__global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a, DrawArgs d) {
+__global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a, DrawArgs d) {
     constexpr int WAVES = T / 64;
-    __shared__ float pm[WAVES], pf[WAVES];
+    __shared__ float pm[WAVES];
     __shared__ double ps[WAVES];
     __shared__ int done;
     const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -600,10 +600,11 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a
             asm("" : "+v"(q[i]));  // (see forget)
             s[i] = i < (int)nv ? sum_of(q[i], y_of) : 0.f;
         }
-        const float sum = pairs<HELD>(s) + (threadIdx.x == 0 ? exp2_(y_of.fast(r.first)) : 0.f), all = group_all<64>(sum, Add());
+        const float sum = pairs<HELD>(s) + (threadIdx.x == 0 ? exp2_(y_of.fast(r.first)) : 0.f);
+        const double all = group_all<64>((double)sum, Add());  // (lanes and waves in 64 bits: a third fewer rows stay open)
         if (lane == 0) {
             pm[wave] = m;
-            pf[wave] = all;
+            ps[wave] = all;
         }
     }
     if (threadIdx.x == 0) done = 0;
@@ -621,28 +622,32 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a
     }
     if (!doubtful(m, a.c)) {
         const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
-        const float w = times2(pf[of], scaled(pm[of], a.c) - y_of.M), inc = group_scan<WAVES>(w), z = __shfl(inc, WAVES - 1);
-        const float target = (float)(u * (double)z), near = (float)d.margin * z;
+        const double w = __builtin_ldexp(ps[of], (int)(scaled(pm[of], a.c) - y_of.M)), inc = group_scan<WAVES>(w), z = __shfl(inc, WAVES - 1);
+        const double target = u * z;
+        const float near = (float)(d.margin * z);
         const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WAVES) - 1));
         if (wave == part) {
             u32 token = 0;
-            float x = r.first, run = __shfl(inc - w, part);
+            float x = r.first;
+            double run = __shfl(inc - w, part);
             bool here = false, sure = true;  // (here: the row's first element is it)
             if (wave == 0 && r.head) {
                 run = exp2_(y_of.fast(r.first));
                 here = run > target;
-                sure = here ? lane == 0 && run - target >= near : target - run >= near;
+                sure = here ? lane == 0 && run - target >= (double)near : target - run >= (double)near;
             }
             if (!here && sure) {
                 const float d2 = scaled(mine_m, a.c) - y_of.M;
                 raw4 mq = q[0];
-                float mine = 0.f, start = run;
+                float mine = 0.f;
+                double start = run;
                 u32 step = 0;
                 bool found = false;
 #pragma unroll
                 for (int i = 0; i < HELD; ++i) {
                     if (i < (int)nv) {
-                        const float t = times2(s[i], d2), upto = run + group_all<64>(t, Add());
+                        const float t = times2(s[i], d2);
+                        const double upto = run + (double)group_all<64>(t, Add());
                         const bool now = !found && upto > target;
                         mine = now ? t : mine;
                         start = now ? run : start;
@@ -652,12 +657,12 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a
                         run = upto;
                     }
                 }
-                const float t = target - (start + (group_scan<64>(mine) - mine));
+                const float t = (float)(target - (start + (double)(group_scan<64>(mine) - mine)));
                 sure = found && place_of<DT>(mq, y_of, t, near, r.head + (v0 + step * 64 + lane) * VEC<DT>, token, x);
             }
             if (sure) {
                 d.token[row] = (int)token;
-                d.ml2p[row] = log2_(z) - y_of.fast(x);
+                d.ml2p[row] = log2_((float)z) - y_of.fast(x);
                 done = 1;
             }
         }
@@ -676,6 +681,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_draw_held(Rows a
         }
     }
     sum = group_all<64>(sum, Add());
+    __syncthreads();  // (every wave has read the first ones)
     if (lane == 0) ps[wave] = sum;
     __syncthreads();
     const double part_sum = lane < (u32)WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum);
@@ -752,14 +758,13 @@ size_t split_bytes(u32 rows, u32 shift) { return shift ? ((size_t)rows << shift)
 
 // How near u Z may come to an end of a token's interval, as a share of Z, before sums in 32 bits leave the token open, in half
 // steps.  The weights: 2 for the power, 1.4 times its exponent for the exponent's two roundings, which the weights' mean
-// makes at most log2 V + 1 (they weigh once: what is off in the running sum is off in Z too).  Of the additions behind each
-// other, in Z: 3 in a vector and at most 8 (one after the other) or 4 + 1 (in pairs, and the row's first element) over a lane's,
-// 6 over lanes, 4 over waves.
-// The running sum up to a wave, or inside it up to a step of 64 vectors, has at most as many; then one for each step before,
-// 8 in the last vector, 3 where its parts are joined, 2 for the target.
+// makes at most log2 V + 1 (they weigh once: what is off in the running sum is off in Z too).  Rows of few tokens: of the
+// additions behind each other, in Z and in the running sum 3 in a vector (in pairs), 8 steps, 6 over lanes; 8 in the last vector, 3
+// where its parts are joined, 2 for the target.  Rows held by a workgroup: in Z 3 in a vector, 4 over a lane's (in pairs) and 1
+// for the row's first element; in the running sum 3 and 6 over lanes, 8 in the last vector, 3 where its parts are joined.
 double margin_of(const Rows &a) {
-    const double adds = a.nvec <= SUB_VECS ? 3 + 8 + 6 : 3 + 4 + 1 + 6 + 4, steps = a.nvec <= SUB_VECS ? 0 : a.nvec <= 512 * 8 ? 8 : 16;
-    return 0x1p-24 * (2 + 1.4 * (std::log2((double)a.vocab) + 1) + 2 * adds + steps + 8 + 3 + 2);
+    const double sums = a.nvec <= SUB_VECS ? 2 * (3 + 8 + 6) + 8 + 3 + 2 : (3 + 4 + 1) + (3 + 6) + 8 + 3;
+    return 0x1p-24 * (2 + 1.4 * (std::log2((double)a.vocab) + 1) + sums);
 }
 
 template <int DT>
@@ -768,7 +773,7 @@ void launch_wide(const Rows &a, const DrawArgs &d, hipStream_t s) {
         hipLaunchKernelGGL((k_logits_draw<DT>), grid_of(a.rows), dim3(WIDE), 0, s, a, d);
         return;
     }
-    // the fewest lanes that hold the row with eight waves a SIMD, then with four
+    // the fewest lanes that hold the row with six waves a SIMD, then with four
     if (a.nvec <= 256 * 8) hipLaunchKernelGGL((k_logits_draw_held<DT, 256, 8>), grid_of(a.rows), dim3(256), 0, s, a, d);
     else if (a.nvec <= 512 * 8) hipLaunchKernelGGL((k_logits_draw_held<DT, 512, 8>), grid_of(a.rows), dim3(512), 0, s, a, d);
     else if (DT == MC_LOGITS_F32 || a.nvec <= 512 * 16) hipLaunchKernelGGL((k_logits_draw_held<DT, 512, 16>), grid_of(a.rows), dim3(512), 0, s, a, d);
