@@ -41,6 +41,7 @@ class LogitsMonteCarlo(MonteCarlo):
         return [self._ids.get(c, OUTSIDE) for c in pwd]
 
     # ---- sampling (lib4mc/MonteCarloParent.py:33-46) ---------------------------------------------------------------
+    @torch.no_grad()
     def _sample_batch(self, n: int, seed: int, first: int) -> Tuple[torch.Tensor, torch.Tensor]:
         tokens = torch.full((n, self.max_len), SKIP, dtype=torch.int64, device=self.device)
         ml2p = torch.zeros((n, self.max_len), dtype=torch.float32, device=self.device)
@@ -94,6 +95,7 @@ class LogitsMonteCarlo(MonteCarlo):
         ml2p, parts = self.score_batch([pwd])
         return ml2p[0], parts[0]
 
+    @torch.no_grad()
     def score_batch(self, pwds: List[str]):
         pwds = list(pwds)
         ml2p: List[float] = []

@@ -116,6 +116,21 @@ def test_the_whole_flow_to_guess_numbers():
         prev = rank
 
 
+def test_the_model_is_asked_without_gradients():
+    asked = []
+
+    class Trained(Bigram):
+        def logits(self, tokens):
+            asked.append(torch.is_grad_enabled())
+            return super().logits(tokens)
+
+    m = Trained("abc", 2, max_len=3)
+    m.table.requires_grad_()
+    want = Bigram("abc", 2, max_len=3).score_batch(["ac", "a"])
+    assert m.score_batch(["ac", "a"]) == want and len(m.sample(5)) == 5
+    assert asked and not any(asked) and torch.is_grad_enabled()
+
+
 def test_a_model_that_leaves_nothing_is_an_error():
     m = Bigram("ab", 1)
     m.table[:] = -math.inf
