@@ -184,7 +184,7 @@ __global__ __launch_bounds__(BLOCK, !TOP ? 8 : NV > 5 ? 4 : 6) void k_logits_sco
 constexpr int CELL_ROWS = 16;  // cells of a thread
 constexpr u32 LIST_CAP = 256, CAND_CAP = 512;
 
-// A pass over the row keeps, beside its sums, the largest logit of every cell (one thread's vectors of some chunks) and of
+// A pass over the row keeps, beside its sums, the largest logit of every cell (one thread's vectors of `per_cell` chunks) and of
 // every thread.  The k-th largest of n groups of threads is a lower bound of the k-th largest of all (about n ln(n / (n - k))
 // logits of a random row reach it): only the cells that do are looked at again.
 template <int T>
@@ -344,6 +344,7 @@ struct Split {
     u32 shift, vecs;
     float4 *stats;  // [row][part]: m, s, e
     u64 *keys;      // [row][place][part]
+    u32 per_cell;   // chunks a cell
 };
 
 __device__ __forceinline__ void put_skipped(const ScoreOut &out, u32 row) {
@@ -394,7 +395,9 @@ __global__ __launch_bounds__(T, 8) void k_logits_score(Rows a, ScoreOut out, Spl
     const Span r = span_of<DT>(a, p);
     const float x = !PART && tok >= 0 ? element<DT>(p, tok) : 0.f;
     const u32 v0 = PART ? min(part * sp.vecs, r.nvec) : 0, v1 = PART ? min(r.nvec, v0 + sp.vecs) : r.nvec;
-    const u32 chunks = (v1 - v0 + T * UNROLL - 1) / (T * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
+    // (cells of as many chunks as the launch's LDS was counted with: a shorter last part, or a row without its first element, may
+    // have fewer chunks, and fewer chunks spread anew may need more rows of cells: 17 make 9, 16 make 16)
+    const u32 chunks = (v1 - v0 + T * UNROLL - 1) / (T * UNROLL), per_cell = sp.per_cell;
     Stat st{-INFINITY, 0.f, 0.f, false};
     float cell = -INFINITY;
     for (u32 ch = 0, in = 0, cr = 0; ch < chunks; ++ch) {
@@ -513,22 +516,23 @@ u32 split_vecs(u32 nvec, u32 shift) {
 
 size_t split_bytes(u32 rows, u32 shift, u32 top) { return shift ? ((size_t)rows << shift) * (16 + 8 * (size_t)top) : 0; }
 
-// bytes of the cells of workgroups of `threads` lanes over `vecs` vectors
-size_t cell_bytes(u32 vecs, u32 threads) {
-    const u32 chunks = (vecs + threads * UNROLL - 1) / (threads * UNROLL), per_cell = (chunks + CELL_ROWS - 1) / CELL_ROWS;
-    return (chunks + per_cell - 1) / per_cell * threads * sizeof(float);
-}
+// The cells of workgroups of `threads` lanes over at most `vecs` vectors: chunks a cell, bytes in all.
+u32 chunks_of(u32 vecs, u32 threads) { return (vecs + threads * UNROLL - 1) / (threads * UNROLL); }
+u32 cell_chunks(u32 vecs, u32 threads) { return (chunks_of(vecs, threads) + CELL_ROWS - 1) / CELL_ROWS; }
+size_t cell_bytes(u32 vecs, u32 threads, u32 per_cell) { return (chunks_of(vecs, threads) + per_cell - 1) / per_cell * threads * sizeof(float); }
 
 template <int DT, bool ENT, bool TOP>
 void launch(const Rows &a, const ScoreOut &out, Split sp, hipStream_t s) {
+    const u32 vecs = sp.shift ? sp.vecs : a.nvec, threads = !sp.shift && wide(a.rows, a.nvec) ? WIDE : BLOCK;
+    sp.per_cell = cell_chunks(vecs, threads);
+    const size_t cells = TOP ? cell_bytes(vecs, threads, sp.per_cell) : 0;
     if (sp.shift) {
-        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK),
-                           TOP ? cell_bytes(sp.vecs, BLOCK) : 0, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, true>), grid_of(a.rows << sp.shift), dim3(BLOCK), cells, s, a, out, sp);
         hipLaunchKernelGGL((k_logits_score_join<DT, ENT, TOP>), grid_of(a.rows), dim3(BLOCK), 0, s, a, out, sp);
-    } else if (!wide(a.rows, a.nvec)) {
-        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), TOP ? cell_bytes(a.nvec, BLOCK) : 0, s, a, out, sp);
+    } else if (threads == BLOCK) {
+        hipLaunchKernelGGL((k_logits_score<DT, BLOCK, ENT, TOP, false>), grid_of(a.rows), dim3(BLOCK), cells, s, a, out, sp);
     } else {
-        hipLaunchKernelGGL((k_logits_score<DT, WIDE, ENT, TOP, false>), grid_of(a.rows), dim3(WIDE), TOP ? cell_bytes(a.nvec, WIDE) : 0, s, a, out, sp);
+        hipLaunchKernelGGL((k_logits_score<DT, WIDE, ENT, TOP, false>), grid_of(a.rows), dim3(WIDE), cells, s, a, out, sp);
     }
 }
 
@@ -565,7 +569,7 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
                     else hipLaunchKernelGGL((k_logits_score_sub<DT, G, NV, false, false>), grid_of(rows_to_blocks(a.rows, G)), dim3(BLOCK), 0, s, a, out, 0u);
                 }));
     } else {
-        Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr};
+        Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr, 0};
         if (sp.shift) {
             if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift, top) || (uintptr_t)workspace % 16) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift, top), workspace_bytes);

@@ -702,3 +702,24 @@ def test_no_rows():
     assert lg.logits_gradient(x, t, w).grad.shape == (0, 5, 7)
     assert lg.logits_draw(x[:, 0], seed=1).tokens.shape == (0,)
     assert lg.logits_keys(w).shape == (0,)
+
+
+# ---- alternatives of rows whose parts, or vectors, are fewer than the launch's largest --------------------------------
+@pytest.mark.parametrize("vocab,rows,dtype,top", [(262208, 600, "bf16", 10), (262145, 512, "bf16", 5), (262208, 300, "fp32", 33), (262208, 600, "fp32", 8),
+                                                  (524289, 1024, "bf16", 5), (300001, 700, "fp16", 64)])
+def test_alternatives_of_shorter_last_parts(vocab, rows, dtype, top):
+    """The largest logits in a row's last part (17 chunks a part and 16 in the last one), in its first element and anywhere, every row
+    against a sort by logit and id."""
+    g = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    x = torch.randn(rows, vocab, generator=g, device="cuda").mul_(2.0).to(DTYPES[dtype])
+    at = torch.randint(vocab - vocab // 5, vocab, (rows, top // 2 + 1), generator=g, device="cuda")
+    x.scatter_(1, at, torch.rand(rows, top // 2 + 1, generator=g, device="cuda").mul_(4).add_(12).to(x.dtype))
+    x[::3, 0] = 14.0
+    x[::4] = torch.randn((rows + 3) // 4, vocab, generator=g, device="cuda").sub_(60.0).to(x.dtype)      # (no logit near 0)
+    r = lg.logits_score(x, torch.zeros(rows, dtype=torch.int64, device="cuda"), top=top)
+    order = torch.arange(vocab, 0, -1, device="cuda")
+    for i in range(0, rows, 64):
+        bits = (x[i:i + 64].float() + 0.0).view(torch.int32)
+        keys = (bits ^ ((bits >> 31) & 0x7FFFFFFF)).long() * (1 << 32) + order
+        want = torch.topk(keys, top, dim=-1).indices
+        assert torch.equal(r.top_tokens[i:i + 64].long(), want), i

@@ -169,3 +169,42 @@ def test_the_polynomial_of_the_draw():
         worst = max(worst, abs(p / (f * Decimal(2).ln()).exp() - 1))
     margin = float(re.search(r"MARGIN = ([0-9e.-]+);", src).group(1))
     assert worst < Decimal("4.1e-11") and margin >= 2 * float(worst)
+
+
+def test_the_cells_of_alternatives_fit_what_is_allocated():
+    """Rows of cells that k_logits_score writes (csrc/mc_logits_score.hip) against those its LDS is counted for, in whole numbers: of
+    every part of a row cut into parts, of whole rows, and of rows whose first element stays before their vectors."""
+    import os
+    import re
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "montecarlo_amd", "csrc", "mc_logits_score.hip")).read()
+    kernel = src[src.index("void k_logits_score(Rows a"):src.index("// the parts of a row joined")]
+    # the kernel fills cells of as many chunks as the host counted: it does not spread its own chunks anew
+    assert re.search(r"per_cell = sp\.per_cell;", kernel) and "CELL_ROWS" not in kernel
+
+    def up(a, b):
+        return -(-a // b)
+
+    def cells(vecs, lanes):                                # cell_chunks, cell_bytes
+        per_cell = up(up(vecs, 4 * lanes), 16)
+        return per_cell, up(up(vecs, 4 * lanes), per_cell)
+
+    rng = np.random.default_rng(5)
+    vocabs = [16384 * 8 * k + d for k in range(1, 9) for d in (-9, -1, 0, 1, 2, 64, 4097)] + [262208, 262145, 524289, 1 << 20, (1 << 31) - 65]
+    vocabs += np.exp(rng.uniform(math.log(4097), math.log(3e6), 400)).astype(int).tolist()
+    for vocab in vocabs:
+        for rows in (1, 3, 25, 256, 257, 300, 512, 600, 1023, 1024, 4096):
+            for size in (2, 4):
+                per = 16 // size
+                nvec, shift = up(vocab, per), 0
+                while vocab > 160000 and shift < 6 and (rows << shift) < 1024 and (nvec >> (shift + 1)) >= 1024:
+                    shift += 1
+                for mine in {nvec, up(vocab - 1, per) if size == 2 else nvec}:
+                    if shift:
+                        vecs = up(up(nvec, 1 << shift), 1024) * 1024
+                        per_cell, room = cells(vecs, 256)
+                        used = [up(up(max(0, min(mine, (p + 1) * vecs) - p * vecs), 1024), per_cell) for p in range(1 << shift)]
+                    else:
+                        lanes = 1024 if nvec >= 16384 or (rows <= 256 and nvec >= 2048) else 256
+                        per_cell, room = cells(nvec, lanes)
+                        used = [up(up(mine, 4 * lanes), per_cell)]
+                    assert max(used) <= room <= 16, (vocab, rows, size, used, room)
