@@ -554,7 +554,7 @@ int mc_rank_query(const double *keys_sorted, const double *positions, uint64_t n
  * Rows: logits[o][i][0..vocab) of MC_LOGITS_F32 / _F16 / _BF16, row o * inner + i at o * outer_stride + i * inner_stride
  * ELEMENTS, consecutive tokens adjacent; any strides (a slice of a longer sequence, rows that overlap or repeat), any
  * alignment of the element's own.  Tokens and weights come with strides of their own for the same (outer, inner); outputs
- * are contiguous [outer * inner].  Sums are held in 32 bits (the draw decides in 64).  All calls are asynchronous on
+ * are contiguous [outer * inner].  Sums are held in 32 bits (the draw decides in 64); -log2 p and entropies are never below 0.  All calls are asynchronous on
  * `stream`, allocate nothing and may be captured into a graph.  A workspace (16-byte aligned, mc_logits_*_workspace_bytes;
  * NULL where that is 0) holds nothing between calls, but calls that may overlap need one each.  Temperatures 1e-30 .. 1e30.
  *   token ids   0 .. vocab - 1; MC_TOKEN_SKIP: the row is not read (padding), its outputs are 0; anything else is a token
@@ -600,9 +600,10 @@ int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows, uint64_t v
                    const uint8_t *live, int32_t *out_token, float *out_ml2p, void *workspace, size_t workspace_bytes,
                    void *stream);
 /* -log2 p of whole passwords, the keys of mc_rank_build: the sum in 64 bits of a password's ml2p; 1022.0 where one of
- * them is +inf (as mc_score), 0.0 for no symbols.  Packed: password t is ml2p[offsets[t] .. offsets[t+1]) of `longest`
- * values in all (a pair of offsets that does not ascend within them names nothing).  Padded (offsets NULL):
- * ml2p[t * stride + 0 .. lengths[t]), lengths of 4 or 8 bytes cut to 0 .. longest, or NULL: `longest` each. */
+ * them is +inf (as mc_score; finite sums are not cut), 0.0 for no symbols and where the sum is below 0 (the rank indexes
+ * take non-negative keys).  Packed: password t is ml2p[offsets[t] .. offsets[t+1]) of `longest` values in all (a pair of
+ * offsets that does not ascend within them names nothing).  Padded (offsets NULL): ml2p[t * stride + 0 .. lengths[t]),
+ * lengths of 4 or 8 bytes cut to 0 .. longest, or NULL: `longest` each. */
 int mc_logits_keys(const float *ml2p, const int64_t *offsets, const void *lengths, uint32_t length_bytes,
                    uint64_t count, int64_t stride, uint64_t longest, double *out_keys, void *stream);
 

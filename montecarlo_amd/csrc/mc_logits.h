@@ -238,15 +238,19 @@ struct Expo {
 // whether a row's fast sums do not stand
 __device__ __forceinline__ bool doubtful(float m, float c) { return fabsf(m) < INFINITY && fabsf(m * c) > FAR; }
 
+// A -log2 p or an entropy as it is put.  A token of probability 1 has log2 Z = y but for the roundings of a power and a logarithm,
+// which may leave a few 2^-24 on either side of 0; keys are sorted by their bits, where a negative one would come last of all.
+__device__ __forceinline__ float at_least_0(float v) { return maximum(v, 0.f); }
+
 // what a row's statistics say about its token
 __device__ __forceinline__ float ml2p_of(int tok, const Stat &st, float x, float c) {
     if (tok == MC_TOKEN_SKIP) return 0.f;
     if (!(st.s == st.s)) return st.s;
-    return tok >= 0 && st.s > 0.f ? log2_(st.s) - Expo(st, c)(x) : INFINITY;
+    return tok >= 0 && st.s > 0.f ? at_least_0(log2_(st.s) - Expo(st, c)(x)) : INFINITY;
 }
 
 __device__ __forceinline__ float entropy_of(int tok, const Stat &st) {
-    return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : log2_(st.s) - st.e * inverse(st.s);
+    return tok == MC_TOKEN_SKIP || st.s == 0.f ? 0.f : at_least_0(log2_(st.s) - st.e * inverse(st.s));
 }
 
 // ---- reductions over groups of lanes and over workgroups ---------------------------------------------------------------

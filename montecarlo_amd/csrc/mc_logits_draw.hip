@@ -68,7 +68,7 @@ __device__ __forceinline__ float no_draw(float m) { return m == -INFINITY ? INFI
 __device__ __forceinline__ float ml2p_under(double z, double y) {
     int e;
     const double m = frexp(z, &e);
-    return (float)(((double)e - y) + (double)log2f((float)m));
+    return at_least_0((float)(((double)e - y) + (double)log2f((float)m)));
 }
 
 struct DrawArgs {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
         const bool mine = draw_fast<DT, G>(r, y_of, u, d.margin, token, x, st.s) && !doubtful(m, a.c);
         if (mine) {
             d.token[row] = (int)token;
-            d.ml2p[row] = log2_(st.s) - y_of.fast(x);
+            d.ml2p[row] = at_least_0(log2_(st.s) - y_of.fast(x));
         }
         st.exact = group_sum<G>(mine) == 0;  // still open
     } else if (there && lane == 0) {
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
             }
             if (sure) {
                 d.token[row] = (int)token;
-                d.ml2p[row] = log2_((float)z) - y_of.fast(x);
+                d.ml2p[row] = at_least_0(log2_((float)z) - y_of.fast(x));
                 done = 1;
             }
         }
@@ -791,7 +791,8 @@ struct KeyArgs {
     double *out;
 };
 
-__device__ __forceinline__ double key_of(double sum) { return sum == INFINITY ? 1022.0 : sum; }
+// (not below 0, which rank indexes would put last: the caller's own values of certain tokens may be off by a rounding)
+__device__ __forceinline__ double key_of(double sum) { return sum == INFINITY ? 1022.0 : sum <= 0. ? 0. : sum; }
 
 // Password i's values p[0 .. n).  (Offsets that do not ascend or leave the array name none: nothing is read through them.)
 __device__ __forceinline__ u64 values_of(const KeyArgs &k, u64 i, u64 &from) {

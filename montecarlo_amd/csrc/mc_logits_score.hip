@@ -37,7 +37,7 @@ __device__ __forceinline__ u32 index_of(u64 key) { return 0xFFFFFFFFu - (u32)key
 
 // one alternative's outputs
 __device__ __forceinline__ void put_top(const ScoreOut &out, u32 row, u32 rank, u64 key, const Stat &st, float lz, float c) {
-    const float v = lz - Expo(st, c)(value_of((u32)(key >> 32)));
+    const float v = at_least_0(lz - Expo(st, c)(value_of((u32)(key >> 32))));
     out.top[(u64)row * out.k + rank] = v < INFINITY ? (int)index_of(key) : MC_TOKEN_OUTSIDE;
     out.top_ml2p[(u64)row * out.k + rank] = v < INFINITY ? v : INFINITY;
 }

@@ -723,3 +723,55 @@ def test_alternatives_of_shorter_last_parts(vocab, rows, dtype, top):
         keys = (bits ^ ((bits >> 31) & 0x7FFFFFFF)).long() * (1 << 32) + order
         want = torch.topk(keys, top, dim=-1).indices
         assert torch.equal(r.top_tokens[i:i + 64].long(), want), i
+
+
+# ---- nothing is below 0 ------------------------------------------------------------------------------------------------
+def not_negative(t, most=None):
+    """No sign bit anywhere (rank indexes sort the bits), and at most `most` where that is given."""
+    bits = t.contiguous().view(torch.int64 if t.dtype == torch.float64 else torch.int32)
+    assert bool((bits >= 0).all()), t[t.view(-1) < 0][:5] if t.dim() == 1 else t.min()
+    assert most is None or t.max().item() <= most
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("vocab,rows", [(1, 900), (5, 900), (97, 900), (97, 20000), (700, 900), (3001, 900), (9001, 900), (20001, 600), (20001, 9), (66001, 600),
+                                        (140001, 520), (200003, 9)])
+def test_certain_tokens_score_0_and_never_less(vocab, rows, dtype):
+    """Rows with one token left and rows whose others are 30 below it, at many logits and temperatures: -log2 p and entropy are 0 or
+    a rounding above it.  (A power and a logarithm of a number in (1/2, 1], off by a step of 2^-23 of their value each: below 2^-21;
+    `vocab` others of 2^-43 add no more than 2^-24.)"""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    at = torch.arange(rows, device="cuda") * 7 % vocab
+    value = torch.linspace(-100, 100, rows, device="cuda")
+    x = torch.full((rows, vocab), -math.inf, device="cuda")
+    x.scatter_(1, at[:, None], value[:, None])
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64) * 0.999
+    w = torch.rand(rows, generator=g, device="cuda")
+    for others in (False, True):
+        if others:
+            x = torch.where(x == -math.inf, value[:, None] - 30.5, x)
+        xs = x.to(DTYPES[dtype])
+        for t in (1.0, 0.7, 0.05) if others else (1.0, 0.02, 0.7, 3.1, 40.0):
+            r = lg.logits_score(xs, at, temperature=t, entropy=True, top=1)
+            # (30 below it in bits of 1.44 / T: the others together are below vocab * 2^-43 of the row, their entropy 45 times that)
+            most = 2.0 ** -21 + vocab * 2.0 ** -43 * 45 * others
+            for v in (r.ml2p, r.entropy, r.top_ml2p.view(-1), lg.logits_score(xs, at, temperature=t).ml2p):
+                not_negative(v, most)
+            assert torch.equal(r.top_tokens[:, 0].long(), at)
+            gr = lg.logits_gradient(xs, at, w, entropy_weights=w, temperature=t)
+            not_negative(gr.ml2p, most)
+            not_negative(gr.entropy, most)
+            d = lg.logits_draw(xs, u, temperature=t)
+            assert torch.equal(d.tokens.long(), at) or others
+            not_negative(d.ml2p)
+            not_negative(d.ml2p[d.tokens == at], most)
+
+
+def test_keys_are_never_below_0():
+    m = torch.tensor([[-6e-8, 3e-8, 0.0], [-0.0, -0.0, -0.0], [-6e-8, 1.0, 0.0], [-1e-7, math.inf, 0.0], [-1e-7, math.nan, 0.0]]).cuda()
+    off = torch.arange(0, 16, 3).cuda()
+    many = m[:3].repeat(2000, 1)
+    for got in (lg.logits_keys(m), lg.logits_keys(m.view(-1), offsets=off)):
+        not_negative(got[:4])
+        assert got[:2].tolist() == [0.0, 0.0] and got[2].item() == 1.0 + float(m[2, 0]) and got[3].item() == 1022.0 and math.isnan(got[4].item())
+    not_negative(lg.logits_keys(many.view(-1), offsets=torch.arange(0, 18001, 3).cuda()))

@@ -159,3 +159,30 @@ def test_a_model_learns_its_corpus():
     x.backward(lg.logits_gradient(x, tokens, w).grad)
     # sums of at most 18 gradients, each off by its bound (p and the roundings of p - 1)
     assert table.grad.abs().max().item() <= 18 * 2.0 ** -24 * (steps_of(v) + 8) / int((tokens >= 0).sum())
+
+
+def test_passwords_that_are_certain_keep_their_place():
+    """A sharpened model whose commonest password is certain up to a rounding at every place: keys are 0 or above, and guess numbers of
+    all passwords are those of 64 bits on the same keys."""
+    m = Bigram("abcdef", 7, max_len=8, temperature=0.02)
+    m.table[:] = -9.0
+    v = len(m.vocabulary)
+    g = torch.Generator().manual_seed(1)
+    m.table[:, :] += torch.rand(v + 1, v, generator=g).to(m.table)
+    for a, b in ((v, 0), (0, 2), (2, 3), (3, 4), (4, m.end)):         # "acde", each step far above the others
+        m.table[a, b] = 5.0 + 0.37 * a
+    m.seed(2)
+    keys = m.sample(5000)
+    raw = np.array(keys.tolist())
+    assert raw.min() >= 0 and not np.signbit(raw).any() and (raw < 1e-5).all()
+    assert m.sample1()[1] == "acde" and 0 <= m.calc_ml2p("acde")[0] < 1e-5
+    # certain ones among others (continuations that were forced): the index of all of them in order
+    other = Bigram("abcdef", 8, max_len=8)
+    other.seed(3)
+    mixed = torch.cat([keys.tensor, other.sample(3000).tensor])[torch.randperm(8000, generator=g).to(m.device)]
+    srt = np.sort(mixed.cpu().numpy())
+    pos = np.cumsum(2.0 ** (srt - math.log2(8000)))
+    mc = MonteCarloLib(mixed.clone())
+    for x in [0.0, 1e-7, float(srt[2500]), float(srt[4999]), 0.5, float(srt[6000]), float(srt[7999])]:
+        i = int(np.searchsorted(srt, x, side="right"))
+        assert abs(mc.ml2p2rank(x) - (pos[i - 1] if i else 1)) <= 1e-9 * pos[-1], x
