@@ -226,13 +226,17 @@ __device__ __forceinline__ float scaled(float m, float c) { return ceilf(fmaxf(m
 // s 2^d for a whole number d
 __device__ __forceinline__ float times2(float s, float d) { return __builtin_amdgcn_ldexpf(s, (int)d); }
 
+// The exponent (x - m) c of a logit below the largest one, by halves: two logits of 32 bits may lie further apart than their type
+// reaches, where the exponent does not (halves of such logits are exact; c is below 2^101).
+__device__ __forceinline__ float below(float x, float m, float c) { return __builtin_fmaf(x, 0.5f, -0.5f * m) * (c + c); }
+
 // the exponent of a logit under a row's statistics
 struct Expo {
     float m, c, M;
     bool exact;
     __device__ __forceinline__ Expo(const Stat &st, float c_) : m(fmaxf(st.m, LOWEST)), c(c_), M(scaled(st.m, c_)), exact(st.exact) {}
     __device__ __forceinline__ float fast(float x) const { return __builtin_fmaf(x, c, -M); }
-    __device__ __forceinline__ float operator()(float x) const { return exact ? (x - m) * c : fast(x); }
+    __device__ __forceinline__ float operator()(float x) const { return exact ? below(x, m, c) : fast(x); }
 };
 
 // whether a row's fast sums do not stand
@@ -492,7 +496,7 @@ __device__ __forceinline__ Stat sub_sums(const SubRow<DT, NV> &r, float m, float
     for (int i = 0; i < SubRow<DT, NV>::N; ++i) {
 #pragma unroll
         for (int j = 0; j < VEC<DT>; ++j) {
-            const float x = unpack<DT>(vec_of(r, i), j), y = EXACT ? (x - y_of.m) * c : y_of.fast(x), w = exp2_(y);
+            const float x = unpack<DT>(vec_of(r, i), j), y = EXACT ? below(x, y_of.m, c) : y_of.fast(x), w = exp2_(y);
             st.s += w;
             if (ENT) st.e = __builtin_fmaf(w, fmaxf(y, -FAR), st.e);
         }
@@ -586,7 +590,7 @@ template <int DT, int T, bool ENT>
 __device__ __forceinline__ Stat exact_stat(const Span &r, float c, float m) {
     Stat st{m, 0.f, 0.f, true};
     const auto add = [&](float x) {
-        const float y = (x - m) * c, w = exp2_(y);
+        const float y = below(x, m, c), w = exp2_(y);
         st.s += w;
         st.e += w * fmaxf(y, -FAR);
     };

@@ -775,3 +775,22 @@ def test_keys_are_never_below_0():
         not_negative(got[:4])
         assert got[:2].tolist() == [0.0, 0.0] and got[2].item() == 1.0 + float(m[2, 0]) and got[3].item() == 1022.0 and math.isnan(got[4].item())
     not_negative(lg.logits_keys(many.view(-1), offsets=torch.arange(0, 18001, 3).cuda()))
+
+
+@pytest.mark.parametrize("temperature", [1e30, 1e29, 1e10])
+@pytest.mark.parametrize("vocab,rows", [(5, 7), (97, 3000), (700, 7), (9001, 7), (9001, 600), (200003, 3)])
+def test_logits_further_apart_than_the_type_reaches(vocab, rows, temperature):
+    """The difference of two float32 logits may pass the largest float32 number where the exponent that it stands for does not."""
+    x = make(rows, vocab, torch.float32, vocab)
+    for i, (hi, lo) in enumerate([(3e38, -3e38), (3.4e38, -3.4e38), (2e38, -2.5e38)]):
+        x[2 * i % rows] = torch.where(torch.arange(vocab) % 3 == i % 3, hi, lo)
+    some = list(range(min(rows, 7)))
+    toks = torch.arange(rows) % vocab
+    g = torch.Generator().manual_seed(vocab)
+    w, u = torch.rand(rows, generator=g), torch.rand(rows, generator=g, dtype=torch.float64)
+    r = lg.logits_score(x.cuda(), toks.cuda(), temperature=temperature, entropy=True, top=min(4, vocab))
+    check_score(x[some], toks[some], lg.LogitScores(*(t[some] for t in r)), temperature, min(4, vocab))
+    gr = lg.logits_gradient(x.cuda(), toks.cuda(), w.cuda(), entropy_weights=w.cuda(), temperature=temperature)
+    check_gradient(x[some], toks[some], w[some], w[some], lg.LogitGradient(*(t[some] for t in gr)), temperature, "fp32")
+    d = lg.logits_draw(x.cuda(), u.cuda(), temperature=temperature)
+    check_draw(x[some], u[some], None, lg.LogitDraws(d.tokens[some], d.ml2p[some]), temperature)
