@@ -71,6 +71,18 @@ __device__ __forceinline__ float ml2p_under(double z, double y) {
     return at_least_0((float)(((double)e - y) + (double)log2f((float)m)));
 }
 
+// What a row's tokens score under the sums that it began with: a token comes with one value, whether its uniform was
+// decided by these sums or, beside the border of an interval, by those of a later pass.
+struct Under64 {
+    double z, m, c;
+    __device__ __forceinline__ float operator()(float x) const { return ml2p_under(z, ((double)x - m) * c); }
+};
+struct Under32 {
+    float lz;  // log2 Z
+    Expo y_of;
+    __device__ __forceinline__ float operator()(float x) const { return at_least_0(lz - y_of.fast(x)); }
+};
+
 struct DrawArgs {
     const double *uniforms;  // or null: Philox
     u64 seed, first_id;
@@ -232,7 +244,7 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
         const bool mine = draw_fast<DT, G>(r, y_of, u, d.margin, token, x, st.s) && !doubtful(m, a.c);
         if (mine) {
             d.token[row] = (int)token;
-            d.ml2p[row] = at_least_0(log2_(st.s) - y_of.fast(x));
+            d.ml2p[row] = Under32{log2_(st.s), y_of}(x);
         }
         st.exact = group_sum<G>(mine) == 0;  // still open
     } else if (there && lane == 0) {
@@ -254,7 +266,7 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
         }
         if (open && lane == 0) {
             d.token[row] = (int)token;
-            d.ml2p[row] = ml2p_under(z, ((double)x - (double)m) * d.power.c);
+            d.ml2p[row] = doubtful(m, a.c) ? Under64{z, (double)m, d.power.c}(x) : Under32{log2_(st.s), y_of}(x);
         }
     }
 }
@@ -266,7 +278,7 @@ constexpr int WIDE = 512, WIDE_WAVES = WIDE / 64, STEPS = 4;
 // holds the token (true there) looks for it, first by steps of 4 x 64 tokens.  Where sums that are right to 1e-10 leave it open:
 // one row of 131072 in 40000, which took a single wave 1.8 ms.
 template <int DT, int T>
-__device__ __forceinline__ bool draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token, float &x, double &z) {
+__device__ __forceinline__ bool draw_exact(const char *p, const Rows &a, const Definition &weight, double u, u32 &token, float &x) {
     constexpr int WAVES = T / 64;
     constexpr u32 STEP = 4 * 64;
     __shared__ double part[WAVES];
@@ -291,8 +303,7 @@ __device__ __forceinline__ bool draw_exact(const char *p, const Rows &a, const D
     if (lane == 0) part[wave] = s;
     __syncthreads();
     const double inc = group_scan<64>(lane < (u32)WAVES ? part[lane] : 0.);
-    z = __shfl(inc, 63);
-    const double target = u * z;
+    const double target = u * __shfl(inc, 63);
     const u64 passes = __ballot(inc > target);
     const u32 who = passes ? (u32)__ffsll((unsigned long long)passes) - 1 : WAVES - 1;
     if (wave != who) return false;
@@ -452,10 +463,10 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
 
 // A row of which lane i holds the sum of part i of `share` vectors: its token, by one wave; false where its outputs are still to
 // be put.  `within` (if by_shares): the same for the PART_WAVES shares of the lane's part.  (Sums of Power are those of PowerBelow
-// for m = 0 but for roundings far below the margin.)
-template <int DT>
+// for m = 0 but for roundings far below the margin.)  `value`: what a token scores.
+template <int DT, typename V>
 __device__ __forceinline__ bool put_token(const DrawArgs &d, u32 row, const Span &r, const PowerBelow &weight, double mine, u32 share, double u,
-                                          bool by_shares, const double (&within)[PART_WAVES]) {
+                                          bool by_shares, const double (&within)[PART_WAVES], const V &value) {
     const double inc = group_scan<64>(mine), z = __shfl(inc, 63), target = u * z;
     const u64 passes = __ballot(inc > target);
     if (!passes) return false;
@@ -478,20 +489,19 @@ __device__ __forceinline__ bool put_token(const DrawArgs &d, u32 row, const Span
     if (!locate<DT>(r, weight, min(v0, r.nvec), min(r.nvec, v1), before, target, MARGIN * z, token, x)) return false;
     if ((threadIdx.x & 63) == 0) {
         d.token[row] = (int)token;
-        d.ml2p[row] = ml2p_under(z, ((double)x - weight.m) * d.power.c);
+        d.ml2p[row] = value(x);
     }
     return true;
 }
 
 // the same by the definition, by the workgroup
-template <int DT, int T>
-__device__ __forceinline__ void put_exact(const Rows &a, const DrawArgs &d, u32 row, const char *p, float m, double u) {
+template <int DT, int T, typename V>
+__device__ __forceinline__ void put_exact(const Rows &a, const DrawArgs &d, u32 row, const char *p, float m, double u, const V &value) {
     u32 token;
     float x = m;
-    double z;
-    if (draw_exact<DT, T>(p, a, Definition{d.t, (double)m}, u, token, x, z) && (threadIdx.x & 63) == 0) {
+    if (draw_exact<DT, T>(p, a, Definition{d.t, (double)m}, u, token, x) && (threadIdx.x & 63) == 0) {
         d.token[row] = (int)token;
-        d.ml2p[row] = ml2p_under(z, ((double)x - (double)m) * d.power.c);
+        d.ml2p[row] = value(x);
     }
 }
 
@@ -539,14 +549,15 @@ __global__ __launch_bounds__(WIDE, 4) void k_logits_draw(Rows a, DrawArgs d) {
         if (lane == 0) ps[wave] = s;  // (nobody has read the first ones)
         __syncthreads();
     }
-    const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum);
-    const u64 passes = __ballot(inc > u * __shfl(inc, 63));
+    const double part_sum = lane < WIDE_WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), z = __shfl(inc, 63);
+    const u64 passes = __ballot(inc > u * z);
+    const Under64 value{z, weight.m, d.power.c};
     if (wave == (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) {
         const double none[PART_WAVES] = {};
-        if (put_token<DT>(d, row, r, weight, part_sum, share, u, false, none)) done = 1;
+        if (put_token<DT>(d, row, r, weight, part_sum, share, u, false, none, value)) done = 1;
     }
     __syncthreads();
-    if (!done) put_exact<DT, WIDE>(a, d, row, p, m, u);
+    if (!done) put_exact<DT, WIDE>(a, d, row, p, m, u, value);
 }
 
 // One workgroup a row, in 32 bits first, the row in the registers of T lanes, HELD vectors each at most: what decides it is not
@@ -620,10 +631,12 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
         }
         return;
     }
+    float lz = 0.f;  // log2 of the row's sum in 32 bits (one value for all waves)
     if (!doubtful(m, a.c)) {
         const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
         const double w = __builtin_ldexp(ps[of], (int)(scaled(pm[of], a.c) - y_of.M)), inc = group_scan<WAVES>(w), z = __shfl(inc, WAVES - 1);
         const double target = u * z;
+        lz = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(log2_((float)z))));
         const float near = (float)(d.margin * z);
         const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WAVES) - 1));
         if (wave == part) {
@@ -662,7 +675,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
             }
             if (sure) {
                 d.token[row] = (int)token;
-                d.ml2p[row] = at_least_0(log2_((float)z) - y_of.fast(x));
+                d.ml2p[row] = Under32{lz, y_of}(x);
                 done = 1;
             }
         }
@@ -684,20 +697,24 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
     __syncthreads();  // (every wave has read the first ones)
     if (lane == 0) ps[wave] = sum;
     __syncthreads();
-    const double part_sum = lane < (u32)WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum);
-    const u64 passes = __ballot(inc > u * __shfl(inc, 63));
+    const double part_sum = lane < (u32)WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), z = __shfl(inc, 63);
+    const u64 passes = __ballot(inc > u * z);
+    const auto value = [&](float x) {
+        return doubtful(m, a.c) ? Under64{z, (double)m, d.power.c}(x) : Under32{lz, Expo(Stat{m, 0.f, 0.f, false}, a.c)}(x);
+    };
     if (wave == (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) {
         const double none[PART_WAVES] = {};
-        if (put_token<DT>(d, row, r, weight, part_sum, nv * 64, u, false, none)) done = 1;
+        if (put_token<DT>(d, row, r, weight, part_sum, nv * 64, u, false, none, value)) done = 1;
     }
     __syncthreads();
-    if (!done) put_exact<DT, T>(a, d, row, p, m, u);
+    if (!done) put_exact<DT, T>(a, d, row, p, m, u, value);
 }
 
 // The parts of a row joined, by the workgroup's first wave; the others help where it leaves the token open.
 template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_logits_draw_join(Rows a, DrawArgs d, Split sp) {
     __shared__ int done;
+    __shared__ double total;
     const u32 row = block_id(), lane = threadIdx.x & 63;
     if (row >= a.rows) return;
     if (d.live && !d.live[row]) {
@@ -726,19 +743,23 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_join(Rows a, DrawArgs d, 
         }
         return;
     }
+    const bool suits = good(m, d.power.c);
+    const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
     if (threadIdx.x < 64) {
-        const bool suits = good(m, d.power.c);
-        const PowerBelow weight{d.power.c, suits ? 0. : (double)m};
         if (!suits) {
             float unused;
             sum_vecs<DT, UNROLL>(r, weight, 0, r.nvec, lane, mine, unused);
             if (lane) mine = 0.;
         }
-        const bool sure = put_token<DT>(d, row, r, weight, mine, suits ? sp.vecs : r.nvec, u, suits, within);
-        if (lane == 0) done = sure;
+        const double z = __shfl(group_scan<64>(mine), 63);
+        const bool sure = put_token<DT>(d, row, r, weight, mine, suits ? sp.vecs : r.nvec, u, suits, within, Under64{z, weight.m, d.power.c});
+        if (lane == 0) {
+            done = sure;
+            total = z;
+        }
     }
     __syncthreads();
-    if (!done) put_exact<DT, BLOCK>(a, d, row, p, m, u);
+    if (!done) put_exact<DT, BLOCK>(a, d, row, p, m, u, Under64{total, weight.m, d.power.c});
 }
 
 // Rows begin with 64 bits where 32 would leave too many open: from 128 KB on (of 4-byte logits, which 64 bits keep up with: 2048

@@ -408,6 +408,28 @@ def test_draw_frequencies():
     assert (n.cpu() - torch.tensor([1 / 8, 2 / 8, 0, 5 / 8])).abs().max() < 5 * math.sqrt(0.25 / 80000)
 
 
+@pytest.mark.parametrize("rows", [700, 40])
+@pytest.mark.parametrize("vocab,dtype,temperature", [(5, "fp32", 1.0), (97, "bf16", 1.0), (97, "fp32", 1e-4), (600, "fp16", 0.7), (4099, "fp16", 1.0), (20001, "bf16", 1.0),
+                                                     (20001, "fp32", 1e-4), (66001, "bf16", 1.0), (33001, "fp32", 1.0), (140001, "fp16", 1.0), (140001, "fp32", 1e-3)])
+def test_a_drawn_token_comes_with_one_value_whatever_its_uniform(vocab, dtype, rows, temperature):
+    """The -log2 p of a token is that of the row, not that of the way its uniform was decided on (32 bits, 64, the definition): equal
+    samples have equal keys."""
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.randn(vocab, generator=g) * 2).to(DTYPES[dtype])
+    x[::max(2, vocab // 9)] = x.max() + 3                   # ten tokens that hold half of the row or more
+    c = np.cumsum(np.exp((x.double().numpy() - x.double().max().item()) / temperature))
+    c /= c[-1]
+    top = np.nonzero(np.diff(c, prepend=0.0) > 0.02)[0][:6]
+    assert len(top) >= 2
+    us = np.concatenate([[c[at] - d for d in (1.5e-11, 8e-11, 2e-8, 3e-7, 1e-4, 1e-3)] for at in top])
+    us = np.clip(np.concatenate([us, np.linspace(0, 1, rows, endpoint=False)])[:rows], 0, 1 - 2.0 ** -53)
+    d = lg.logits_draw(x.cuda().expand(rows, vocab), torch.from_numpy(us).cuda(), temperature=temperature)
+    toks, bits = d.tokens.cpu().numpy(), d.ml2p.cpu().numpy().view(np.int32)
+    for t in top:
+        mine = bits[toks == t]
+        assert len(mine) >= 6 and len(set(mine.tolist())) == 1, (t, len(mine), sorted(set(d.ml2p.cpu().numpy()[toks == t].tolist())))
+
+
 # ---- keys ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("batch,length", [(1, 0), (1, 1), (3, 5), (257, 24), (1000, 1), (65, 300), (70001, 9), (2, 40000)])
 def test_keys(batch, length):
