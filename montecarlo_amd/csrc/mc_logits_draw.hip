@@ -253,6 +253,10 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
     }
     const bool open = st.exact;
     if (__ballot(open)) {  // the whole wave decides again, in 64 bits
+        // (what the row's tokens score under waits in LDS: its registers, across what follows, cost all waves one of seven a SIMD)
+        __shared__ float2 sums[BLOCK];
+        sums[threadIdx.x] = make_float2(st.s, y_of.M);
+        asm volatile("" ::: "memory");
         forget(r);
         double z;
         bool now = draw_sub<DT, G>(r, PowerBelow{d.power.c, (double)m}, u, MARGIN, token, x, z);
@@ -266,7 +270,10 @@ __global__ __launch_bounds__(BLOCK, NV > 5 ? 4 : 6) void k_logits_draw_sub(Rows 
         }
         if (open && lane == 0) {
             d.token[row] = (int)token;
-            d.ml2p[row] = doubtful(m, a.c) ? Under64{z, (double)m, d.power.c}(x) : Under32{log2_(st.s), y_of}(x);
+            const float2 sum = sums[threadIdx.x];
+            Expo again = y_of;
+            again.M = sum.y;
+            d.ml2p[row] = doubtful(m, a.c) ? Under64{z, (double)m, d.power.c}(x) : Under32{log2_(sum.x), again}(x);
         }
     }
 }
