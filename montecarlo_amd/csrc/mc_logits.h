@@ -223,8 +223,9 @@ struct Stat {
 
 __device__ __forceinline__ float scaled(float m, float c) { return ceilf(fmaxf(m * c, -FAR)); }
 
-// s 2^d for a whole number d
-__device__ __forceinline__ float times2(float s, float d) { return __builtin_amdgcn_ldexpf(s, (int)d); }
+// s 2^d for a whole number d (between -2^16 and 0 in rows whose sums stand; beside a NaN, a +inf or a maximum whose scaled value
+// overflows it may be anything, which no conversion to a whole number is defined for: kept within 2^17, NaN included)
+__device__ __forceinline__ float times2(float s, float d) { return __builtin_amdgcn_ldexpf(s, (int)__builtin_amdgcn_fmed3f(d, -131072.f, 131072.f)); }
 
 // The exponent (x - m) c of a logit below the largest one, by halves: two logits of 32 bits may lie further apart than their type
 // reaches, where the exponent does not (halves of such logits are exact; c is below 2^101).

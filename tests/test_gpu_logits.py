@@ -816,3 +816,24 @@ def test_logits_further_apart_than_the_type_reaches(vocab, rows, temperature):
     check_gradient(x[some], toks[some], w[some], w[some], lg.LogitGradient(*(t[some] for t in gr)), temperature, "fp32")
     d = lg.logits_draw(x.cuda(), u.cuda(), temperature=temperature)
     check_draw(x[some], u[some], None, lg.LogitDraws(d.tokens[some], d.ml2p[some]), temperature)
+
+
+@pytest.mark.parametrize("vocab,rows", [(5, 9), (97, 300), (700, 9), (3001, 40), (9001, 40), (20001, 600), (200003, 9)])
+def test_nan_and_infinities_beside_each_other(vocab, rows):
+    """+inf, -inf and NaN in one row, in either order and beside logits whose scaled values overflow: NaN, and no token."""
+    x = torch.zeros(rows, vocab)
+    for i in range(min(rows, 9)):
+        first, second = [(math.inf, math.nan), (math.nan, math.inf), (3e38, math.nan), (math.nan, 3e38), (-math.inf, math.nan), (math.inf, math.inf),
+                         (math.inf, -math.inf), (3e38, math.inf), (math.inf, 3e38)][i]
+        x[i, 0], x[i, vocab - 1] = first, second
+    toks = torch.arange(rows) % vocab
+    w, u = torch.ones(rows), torch.full((rows,), 0.25, dtype=torch.float64)
+    for t in (1.0, 1e-5):
+        r = lg.logits_score(x.cuda(), toks.cuda(), temperature=t, entropy=True, top=2)
+        g = lg.logits_gradient(x.cuda(), toks.cuda(), w.cuda(), entropy_weights=w.cuda(), temperature=t)
+        d = lg.logits_draw(x.cuda(), u.cuda(), temperature=t)
+        n = min(rows, 9)
+        for v in (r.ml2p, r.entropy, r.top_ml2p[:, 0], g.ml2p, g.entropy, d.ml2p):
+            assert bool(v[:n].isnan().all()) and not bool(v[n:].isnan().any())
+        assert bool((r.top_tokens[:n] == OUTSIDE).all()) and bool((d.tokens[:n] == OUTSIDE).all())
+        assert bool(g.grad[:n].isnan().all()) and bool(torch.isfinite(g.grad[n:]).all())
