@@ -574,7 +574,8 @@ template <int DT, int T, int HELD>
 __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a, DrawArgs d) {
     constexpr int WAVES = T / 64;
     __shared__ float pm[WAVES];
-    __shared__ double ps[WAVES];
+    __shared__ double ps[WAVES], under64[WAVES];  // (what the tokens score under: every wave's own copy, in no register meanwhile)
+    __shared__ float2 under32[WAVES];
     __shared__ int done;
     const u32 row = block_id(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (row >= a.rows) return;
@@ -638,12 +639,11 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
         }
         return;
     }
-    float lz = 0.f;  // log2 of the row's sum in 32 bits (one value for all waves)
     if (!doubtful(m, a.c)) {
         const Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
         const double w = __builtin_ldexp(ps[of], (int)(scaled(pm[of], a.c) - y_of.M)), inc = group_scan<WAVES>(w), z = __shfl(inc, WAVES - 1);
         const double target = u * z;
-        lz = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(log2_((float)z))));
+        if (lane == 0) under32[wave] = make_float2(log2_((float)z), y_of.M);
         const float near = (float)(d.margin * z);
         const u32 part = (u32)__popcll(__ballot(inc <= target) & ((1u << WAVES) - 1));
         if (wave == part) {
@@ -682,7 +682,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
             }
             if (sure) {
                 d.token[row] = (int)token;
-                d.ml2p[row] = Under32{lz, y_of}(x);
+                d.ml2p[row] = Under32{log2_((float)z), y_of}(x);
                 done = 1;
             }
         }
@@ -706,8 +706,12 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
     __syncthreads();
     const double part_sum = lane < (u32)WAVES ? ps[lane] : 0., inc = group_scan<64>(part_sum), z = __shfl(inc, 63);
     const u64 passes = __ballot(inc > u * z);
+    if (lane == 0) under64[wave] = z;
     const auto value = [&](float x) {
-        return doubtful(m, a.c) ? Under64{z, (double)m, d.power.c}(x) : Under32{lz, Expo(Stat{m, 0.f, 0.f, false}, a.c)}(x);
+        if (doubtful(m, a.c)) return Under64{under64[wave], (double)m, d.power.c}(x);
+        Expo y_of(Stat{m, 0.f, 0.f, false}, a.c);
+        y_of.M = under32[wave].y;
+        return Under32{under32[wave].x, y_of}(x);
     };
     if (wave == (passes ? (u32)__ffsll((unsigned long long)passes) - 1 : 0u)) {
         const double none[PART_WAVES] = {};
