@@ -133,12 +133,13 @@ struct Span {
     float first;  // the head's logit, or -inf
 };
 
+// (`read`: false for a row that is skipped, of which nothing is loaded)
 template <int DT>
-__device__ __forceinline__ Span span_of(const Rows &a, const char *row) {
+__device__ __forceinline__ Span span_of(const Rows &a, const char *row, bool read) {
     if constexpr (Elt<DT>::BYTES == 2) {
         if ((uintptr_t)row & 2) {
             const u32 n = a.vocab - 1;
-            return Span{row + 2, 1, n, (n + VEC<DT> - 1) / VEC<DT>, n / VEC<DT>, element<DT>(row, 0)};
+            return Span{row + 2, 1, n, (n + VEC<DT> - 1) / VEC<DT>, n / VEC<DT>, read ? element<DT>(row, 0) : -INFINITY};
         }
     }
     return Span{row, 0, a.vocab, a.nvec, a.full, -INFINITY};

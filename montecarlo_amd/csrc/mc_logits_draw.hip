@@ -451,7 +451,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_sums(Rows a, DrawArgs d, 
     __shared__ float pm[PART_WAVES];
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (row >= a.rows || (d.live && !d.live[row])) return;
-    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row), true);
     const u32 share = sp.vecs / PART_WAVES, v0 = min(part * sp.vecs + wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     double s;
     float m;
@@ -528,7 +528,7 @@ __global__ __launch_bounds__(WIDE, 4) void k_logits_draw(Rows a, DrawArgs d) {
         return;
     }
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, true);
     const double u = uniform_of(d, row);
     const u32 share = (r.nvec + WIDE_WAVES - 1) / WIDE_WAVES, v0 = min(wave * share, r.nvec), v1 = min(r.nvec, v0 + share);
     double s;
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 6) void k_logits_draw_held(Rows a
         return;
     }
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, true);
     const u32 nv = (r.nvec + T - 1) / T, v0 = wave * nv * 64;
     raw4 q[HELD];
 #pragma unroll
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_draw_join(Rows a, DrawArgs d, 
         return;
     }
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, true);
     const double u = uniform_of(d, row);
     double mine = 0., within[PART_WAVES] = {};
     float m = -INFINITY;

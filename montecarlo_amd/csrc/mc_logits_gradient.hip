@@ -1,7 +1,8 @@
 // The gradient of weights * (-log2 p of the given token) + entropy weights * entropy for the logits, with both values
 // (formulas: mc_logits_score.hip).  A row is read once and its gradient written once while its vectors fit the registers
 // of a group of lanes or of one workgroup of up to 1024 lanes (131072 tokens of two bytes); longer rows, and
-// rows too few to fill the GPU, are summed part by part by one launch and written by a second one.
+// rows too few to fill the GPU, are summed part by part by one launch, joined by a second one (before anything is written, since the
+// gradient may take the logits' place) and written by a third.
 #include "mc_logits.h"
 
 namespace {
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(T, HELD > 8 ? 4 : 8) void k_logits_gradient_held(Ro
     if (row >= a.rows) return;
     const int tok = token_of(a, row);
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, tok != MC_TOKEN_SKIP);
     char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
     const u32 nv = (r.nvec + T - 1) / T;
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
@@ -176,7 +177,7 @@ template <int DT, bool ENT>
 __global__ __launch_bounds__(BLOCK) void k_logits_gradient_sums(Rows a, Split sp) {
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
     if (row >= a.rows || token_of(a, row) == MC_TOKEN_SKIP) return;
-    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row), true);
     const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
     Stat st{-INFINITY, 0.f, 0.f, false};
     for (u32 v = v0; v < v1; v += BLOCK * UNROLL) {
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_join(Rows a, GradOut 
             st = Stat{f.x, f.y, f.z, false};
         }
         st = group_stat<64, ENT>(st, a.c);
-        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(span_of<DT>(a, p), a.c, st.m);
+        if (doubtful(st.m, a.c)) st = exact_stat<DT, BLOCK, ENT>(span_of<DT>(a, p, true), a.c, st.m);
     }
     __syncthreads();  // (every wave has read the parts)
     if (threadIdx.x == 0) {
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_gradient_parts(Rows a, GradOut
     const u32 id = block_id(), row = id >> sp.shift, part = id & ((1u << sp.shift) - 1);
     if (row >= a.rows) return;
     const int tok = token_of(a, row);
-    const Span r = span_of<DT>(a, at(a.logits, a.inner, row));
+    const Span r = span_of<DT>(a, at(a.logits, a.inner, row), tok != MC_TOKEN_SKIP);
     char *gp = out.grad + (u64)row * a.vocab * Elt<DT>::BYTES;
     const u32 v0 = min(part * sp.vecs, r.nvec), v1 = min(r.nvec, v0 + sp.vecs);
     const float4 f = sp.stats[(u64)row << sp.shift];

@@ -392,7 +392,7 @@ __global__ __launch_bounds__(T, 8) void k_logits_score(Rows a, ScoreOut out, Spl
         return;
     }
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, true);
     const float x = !PART && tok >= 0 ? element<DT>(p, tok) : 0.f;
     const u32 v0 = PART ? min(part * sp.vecs, r.nvec) : 0, v1 = PART ? min(r.nvec, v0 + sp.vecs) : r.nvec;
     // (cells of as many chunks as the launch's LDS was counted with: a shorter last part, or a row without its first element, may
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(BLOCK) void k_logits_score_join(Rows a, ScoreOut ou
         return;
     }
     const char *p = at(a.logits, a.inner, row);
-    const Span r = span_of<DT>(a, p);
+    const Span r = span_of<DT>(a, p, true);
     const float x = tok >= 0 ? element<DT>(p, tok) : 0.f;
     const u32 parts = 1u << sp.shift, lane = threadIdx.x & 63;
     Stat st{-INFINITY, 0.f, 0.f, false};

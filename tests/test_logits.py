@@ -208,3 +208,26 @@ def test_the_cells_of_alternatives_fit_what_is_allocated():
                         per_cell, room = cells(nvec, lanes)
                         used = [up(up(mine, 4 * lanes), per_cell)]
                     assert max(used) <= room <= 16, (vocab, rows, size, used, room)
+
+
+def test_kernels_load_nothing_of_skipped_rows():
+    """Every place where a kernel looks at where a row begins (which loads the first element of rows of two bytes at an odd one) lies
+    behind the question whether the row is skipped, or is told."""
+    import os
+    import re
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "montecarlo_amd", "csrc")
+    head = open(os.path.join(here, "mc_logits.h")).read()
+    body = head[head.index("Span span_of("):head.index("// vector v of a row;")]
+    assert "bool read" in body and re.search(r"read \? element<DT>\(row, 0\) : -INFINITY", body)
+    seen = 0
+    for name in ("score", "gradient", "draw"):
+        src = open(os.path.join(here, f"mc_logits_{name}.hip")).read()
+        for kernel in re.split(r"\n__global__ ", src)[1:]:
+            for m in re.finditer(r"span_of<DT>\(([^;]*)\)[,;]", kernel):
+                seen += 1
+                before = kernel[:m.start()]
+                told = "tok != MC_TOKEN_SKIP" in m.group(1)
+                asked = re.search(r"if \((tok == MC_TOKEN_SKIP|d\.live && !d\.live\[row\])\) \{.*?return;|(== MC_TOKEN_SKIP|!d\.live\[row\]\))\) return;"
+                                  r"|if \(tok != MC_TOKEN_SKIP\) \{", before, re.S)
+                assert told or asked, (name, kernel[:60])
+    assert seen >= 9
