@@ -557,6 +557,7 @@ int mc_rank_query(const double *keys_sorted, const double *positions, uint64_t n
  * are contiguous [outer * inner].  Sums are held in 32 bits (the draw decides in 64); -log2 p and entropies are never below 0.  All calls are asynchronous on
  * `stream`, allocate nothing and may be captured into a graph.  A workspace (16-byte aligned, mc_logits_*_workspace_bytes;
  * NULL where that is 0) holds nothing between calls, but calls that may overlap need one each.  Temperatures 1e-30 .. 1e30.
+ * Every pointer is aligned to what it points to.
  *   token ids   0 .. vocab - 1; MC_TOKEN_SKIP: the row is not read (padding), its outputs are 0; anything else is a token
  *               outside the model, as MC_TOKEN_OUTSIDE: impossible (+inf)
  *   -inf        a token switched off: probability 0.  A row with nothing left: ml2p +inf, entropy 0, no alternatives, no

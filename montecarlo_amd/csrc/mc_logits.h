@@ -623,6 +623,8 @@ inline int bad(const char *who, const char *why) {
     return MC_ERR_ARG;
 }
 
+inline bool aligned(const void *p, size_t bytes) { return (uintptr_t)p % bytes == 0; }  // (null is)
+
 inline Div make_div(u64 d) {
     Div r{(u32)d, 0, 0};
     while ((1ull << r.shift) < d) ++r.shift;
@@ -646,7 +648,7 @@ inline int rows_of(const char *who, Rows &a, const void *logits, uint32_t dtype,
     if (!(temperature >= 1e-30 && temperature <= 1e30)) return bad(who, "the temperature is a positive number (1e-30 .. 1e30)");
     if (outer * inner && !logits) return bad(who, "no logits");
     const int bytes = dtype == MC_LOGITS_F32 ? 4 : 2;
-    if ((uintptr_t)logits % bytes) return bad(who, "logits that are not aligned to their type");
+    if (!aligned(logits, bytes)) return bad(who, "logits that are not aligned to their type");
     a.rows = (u32)(outer * inner);
     if (outer > 1 && flat && one_run(inner, outer_stride, inner_stride)) {
         inner *= outer;
@@ -665,7 +667,7 @@ inline int tokens_of(const char *who, Rows &a, const void *tokens, uint32_t toke
                      uint64_t rows) {
     if (token_bytes != 4 && token_bytes != 8) return bad(who, "token ids of 4 or 8 bytes");
     if (rows && !tokens) return bad(who, "no tokens");
-    if ((uintptr_t)tokens % token_bytes) return bad(who, "tokens that are not aligned to their type");
+    if (!aligned(tokens, token_bytes)) return bad(who, "tokens that are not aligned to their type");
     a.token_bytes = token_bytes;
     a.tokens = view_of(tokens, outer_stride, inner_stride, token_bytes);
     return MC_OK;

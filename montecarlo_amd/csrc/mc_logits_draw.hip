@@ -911,6 +911,8 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     if (int rc = rows_of(who, a, logits, dtype, 1, rows, vocab, 0, row_stride, temperature, true)) return rc;
     if (a.rows == 0) return MC_OK;
     if (!out_token || !out_ml2p) return bad(who, "no output");
+    if (!aligned(uniforms, 8)) return bad(who, "uniforms that are not aligned to their type");
+    if (!aligned(out_token, 4) || !aligned(out_ml2p, 4)) return bad(who, "outputs that are not aligned to their type");
     hipStream_t s = (hipStream_t)stream;
     const double c = LOG2E / temperature;
     DrawArgs d{uniforms, seed, first_id, draw, temperature, margin_of(a), Power{c, (float)(-1000. / c)}, live, out_token, out_ml2p};
@@ -919,7 +921,7 @@ extern "C" int mc_logits_draw(const void *logits, uint32_t dtype, uint64_t rows,
     } else {
         Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr};
         if (sp.shift) {
-            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
+            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || !aligned(workspace, 16)) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);
                 return MC_ERR_WORKSPACE;
             }
@@ -947,6 +949,8 @@ extern "C" int mc_logits_keys(const float *ml2p, const int64_t *offsets, const v
     if (lengths && length_bytes != 4 && length_bytes != 8) return bad(who, "lengths of 4 or 8 bytes");
     if (count == 0) return MC_OK;
     if (!out_keys || (longest && !ml2p)) return bad(who, "null pointer");
+    if (!aligned(ml2p, 4) || !aligned(offsets, 8) || !aligned(lengths, lengths ? length_bytes : 1) || !aligned(out_keys, 8))
+        return bad(who, "values, offsets, lengths and keys are aligned to their types");
     const KeyArgs k{ml2p, (const i64 *)offsets, lengths, lengths ? length_bytes : 0u, (u64)count, (u64)longest, (i64)stride, out_keys};
     hipStream_t s = (hipStream_t)stream;
     const u64 usual = offsets ? longest / count : longest;  // symbols of a password, or as many as it may have

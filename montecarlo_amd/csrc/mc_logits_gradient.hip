@@ -298,13 +298,15 @@ extern "C" int mc_logits_gradient(const void *logits, uint32_t dtype, uint64_t o
     if (a.rows == 0) return MC_OK;
     if (!weights) return bad(who, "no weights");
     if (!out_ml2p || !out_grad || (entropy_weights && !out_entropy)) return bad(who, "no output");
-    if ((uintptr_t)out_grad % (dtype == MC_LOGITS_F32 ? 4 : 2)) return bad(who, "a gradient that is not aligned to its type");
+    if (!aligned(out_grad, dtype == MC_LOGITS_F32 ? 4 : 2)) return bad(who, "a gradient that is not aligned to its type");
+    if (!aligned(weights, 4) || !aligned(entropy_weights, 4)) return bad(who, "weights that are not aligned to their type");
+    if (!aligned(out_ml2p, 4) || (entropy_weights && !aligned(out_entropy, 4))) return bad(who, "outputs that are not aligned to their type");
     GradOut out{view_of(weights, weight_outer_stride, weight_inner_stride, 4),
                 view_of(entropy_weights, entropy_outer_stride, entropy_inner_stride, 4),
                 (float)(1.0 / temperature), out_ml2p, out_entropy, (char *)out_grad};
     Split sp{split_shift(a.rows, a.nvec), 0, nullptr};
     if (sp.shift) {
-        if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || (uintptr_t)workspace % 16) {
+        if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift) || !aligned(workspace, 16)) {
             mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift), workspace_bytes);
             return MC_ERR_WORKSPACE;
         }

@@ -558,6 +558,8 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
     if (top > MC_LOGITS_MAX_TOP || top > vocab) return bad(who, "top: at most 64 alternatives, and no more than tokens");
     if (a.rows == 0) return MC_OK;
     if (!out_ml2p || (top && (!out_top || !out_top_ml2p))) return bad(who, "no output");
+    if (!aligned(out_ml2p, 4) || !aligned(out_entropy, 4) || (top && !(aligned(out_top, 4) && aligned(out_top_ml2p, 4))))
+        return bad(who, "outputs that are not aligned to their type");
     ScoreOut out{out_ml2p, out_entropy, out_top_ml2p, out_top, top};
     hipStream_t s = (hipStream_t)stream;
     if (a.nvec <= SUB_VECS) {
@@ -571,7 +573,7 @@ extern "C" int mc_logits_score(const void *logits, uint32_t dtype, uint64_t oute
     } else {
         Split sp{split_shift(a.rows, a.vocab, a.nvec), 0, nullptr, nullptr, 0};
         if (sp.shift) {
-            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift, top) || (uintptr_t)workspace % 16) {
+            if (!workspace || workspace_bytes < split_bytes(a.rows, sp.shift, top) || !aligned(workspace, 16)) {
                 mc_set_error("%s: an aligned workspace of %zu bytes is needed, not %zu", who, split_bytes(a.rows, sp.shift, top), workspace_bytes);
                 return MC_ERR_WORKSPACE;
             }

@@ -231,3 +231,19 @@ def test_kernels_load_nothing_of_skipped_rows():
                                   r"|if \(tok != MC_TOKEN_SKIP\) \{", before, re.S)
                 assert told or asked, (name, kernel[:60])
     assert seen >= 9
+
+
+@pytest.mark.parametrize("name,args,which", [
+    ("mc_logits_score", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, ADDR, 2, ADDR, ADDR, None, 0, None], {12: 2, 13: 2, 15: 2, 16: 2}),
+    ("mc_logits_gradient", [ADDR, 0, 1, 1, 8, 0, 8, ADDR, 8, 0, 1, 1.0, ADDR, 0, 1, ADDR, 0, 1, ADDR, ADDR, ADDR, None, 0, None], {12: 2, 15: 1, 18: 2, 19: 2}),
+    ("mc_logits_draw", [ADDR, 0, 1, 8, 8, 1.0, ADDR, 0, 0, 0, None, ADDR, ADDR, None, 0, None], {6: 4, 11: 2, 12: 2}),
+    ("mc_logits_keys", [ADDR, ADDR, None, 0, 1, 0, 1, ADDR, None], {0: 2, 1: 4, 7: 4}),
+    ("mc_logits_keys", [ADDR, None, ADDR, 8, 1, 4, 4, ADDR, None], {0: 1, 2: 4, 7: 4}),
+    ("mc_logits_keys", [ADDR, None, ADDR, 4, 1, 4, 4, ADDR, None], {2: 2}),
+])
+def test_what_is_not_aligned_to_its_type_is_refused(name, args, which):
+    for i, off in which.items():
+        mine = list(args)
+        mine[i] += off
+        assert getattr(nv.lib, name)(*mine) == -1, (name, i)
+        assert b"aligned" in nv.lib.mc_last_error(), (name, i)
