@@ -27,10 +27,11 @@ LINK_FLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC", "-ldl"]
 
 
 def sources_digest() -> str:
-    """sha256 over the native sources the library is built from (names and bytes): a measurement of the kernels
-    (profiles/hbm_traffic_latest.json) records it, and bench.py quotes the measurement only while it still holds."""
+    """sha256 over the native sources the library is built from (names and bytes) and the flags it is built with: a
+    measurement of the kernels (profiles/hbm_traffic_latest.json) records it, and bench.py quotes the measurement only while
+    it still holds."""
     import hashlib
-    h = hashlib.sha256()
+    h = hashlib.sha256("\n".join(FLAGS + LINK_FLAGS).encode())
     for path in sorted([os.path.join(CSRC, s) for s in SOURCES] + HEADERS):
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
@@ -42,7 +43,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, s) for s in SOURCES] + HEADERS
+    deps = [os.path.join(CSRC, s) for s in SOURCES] + HEADERS + [os.path.abspath(__file__)]      # (the flags stand here)
     return any(os.path.getmtime(d) > t for d in deps)
 
 
