@@ -37,7 +37,8 @@ class LogitsMonteCarlo(MonteCarlo):
         return self.logits(tokens)[:, -1]
 
     def encode(self, pwd: str) -> List[int]:
-        """A password's tokens; ``OUTSIDE`` for what the vocabulary does not hold.  One character a token, unless overridden."""
+        """A password's tokens; ``OUTSIDE`` (or any other id that is none) for what the vocabulary does not hold.  One character a
+        token, unless overridden."""
         return [self._ids.get(c, OUTSIDE) for c in pwd]
 
     # ---- sampling (lib4mc/MonteCarloParent.py:33-46) ---------------------------------------------------------------
@@ -102,8 +103,10 @@ class LogitsMonteCarlo(MonteCarlo):
         parts: List[List[str]] = []
         for at in range(0, len(pwds), self.batch):
             ids = [self.encode(p) for p in pwds[at:at + self.batch]]
-            # (a password that is too long, or holds the end, is impossible whatever its tokens are: it stands as one unknown token)
-            rows = [[OUTSIDE] if len(r) > self.max_len or self.end in r else r + [self.end] if len(r) < self.max_len else r for r in ids]
+            # (a password that is too long, or holds the end or what is no token -- SKIP too, which would count as certain --, is
+            # impossible whatever its other tokens are: it stands as one unknown token, and the model is asked nothing else)
+            whole = [len(r) <= self.max_len and all(0 <= t < len(self.vocabulary) and t != self.end for t in r) for r in ids]
+            rows = [[OUTSIDE] if not w else r + [self.end] if len(r) < self.max_len else r for r, w in zip(ids, whole)]
             width = max(len(r) for r in rows)
             tokens = torch.tensor([r + [SKIP] * (width - len(r)) for r in rows], dtype=torch.int64, device=self.device)
             scores = logits_score(self.logits(tokens[:, :-1].clamp(min=0)), tokens, temperature=self.temperature)

@@ -1,0 +1,57 @@
+"""The plugin of models that answer with logits (montecarlo_amd.logits_simulator) without a GPU: what it hands to the model and
+to the operators, which are stood in for by the definitions."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from montecarlo_amd import logits_simulator as ls
+from montecarlo_amd.logits import LogitScores
+from tests.logits_ref import OUTSIDE, SKIP, Row
+
+
+class Model(ls.LogitsMonteCarlo):
+    """Logits by place; keeps what it was asked and what was scored."""
+
+    def __init__(self, texts="ab", seed=1, wide=0, **kw):
+        kw.setdefault("max_len", 4)
+        super().__init__(list(texts) + ["<end>"], len(texts), device="cpu", **kw)
+        g = torch.Generator().manual_seed(seed)
+        self.table = torch.randn(self.max_len + 1, len(self.vocabulary) + wide, generator=g)
+        self.asked, self.scored = [], []
+
+    def logits(self, tokens):
+        self.asked.append(tokens)
+        return self.table[:tokens.shape[1] + 1].expand(tokens.shape[0], -1, -1)
+
+
+@pytest.fixture(autouse=True)
+def definitions(monkeypatch):
+    def score(x, tokens, temperature=1.0):
+        assert x.shape[:-1] == tokens.shape
+        rows = [Row(r, temperature).score(t)[0] for r, t in zip(x.reshape(-1, x.shape[-1]).numpy(), tokens.reshape(-1).tolist())]
+        return LogitScores(torch.tensor(rows).view(tokens.shape))
+
+    def keys(ml2p):
+        s = ml2p.double().sum(-1)
+        return torch.where(s == math.inf, 1022.0, s)
+
+    monkeypatch.setattr(ls, "logits_score", score)
+    monkeypatch.setattr(ls, "logits_keys", keys)
+
+
+@pytest.mark.parametrize("bad", [SKIP, -7, 3, 1 << 40])
+def test_an_encoding_that_leaves_the_vocabulary_is_impossible(bad):
+    class Odd(Model):
+        def encode(self, pwd):
+            return [bad if c == "?" else i for c, i in zip(pwd, super().encode(pwd))]
+
+    m = Odd()
+    ml2p, parts = m.score_batch(["a?b", "?", "ab", "b?", "abab"])
+    assert [x == 1022.0 for x in ml2p] == [True, True, False, True, False]
+    assert parts[0] == ["a?b"] and parts[2] == ["a", "b"]
+    for t in m.asked:                                       # the model sees no id that it does not know
+        assert int(t.min()) >= 0 and int(t.max()) < len(m.vocabulary)
+    want = sum(Row(m.table[i].numpy(), 1.0).score(t)[0] for i, t in enumerate([0, 1, 2]))
+    assert abs(ml2p[2] - want) < 1e-5
