@@ -30,11 +30,17 @@ class LogitsMonteCarlo(MonteCarlo):
     @abc.abstractmethod
     def logits(self, tokens: torch.Tensor) -> torch.Tensor:
         """[B, t] tokens (int64; any value behind a password's end) -> [B, t + 1, V] logits on the GPU: place i speaks of token
-        i given the i before it."""
+        i given the i before it.  More logits than tokens (rows padded to a multiple) are cut to the vocabulary's."""
 
     def next_logits(self, tokens: torch.Tensor) -> torch.Tensor:
         """[B, t] tokens -> [B, V] logits of the next one (a model with a state of its own keeps it here)."""
         return self.logits(tokens)[:, -1]
+
+    def _of_vocabulary(self, x: torch.Tensor) -> torch.Tensor:
+        n = len(self.vocabulary)
+        if x.shape[-1] < n:
+            raise ValueError(f"the model answers with {x.shape[-1]} logits for a vocabulary of {n}")
+        return x[..., :n]
 
     def encode(self, pwd: str) -> List[int]:
         """A password's tokens; ``OUTSIDE`` (or any other id that is none) for what the vocabulary does not hold.  One character a
@@ -48,7 +54,7 @@ class LogitsMonteCarlo(MonteCarlo):
         ml2p = torch.zeros((n, self.max_len), dtype=torch.float32, device=self.device)
         live = torch.ones(n, dtype=torch.bool, device=self.device)
         for step in range(self.max_len):
-            x = self.next_logits(tokens[:, :step].clamp(min=0))
+            x = self._of_vocabulary(self.next_logits(tokens[:, :step].clamp(min=0)))
             r = logits_draw(x, seed=seed, first_id=first, draw=step, temperature=self.temperature, live=live)
             tokens[:, step], ml2p[:, step] = r.tokens, r.ml2p
             live = live & (r.tokens != self.end) & (r.tokens != OUTSIDE)
@@ -109,7 +115,8 @@ class LogitsMonteCarlo(MonteCarlo):
             rows = [[OUTSIDE] if not w else r + [self.end] if len(r) < self.max_len else r for r, w in zip(ids, whole)]
             width = max(len(r) for r in rows)
             tokens = torch.tensor([r + [SKIP] * (width - len(r)) for r in rows], dtype=torch.int64, device=self.device)
-            scores = logits_score(self.logits(tokens[:, :-1].clamp(min=0)), tokens, temperature=self.temperature)
+            x = self._of_vocabulary(self.logits(tokens[:, :-1].clamp(min=0)))
+            scores = logits_score(x, tokens, temperature=self.temperature)
             keys = logits_keys(scores.ml2p).tolist()
             ml2p += keys
             parts += [[self.vocabulary[t] for t in r] if k < 1022.0 else [p]

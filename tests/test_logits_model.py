@@ -55,3 +55,33 @@ def test_an_encoding_that_leaves_the_vocabulary_is_impossible(bad):
         assert int(t.min()) >= 0 and int(t.max()) < len(m.vocabulary)
     want = sum(Row(m.table[i].numpy(), 1.0).score(t)[0] for i, t in enumerate([0, 1, 2]))
     assert abs(ml2p[2] - want) < 1e-5
+
+
+def draws(monkeypatch, m):
+    """logits_draw stood in for by the first most probable token, and what it was given."""
+    seen = []
+
+    def draw(x, seed, first_id, draw, temperature, live):
+        seen.append(x.shape)
+        from montecarlo_amd.logits import LogitDraws
+        return LogitDraws(torch.where(live, x.argmax(-1), SKIP).int(), torch.zeros(x.shape[0]))
+
+    monkeypatch.setattr(ls, "logits_draw", draw)
+    return seen
+
+
+def test_a_model_of_fewer_logits_than_tokens_is_refused_and_padding_is_not_looked_at(monkeypatch):
+    m = Model()
+    want = m.score_batch(["ab", "a"])
+    m.table = m.table[:, :2]
+    with pytest.raises(ValueError, match="2 logits for a vocabulary of 3"):
+        m.score_batch(["ab"])
+    seen = draws(monkeypatch, m)
+    with pytest.raises(ValueError, match="2 logits for a vocabulary of 3"):
+        m.sample(5)
+    wide = Model(wide=5)                                    # (rows padded to a multiple of eight)
+    wide.table = torch.cat([Model().table, torch.full((5, 5), 30.0)], 1)
+    assert wide.score_batch(["ab", "a"]) == want
+    strings = {}
+    assert len(wide.sample(5, strings)) == 5 and all(s == (5, 3) for s in seen)
+    assert set("".join(strings)) <= set("ab")
