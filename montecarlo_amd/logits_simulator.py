@@ -111,13 +111,15 @@ class LogitsMonteCarlo(MonteCarlo):
             ids = [self.encode(p) for p in pwds[at:at + self.batch]]
             # (a password that is too long, or holds the end or what is no token -- SKIP too, which would count as certain --, is
             # impossible whatever its other tokens are: it stands as one unknown token, and the model is asked nothing else)
-            whole = [len(r) <= self.max_len and all(0 <= t < len(self.vocabulary) and t != self.end for t in r) for r in ids]
+            whole = [not r or len(r) <= self.max_len and min(r) >= 0 and max(r) < len(self.vocabulary) and self.end not in r for r in ids]
             rows = [[OUTSIDE] if not w else r + [self.end] if len(r) < self.max_len else r for r, w in zip(ids, whole)]
             width = max(len(r) for r in rows)
             tokens = torch.tensor([r + [SKIP] * (width - len(r)) for r in rows], dtype=torch.int64, device=self.device)
             x = self._of_vocabulary(self.logits(tokens[:, :-1].clamp(min=0)))
             scores = logits_score(x, tokens, temperature=self.temperature)
             keys = logits_keys(scores.ml2p).tolist()
+            if any(k != k for k in keys):
+                raise RuntimeError("the model's logits hold NaN or +inf")
             ml2p += keys
             parts += [[self.vocabulary[t] for t in r] if k < 1022.0 else [p]
                       for p, r, k in zip(pwds[at:at + self.batch], ids, keys)]

@@ -85,3 +85,15 @@ def test_a_model_of_fewer_logits_than_tokens_is_refused_and_padding_is_not_looke
     strings = {}
     assert len(wide.sample(5, strings)) == 5 and all(s == (5, 3) for s in seen)
     assert set("".join(strings)) <= set("ab")
+
+
+def test_a_model_that_answers_nan_is_an_error_when_scoring_too():
+    m = Model()
+    m.table[1, 0] = math.nan
+    with pytest.raises(RuntimeError, match="NaN"):
+        m.score_batch(["bb", "ab"])
+    with pytest.raises(RuntimeError, match="NaN"):
+        m.calc_ml2p("ab")
+    m.table[1, 0] = math.inf
+    with pytest.raises(RuntimeError, match="NaN"):
+        m.score_batch(["bb"])
