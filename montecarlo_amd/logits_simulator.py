@@ -26,6 +26,11 @@ class LogitsMonteCarlo(MonteCarlo):
         self.temperature, self.batch = float(temperature), int(batch)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self._ids = {text: i for i, text in enumerate(self.vocabulary) if i != self.end}
+        if type(self).encode is LogitsMonteCarlo.encode:
+            chars = [text for i, text in enumerate(self.vocabulary) if len(text) == 1 and i != self.end]
+            twice = next((c for c in chars if chars.count(c) > 1), None) if len(set(chars)) < len(chars) else None
+            if twice is not None:                           # (samples would hold either, scores only know the last)
+                raise ValueError(f"vocabulary: two tokens are {twice!r}")
 
     @abc.abstractmethod
     def logits(self, tokens: torch.Tensor) -> torch.Tensor:

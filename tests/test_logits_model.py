@@ -97,3 +97,15 @@ def test_a_model_that_answers_nan_is_an_error_when_scoring_too():
     m.table[1, 0] = math.inf
     with pytest.raises(RuntimeError, match="NaN"):
         m.score_batch(["bb"])
+
+
+def test_characters_that_two_tokens_share_are_refused():
+    with pytest.raises(ValueError, match="'a'"):
+        Model("aba")
+    Model(["ab", "ab", "<pad>", "<pad>", "", "", "a"])      # (texts that no character is encoded as)
+
+    class Own(Model):
+        def encode(self, pwd):
+            return [0 for _ in pwd]
+
+    assert Own("aba").encode("a") == [0]                    # an encoding of one's own may know them apart
