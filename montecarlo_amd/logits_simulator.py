@@ -4,7 +4,7 @@ runs on ``montecarlo_amd.logits``.  The keys it samples stay on the GPU and go t
 from __future__ import annotations
 
 import abc
-from typing import Dict, List, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -13,17 +13,27 @@ from .lib4mc.MonteCarloParent import MonteCarlo, SampleKeys
 from .logits import OUTSIDE, SKIP, logits_draw, logits_keys, logits_score
 
 
+def default_batch(tokens: int, max_len: int) -> int:
+    """Passwords at a time: 65536, or as many as their answers' [batch, max_len, tokens] logits stay below 2^31 with."""
+    return max(1, min(1 << 16, (1 << 31) // (tokens * max_len)))
+
+
 class LogitsMonteCarlo(MonteCarlo):
     """``vocabulary``: the text of every token, the end symbol's at position ``end``.  A password is its tokens and the end
     symbol; one of ``max_len`` tokens needs no end symbol (so the probabilities of all strings up to that length add up to
-    1) and longer ones are impossible.  ``batch``: passwords the model is asked about at a time."""
+    1) and longer ones are impossible.  ``batch``: passwords the model is asked about at a time (``default_batch``).
 
-    def __init__(self, vocabulary: Sequence[str], end: int, max_len: int = 32, temperature: float = 1.0, batch: int = 1 << 16,
-                 device=None):
+    Samples carry the probability of the tokens that were drawn, ``calc_ml2p`` that of the tokens that ``encode`` gives: of a
+    sub-word vocabulary, in which a password has several encodings, each speaks of one of them.  Scores are sums of 32 bits per
+    token: a sample's key and its password's score, or those of batches of other sizes, may differ in their last bits."""
+
+    def __init__(self, vocabulary: Sequence[str], end: int, max_len: int = 32, temperature: float = 1.0,
+                 batch: Optional[int] = None, device=None):
         self.vocabulary, self.end, self.max_len = list(vocabulary), int(end), int(max_len)
-        if not 0 <= self.end < len(self.vocabulary) or self.max_len < 1 or batch < 1:
+        if not 0 <= self.end < len(self.vocabulary) or self.max_len < 1 or (batch is not None and batch < 1):
             raise ValueError("end: a position of the vocabulary; max_len and batch: at least 1")
-        self.temperature, self.batch = float(temperature), int(batch)
+        self.temperature = float(temperature)
+        self.batch = default_batch(len(self.vocabulary), self.max_len) if batch is None else int(batch)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self._ids = {text: i for i, text in enumerate(self.vocabulary) if i != self.end}
         if type(self).encode is LogitsMonteCarlo.encode:

@@ -109,3 +109,12 @@ def test_characters_that_two_tokens_share_are_refused():
             return [0 for _ in pwd]
 
     assert Own("aba").encode("a") == [0]                    # an encoding of one's own may know them apart
+
+
+@pytest.mark.parametrize("tokens,max_len,batch", [(3, 4, 1 << 16), (97, 32, 1 << 16), (257, 64, 1 << 16), (32768, 32, 2048), (131072, 64, 256), (1 << 20, 1 << 12, 1)])
+def test_the_default_batch_knows_the_width_of_the_answer(tokens, max_len, batch):
+    """At most 2^31 logits at a time ([batch, places, tokens]), and what was there for models of few tokens."""
+    m = Model([chr(0x4E00 + i) if i < 20000 else f"t{i}" for i in range(tokens - 1)], max_len=1)
+    assert m.batch == 1 << 16 if tokens * 2 * (1 << 16) <= 1 << 31 else m.batch * tokens <= 1 << 31
+    assert ls.default_batch(tokens, max_len) == batch
+    assert Model("ab", batch=70000).batch == 70000
