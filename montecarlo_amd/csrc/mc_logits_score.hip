@@ -162,8 +162,10 @@ __device__ __forceinline__ void sub_top(SubRow<DT, NV> &r, const Rows &a, const 
     if (__ballot(writes && !fits)) top_by_turns<DT, G>(r, st, out, row, writes && !fits, a.c);
 }
 
+// (Waves a SIMD with alternatives: six while the row's vectors leave the registers for it, else four.  Of five vectors of four-byte
+// logits six spill 27 registers inside the loops: 60000 rows of 1200 tokens 484 us.)
 template <int DT, int G, int NV, bool ENT, bool TOP>
-__global__ __launch_bounds__(BLOCK, !TOP ? 8 : NV > 5 ? 4 : 6) void k_logits_score_sub(Rows a, ScoreOut out, u32 room) {
+__global__ __launch_bounds__(BLOCK, !TOP ? 8 : NV > (DT == MC_LOGITS_F32 ? 4 : 5) ? 4 : 6) void k_logits_score_sub(Rows a, ScoreOut out, u32 room) {
     extern __shared__ u64 candidates[];
     const u32 row = block_id() * (BLOCK / G) + threadIdx.x / G, lane = threadIdx.x & (G - 1);
     const bool there = row < a.rows;
