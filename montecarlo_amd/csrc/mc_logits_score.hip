@@ -82,7 +82,8 @@ __device__ __forceinline__ void top_by_turns(SubRow<DT, NV> &r, const Stat &st, 
 // The k largest of a row in registers at once.  The first 16 bits of the order word that k of the row's vectors' largest (or,
 // where these are fewer than 2 k, of its elements) reach, bit by bit; the few elements that reach them go to LDS, and
 // each finds its place by counting the larger ones.  (One after the other, 10 of 1000 took 271 us for 67108 rows, 32 took 938.)
-// `room`: candidates a row has room for; rows with more (many equal ones) take turns.
+// `room`: candidates a row has room for; rows with more (many equal ones) take turns.  The sixteen counts are what bounds it: 2^20
+// rows of 97 two-byte tokens take 52 us without alternatives, 155 with 5 and 282 with 10, which count elements (2 k > G N).
 template <int DT, int G, int NV>
 __device__ __forceinline__ void sub_top(SubRow<DT, NV> &r, const Rows &a, const Stat &st, const ScoreOut &out, u32 row, bool writes, int tok, u64 *room_of_all,
                                         u32 room) {
@@ -507,7 +508,7 @@ u32 split_shift(u32 rows, u32 vocab, u32 nvec) {
 // Lanes of a workgroup that has a row to itself: 1024 for the longest rows (2049 rows of 131073 tokens, a third of them
 // skipped: 197 us with 256 lanes, 137 with 1024: fewer rows at a time share the load evenly) and where there are few rows;
 // else 256, since eight workgroups a compute unit hide each other's phases (8192 rows of 32768 with 10 alternatives: 113 and
-// 178 us).
+// 178 us).  (With alternatives of two-byte rows 1024 lanes leave 6 or 7 registers to scratch.)
 constexpr int WIDE = 1024;
 bool wide(u32 rows, u32 nvec) { return nvec >= 16384 || (rows <= 256 && nvec >= 2048); }
 

@@ -3,8 +3,10 @@
 
 The caller's model gives a row of logits over V tokens for every place; all results are in the units of the Monte Carlo path
 (-log2 p; keys as float64), so ``logits_keys`` feeds ``MonteCarloLib`` directly.  Tensors live on one GPU; every call runs
-on torch's current stream of that GPU, waits for nothing and may be captured into a graph.  No CPU fallback: tensors that
-are not on a GPU are refused."""
+on torch's current stream of that GPU, waits for nothing and may be captured into a graph.  No value of -log2 p, entropy or key
+is below 0.  The last bits of sums in 32 bits depend on how a launch deals a row to lanes, which goes by the number of rows and
+of tokens: the same row scored in calls of other sizes, or scored and drawn from, may differ there.  No CPU fallback: tensors
+that are not on a GPU are refused."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
@@ -179,7 +181,8 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
 
     ``uniforms``: float64 in [0, 1), one a row (injected, as ``DeviceModel.sample_injected``); without them row r takes the uniform
     (``seed``, ``first_id`` + r, ``draw``) of the stream that ``DeviceModel.sample`` draws from, so a batch may be cut
-    anywhere.  ``live``: bool, rows that are False are not read (``SKIP``, 0).  A row with no token left gives
+    anywhere (what is captured into a graph keeps its seed and draw: replays that are to draw anew take ``uniforms``).  A row's token
+    comes with one value, whatever its uniform.  ``live``: bool, rows that are False are not read (``SKIP``, 0).  A row with no token left gives
     ``OUTSIDE`` and +inf."""
     code, _, rows, vocab, _, stride, shape = _rows(logits, 2)
     temperature = _temperature(temperature)
@@ -206,7 +209,8 @@ def logits_keys(ml2p: torch.Tensor, lengths: Optional[torch.Tensor] = None, *,
                 offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
     """-log2 p of whole passwords as float64 keys (what ``MonteCarloLib`` takes): the sums in 64 bits of their tokens'.
     Padded: ``ml2p`` [B, L] with ``lengths`` [B] (int32 or int64; None: L each).  Packed: ``ml2p`` [N] with ``offsets``
-    [B + 1] (int64, ascending).  A password with an impossible token is 1022.0, as everywhere in this package."""
+    [B + 1] (int64, ascending).  A password with an impossible token is 1022.0, as everywhere in this package, and no key is
+    below 0, whatever roundings the values hold: the rank indexes sort the bits of non-negative numbers."""
     if not ml2p.is_cuda:
         raise ValueError("ml2p: a tensor on the GPU is needed (there is no CPU fallback)")
     if ml2p.dtype != torch.float32:
