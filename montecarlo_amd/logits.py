@@ -182,8 +182,8 @@ def logits_draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *
     ``uniforms``: float64 in [0, 1), one a row (injected, as ``DeviceModel.sample_injected``); without them row r takes the uniform
     (``seed``, ``first_id`` + r, ``draw``) of the stream that ``DeviceModel.sample`` draws from, so a batch may be cut
     anywhere (what is captured into a graph keeps its seed and draw: replays that are to draw anew take ``uniforms``).  A row's token
-    comes with one value, whatever its uniform.  ``live``: bool, rows that are False are not read (``SKIP``, 0).  A row with no token left gives
-    ``OUTSIDE`` and +inf."""
+    comes with one value, whatever its uniform.  ``live``: bool, rows that are False are not read (``SKIP``, 0).  A row with no
+    token left gives ``OUTSIDE`` and +inf."""
     code, _, rows, vocab, _, stride, shape = _rows(logits, 2)
     temperature = _temperature(temperature)
     dev = logits.device
