@@ -1,8 +1,7 @@
 """Build libmi355mc.so (the C-ABI + HIP kernels) in-tree with hipcc for gfx950.
 
-hipcc cross-compiles without a GPU, so this runs in the build container; the
-built .so travels to the GPU box with the tree (it is git-ignored, not
-gpurun-ignored).  Usage:  python -m montecarlo_amd.build [--force] [--sanitize]
+hipcc cross-compiles without a GPU; the library is git-ignored and stays in
+the tree beside its sources.  Usage:  python -m montecarlo_amd.build [--force] [--sanitize]
 (--sanitize: the host-only sources under ASan + UBSan into libmi355mc_host_san.so, see build_sanitized)
 """
 from __future__ import annotations
@@ -67,8 +66,8 @@ def sanitizer_runtime() -> str:
 
 def build_sanitized(force: bool = False, verbose: bool = True) -> str:
     """The host-only part of the library (everything that parses caller-supplied text and dict shapes) under
-    AddressSanitizer + UndefinedBehaviorSanitizer, for tests/test_sanitized_host.py.  CPU code only: GPU
-    sanitizers are not available on this pool and nothing here touches the GPU."""
+    AddressSanitizer + UndefinedBehaviorSanitizer, for tests/test_sanitized_host.py.  CPU code only: nothing here
+    touches the GPU."""
     deps = [os.path.join(CSRC, s) for s in HOST_SOURCES] + HEADERS
     if not force and os.path.exists(HOST_SAN_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(HOST_SAN_LIB) for d in deps):
         return HOST_SAN_LIB
